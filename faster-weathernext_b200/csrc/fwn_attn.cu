@@ -18,6 +18,8 @@
 #include "attn_fwd_wide.cuh"
 #include "attn_bwd_wide.cuh"
 #include "gemm.cuh"
+#include "linear.cuh"
+#include "rms.cuh"
 #include "tiles.cuh"
 
 namespace {
@@ -624,6 +626,10 @@ fwn_status fwn_device_error(void* stream, int32_t* code) {
   if (e != cudaSuccess) return cuda_fail(e, "read device error word");
   e = cudaMemcpyToSymbol(fwn::g_device_error, &zero, sizeof(zero));
   if (e != cudaSuccess) return cuda_fail(e, "clear device error word");
+  unsigned int linear_word = 0;
+  e = fwn::take_linear_error(&linear_word);
+  if (e != cudaSuccess) return cuda_fail(e, "device error word (projections)");
+  word |= linear_word;
   *code = !word ? 0 : (word & 0x400u) ? FWN_ERR_INVALID_ARGUMENT : FWN_ERR_DEVICE_TIMEOUT;
   return ok();
 }
@@ -963,6 +969,402 @@ fwn_status fwn_gnn_ln_segment_sum(const void* m, const int32_t* seg_ptr, int64_t
   cudaError_t e = fwn::launch_ln_segment_sum(m, seg_ptr, n_out, f, gamma, beta, eps, norm, residual, out,
                                              out_dtype == FWN_DTYPE_BF16, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "ln_segment_sum");
+  return ok();
+}
+
+namespace {
+
+bool is_float_dtype(int32_t t) { return t == FWN_DTYPE_BF16 || t == FWN_DTYPE_F32; }
+int64_t dtype_size(int32_t t) { return t == FWN_DTYPE_F32 ? 4 : t == FWN_DTYPE_BF16 ? 2 : 1; }
+bool aligned_to(const void* p, int64_t a) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(a) == 0; }
+
+fwn_status check_rms(const fwn_rms_desc* d, bool residual, bool weight, bool bwd) {
+  if (!d) return fail(FWN_ERR_INVALID_ARGUMENT, "desc is null");
+  if (d->rows < 0 || d->d <= 0) return fail(FWN_ERR_INVALID_ARGUMENT, "bad rows=%lld or d=%d", static_cast<long long>(d->rows), d->d);
+  if (d->d > fwn::kRmsMaxWidth) return fail(FWN_ERR_UNSUPPORTED, "d=%d exceeds %d", d->d, fwn::kRmsMaxWidth);
+  if (d->rows > INT32_MAX) return fail(FWN_ERR_UNSUPPORTED, "rows=%lld exceeds 2^31 - 1", static_cast<long long>(d->rows));
+  if (d->flags & ~FWN_RMS_SCALE_ONLY) return fail(FWN_ERR_INVALID_ARGUMENT, "unknown flags %d", d->flags);
+  if (bwd && d->flags) return fail(FWN_ERR_UNSUPPORTED, "FWN_RMS_SCALE_ONLY has no backward");
+  if (!is_float_dtype(d->x_dtype) || (residual && !is_float_dtype(d->residual_dtype)) ||
+      (weight && !is_float_dtype(d->weight_dtype)))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "x, residual and weight are bf16 or float32");
+  if (!is_float_dtype(d->out_dtype) && (bwd || d->out_dtype != FWN_DTYPE_E4M3))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "unknown out dtype %d", d->out_dtype);
+  if (!(d->flags & FWN_RMS_SCALE_ONLY) && !(d->eps >= 0.f)) return fail(FWN_ERR_INVALID_ARGUMENT, "eps must not be negative");
+  if (d->rows > 1 && (d->x_stride < d->d || (residual && d->residual_stride < d->d)))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "row strides must be at least d");
+  return FWN_OK;
+}
+
+// Whether a [rows, d] tensor's rows allow 8 values per access: 32 bytes of float32, 16 of bf16, 8 of e4m3.
+bool wide_rows(const void* p, int32_t dtype, int64_t stride, int64_t rows) {
+  const int64_t bytes = 8 * dtype_size(dtype);
+  return p == nullptr || (aligned_to(p, bytes) && (rows <= 1 || stride % 8 == 0));
+}
+
+}  // namespace
+
+fwn_status fwn_rms_norm(const fwn_rms_desc* desc, const void* x, const void* residual, const void* weight, void* x_out,
+                        void* out, float* scale, void* stream) {
+  fwn_status s = check_rms(desc, residual != nullptr, weight != nullptr, false);
+  if (s != FWN_OK) return s;
+  const fwn_rms_desc& d = *desc;
+  if (d.rows == 0) return ok();
+  if (!x || !out) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
+  if ((residual != nullptr) != (x_out != nullptr)) return fail(FWN_ERR_INVALID_ARGUMENT, "residual and x_out come together");
+  if ((d.out_dtype == FWN_DTYPE_E4M3) != (scale != nullptr))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "scale goes with an E4M3 output, and with that alone");
+  fwn::RmsParams p{};
+  p.x = x;
+  p.residual = residual;
+  p.weight = weight;
+  p.x_out = x_out;
+  p.out = out;
+  p.scale = scale;
+  p.rows = d.rows;
+  p.x_stride = d.x_stride;
+  p.residual_stride = d.residual_stride;
+  p.d = d.d;
+  p.eps = d.eps;
+  p.out_type = d.out_dtype == FWN_DTYPE_BF16 ? fwn::kRmsBf16 : d.out_dtype == FWN_DTYPE_F32 ? fwn::kRmsF32 : fwn::kRmsE4m3;
+  p.x_bf16 = d.x_dtype == FWN_DTYPE_BF16;
+  p.residual_bf16 = d.residual_dtype == FWN_DTYPE_BF16;
+  p.weight_bf16 = d.weight_dtype == FWN_DTYPE_BF16;
+  p.normalize = !(d.flags & FWN_RMS_SCALE_ONLY);
+  p.wide = d.d % 8 == 0 && wide_rows(x, d.x_dtype, d.x_stride, d.rows) &&
+           wide_rows(residual, d.residual_dtype, d.residual_stride, d.rows) && wide_rows(x_out, d.x_dtype, d.d, d.rows) &&
+           wide_rows(out, d.out_dtype, d.d, d.rows) && (!weight || aligned16(weight));
+  cudaError_t e = fwn::launch_rms_norm(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rms_norm");
+  return ok();
+}
+
+fwn_status fwn_rms_norm_bwd_workspace_size(const fwn_rms_desc* desc, size_t* bytes) {
+  if (!bytes) return fail(FWN_ERR_INVALID_ARGUMENT, "bytes is null");
+  fwn_status s = check_rms(desc, false, false, true);
+  if (s != FWN_OK) return s;
+  *bytes = static_cast<size_t>(fwn::rms_bwd_blocks(desc->rows, desc->d, num_sms())) * desc->d * sizeof(float);
+  if (*bytes < 16) *bytes = 16;
+  return ok();
+}
+
+fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, const void* residual, const void* weight,
+                            const void* dh, const void* ds, void* dx, void* d_residual, void* d_weight, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  fwn_status s = check_rms(desc, residual != nullptr, weight != nullptr, true);
+  if (s != FWN_OK) return s;
+  if (d_residual && !is_float_dtype(desc->residual_dtype))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "d_residual is bf16 or float32");
+  const fwn_rms_desc& d = *desc;
+  if (d.rows > 0 && (!x || !dh)) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
+  if (d_weight && !weight) return fail(FWN_ERR_INVALID_ARGUMENT, "d_weight needs weight");
+  if (d_weight) {
+    size_t need = 0;
+    if ((s = fwn_rms_norm_bwd_workspace_size(desc, &need)) != FWN_OK) return s;
+    if (!workspace || workspace_bytes < need || !aligned16(workspace))
+      return fail(FWN_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed", need);
+  }
+  if (d.rows == 0 && !d_weight) return ok();
+  fwn::RmsBwdParams p{};
+  p.x = x;
+  p.residual = residual;
+  p.weight = weight;
+  p.dh = dh;
+  p.ds = ds;
+  p.dx = dx;
+  p.dr = d_residual;
+  p.part = d_weight ? static_cast<float*>(workspace) : nullptr;
+  p.dw = d_weight;
+  p.rows = d.rows;
+  p.x_stride = d.x_stride;
+  p.residual_stride = d.residual_stride;
+  p.d = d.d;
+  p.eps = d.eps;
+  p.x_bf16 = d.x_dtype == FWN_DTYPE_BF16;
+  p.residual_bf16 = d.residual_dtype == FWN_DTYPE_BF16;
+  p.weight_bf16 = d.weight_dtype == FWN_DTYPE_BF16;
+  p.dh_bf16 = d.out_dtype == FWN_DTYPE_BF16;
+  p.dw_bf16 = p.weight_bf16;
+  p.wide = d.d % 8 == 0 && wide_rows(x, d.x_dtype, d.x_stride, d.rows) &&
+           wide_rows(residual, d.residual_dtype, d.residual_stride, d.rows) && wide_rows(dh, d.out_dtype, d.d, d.rows) &&
+           wide_rows(ds, d.x_dtype, d.d, d.rows) && wide_rows(dx, d.x_dtype, d.d, d.rows) &&
+           wide_rows(d_residual, d.residual_dtype, d.d, d.rows) && (!weight || aligned16(weight));
+  cudaError_t e = fwn::launch_rms_norm_bwd(p, fwn::rms_bwd_blocks(d.rows, d.d, num_sms()), static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "rms_norm_bwd");
+  return ok();
+}
+
+namespace {
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// 2D map over `outer` rows of `inner` contiguous elements, row stride ld (elements), with a box of 128 bytes (128-byte
+// swizzle) or 64 bytes (64-byte swizzle) by box_rows.
+fwn_status make_map_ld(CUtensorMap* map, const void* base, int32_t dtype, int64_t inner, int64_t outer, int64_t ld,
+                       int box_bytes, int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(FWN_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
+  const int64_t es = dtype_size(dtype);
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(outer > 1 ? ld * es : round_up(inner * es, 16))};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(box_bytes / es), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, dtype == FWN_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : dtype == FWN_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                   2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FWN_ERR_INVALID_ARGUMENT, "cuTensorMapEncodeTiled (ld) failed (%d)", static_cast<int>(r));
+  return FWN_OK;
+}
+
+// Whether TMA can address `outer` rows of stride ld at p.
+bool tma_rows(const void* p, int32_t dtype, int64_t outer, int64_t ld) {
+  return aligned16(p) && (outer <= 1 || ld * dtype_size(dtype) % 16 == 0);
+}
+
+fwn_status check_linear(const fwn_linear_desc* d) {
+  if (!d) return fail(FWN_ERR_INVALID_ARGUMENT, "desc is null");
+  if (d->m < 0 || d->n <= 0 || d->k <= 0)
+    return fail(FWN_ERR_INVALID_ARGUMENT, "bad shape m=%lld n=%d k=%d", static_cast<long long>(d->m), d->n, d->k);
+  if (d->m > INT32_MAX - 1024) return fail(FWN_ERR_UNSUPPORTED, "m=%lld too large", static_cast<long long>(d->m));
+  if (d->n > INT32_MAX - 1024 || d->k > INT32_MAX - 1024)
+    return fail(FWN_ERR_UNSUPPORTED, "n=%d or k=%d too large", d->n, d->k);
+  if (d->dtype != FWN_DTYPE_BF16 && d->dtype != FWN_DTYPE_E4M3)
+    return fail(FWN_ERR_INVALID_ARGUMENT, "operands are bf16 or e4m3 (got dtype %d)", d->dtype);
+  if (!is_float_dtype(d->out_dtype) || !is_float_dtype(d->bias_dtype) || !is_float_dtype(d->x_dtype))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "out, bias and x are bf16 or float32");
+  if (d->act != FWN_ACT_NONE && d->act != FWN_ACT_GELU_TANH && d->act != FWN_ACT_SWISH)
+    return fail(FWN_ERR_INVALID_ARGUMENT, "unknown activation %d", d->act);
+  if (d->flags & ~(FWN_LINEAR_A_M_CONTIGUOUS | FWN_LINEAR_B_N_CONTIGUOUS | FWN_LINEAR_PRE_GRAD))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "unknown flags %d", d->flags);
+  const bool a_mn = d->flags & FWN_LINEAR_A_M_CONTIGUOUS, b_mn = d->flags & FWN_LINEAR_B_N_CONTIGUOUS;
+  if (d->dtype == FWN_DTYPE_E4M3 && (a_mn || b_mn))
+    return fail(FWN_ERR_UNSUPPORTED, "e4m3 operands have k contiguous");
+  if (d->flags & FWN_LINEAR_PRE_GRAD) {
+    if (d->dtype != FWN_DTYPE_BF16 || d->out_dtype != FWN_DTYPE_BF16 || d->act == FWN_ACT_NONE)
+      return fail(FWN_ERR_UNSUPPORTED, "FWN_LINEAR_PRE_GRAD takes bf16 operands, an activation and a bf16 output");
+  }
+  if ((d->m > 1 && (d->ldo < d->n || (!a_mn && d->lda < d->k))) || (a_mn && d->k > 1 && d->lda < d->m) ||
+      (!b_mn && d->n > 1 && d->ldb < d->k) || (b_mn && d->k > 1 && d->ldb < d->n))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "a row stride is below its row's length");
+  return FWN_OK;
+}
+
+struct LinearPlan {
+  bool rows, rows_wide;      // few rows: linear_rows_kernel
+  bool pack_a, pack_b;       // operand rows that TMA cannot address are copied once
+  int64_t lda, ldb;          // as the kernel reads them
+  int tile, splits;
+  size_t off_b, off_part, off_sum, bytes;
+};
+
+// Time model of the tensor-core kernel, in units of 0.01 us: a stage (128 bytes of k) of a tile's MMAs, and a tile's
+// epilogue, which overlaps the next tile's MMAs; a split product adds a launch and its parts' way through L2.
+LinearPlan plan_linear(const fwn_linear_desc& d, const void* a, const void* b, int sms) {
+  LinearPlan pl{};
+  const int64_t es = dtype_size(d.dtype);
+  const bool a_mn = d.flags & FWN_LINEAR_A_M_CONTIGUOUS, b_mn = d.flags & FWN_LINEAR_B_N_CONTIGUOUS;
+  const bool pre = d.flags & FWN_LINEAR_PRE_GRAD;
+  pl.lda = d.lda;
+  pl.ldb = d.ldb;
+  pl.rows = d.m <= fwn::kLinearRowsMax && !a_mn && !b_mn && !pre;
+  if (pl.rows) {
+    pl.rows_wide = d.k * es % 16 == 0 && tma_rows(a, d.dtype, d.m, d.lda) && tma_rows(b, d.dtype, d.n, d.ldb);
+    return pl;
+  }
+  const int64_t a_outer = a_mn ? d.k : d.m, a_inner = a_mn ? d.m : d.k;
+  const int64_t b_outer = b_mn ? d.k : d.n, b_inner = b_mn ? d.n : d.k;
+  pl.pack_a = !tma_rows(a, d.dtype, a_outer, d.lda);
+  pl.pack_b = !tma_rows(b, d.dtype, b_outer, d.ldb);
+  size_t at = 0;
+  if (pl.pack_a) {
+    pl.lda = round_up(a_inner, 16 / es);
+    at += static_cast<size_t>(round_up(a_outer * pl.lda * es, 256));
+  }
+  pl.off_b = at;
+  if (pl.pack_b) {
+    pl.ldb = round_up(b_inner, 16 / es);
+    at += static_cast<size_t>(round_up(b_outer * pl.ldb * es, 256));
+  }
+  const int64_t kb = (d.k * es + 127) / 128;
+  const int stage[3] = {29, 19, 15}, epilogue[3] = {200, 120, 80};
+  int64_t best = INT64_MAX;
+  for (int t = 0; t < 3; ++t) {
+    const int64_t tiles = ((d.m + fwn::linear_tile_m(t) - 1) / fwn::linear_tile_m(t)) *
+                          ((d.n + fwn::linear_tile_n(t) - 1) / fwn::linear_tile_n(t));
+    const int64_t slots = t == fwn::kTile256 ? sms / 2 : sms;
+    for (int64_t s = 1; s <= 16 && s <= (kb + 3) / 4; ++s) {
+      if (s > 1 && (pre || tiles * s > 4 * slots)) break;
+      const int64_t waves = (tiles * s + slots - 1) / slots, mine = (kb + s - 1) / s * stage[t];
+      int64_t cost = waves * std::max<int64_t>(mine, epilogue[t]) + epilogue[t];
+      if (s > 1) cost += 300 + static_cast<int64_t>(8.0 * s * d.m * d.n / 5e4);
+      if (cost < best) {
+        best = cost;
+        pl.tile = t;
+        pl.splits = static_cast<int>(s);
+      }
+    }
+  }
+  pl.off_part = at;
+  if (pl.splits > 1)
+    at += static_cast<size_t>(pl.splits) * round_up(d.m, fwn::linear_tile_m(pl.tile)) * round_up(d.n, 4) * sizeof(float);
+  pl.off_sum = at;
+  if (pre) at += static_cast<size_t>((d.m + 31) / 32) * d.n * sizeof(float);
+  pl.bytes = at;
+  return pl;
+}
+
+}  // namespace
+
+fwn_status fwn_linear_workspace_size(const fwn_linear_desc* desc, const void* a, const void* b, size_t* bytes) {
+  if (!bytes) return fail(FWN_ERR_INVALID_ARGUMENT, "bytes is null");
+  fwn_status s = check_linear(desc);
+  if (s != FWN_OK) return s;
+  *bytes = desc->m == 0 ? 0 : plan_linear(*desc, a, b, num_sms()).bytes;
+  return ok();
+}
+
+fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const float* a_scale, const void* b,
+                      const float* b_scale, const void* bias, const void* x, void* out, void* d_bias, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  fwn_status s = check_linear(desc);
+  if (s != FWN_OK) return s;
+  const fwn_linear_desc& d = *desc;
+  const bool pre = d.flags & FWN_LINEAR_PRE_GRAD, fp8 = d.dtype == FWN_DTYPE_E4M3;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (d_bias && (!pre || !bias)) return fail(FWN_ERR_INVALID_ARGUMENT, "d_bias goes with FWN_LINEAR_PRE_GRAD and a bias");
+  if (d.m == 0) {
+    if (d_bias) {
+      cudaError_t e = cudaMemsetAsync(d_bias, 0, static_cast<size_t>(d.n) * dtype_size(d.bias_dtype), st);
+      if (e != cudaSuccess) return cuda_fail(e, "clear d_bias");
+    }
+    return ok();
+  }
+  if (!a || !b || !out) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
+  if (fp8 != (a_scale != nullptr) || fp8 != (b_scale != nullptr))
+    return fail(FWN_ERR_INVALID_ARGUMENT, "e4m3 operands come with a_scale and b_scale, bf16 ones without");
+  if (pre && !x) return fail(FWN_ERR_INVALID_ARGUMENT, "FWN_LINEAR_PRE_GRAD needs the gradient of the output");
+  if (x && !pre && d.x_dtype != d.out_dtype) return fail(FWN_ERR_UNSUPPORTED, "the residual has the output's type");
+  if (x && d.m > 1 && d.ldx < d.n) return fail(FWN_ERR_INVALID_ARGUMENT, "ldx is below n");
+  const int sms = num_sms();
+  const LinearPlan pl = plan_linear(d, a, b, sms);
+  if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned_to(workspace, 256)))
+    return fail(FWN_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) needed", pl.bytes);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  fwn::LinearParams p{};
+  p.bias = bias;
+  p.a_scale = a_scale;
+  p.b_scale = b_scale;
+  p.x = x;
+  p.out = out;
+  p.m = d.m;
+  p.ldx = d.ldx;
+  p.ldo = d.ldo;
+  p.n = d.n;
+  p.k = d.k;
+  p.act = d.act == FWN_ACT_GELU_TANH ? 1 : d.act == FWN_ACT_SWISH ? 2 : 0;
+  p.bias_bf16 = d.bias_dtype == FWN_DTYPE_BF16;
+  p.x_f32 = d.x_dtype == FWN_DTYPE_F32;
+  p.out_f32 = d.out_dtype == FWN_DTYPE_F32;
+  p.pre_grad = pre;
+  p.fp8 = fp8;
+  p.a_mn = d.flags & FWN_LINEAR_A_M_CONTIGUOUS;
+  p.b_mn = d.flags & FWN_LINEAR_B_N_CONTIGUOUS;
+  p.splits = 1;
+  cudaError_t e;
+  if (pl.rows) {
+    e = fwn::launch_linear_rows(a, d.lda, b, d.ldb, pl.rows_wide, p, st);
+    if (e != cudaSuccess) return cuda_fail(e, "linear_rows");
+    return ok();
+  }
+  const int es = static_cast<int>(dtype_size(d.dtype));
+  const int64_t a_outer = p.a_mn ? d.k : d.m, a_inner = p.a_mn ? d.m : d.k;
+  const int64_t b_outer = p.b_mn ? d.k : d.n, b_inner = p.b_mn ? d.n : d.k;
+  if (pl.pack_a) {
+    if ((e = fwn::launch_pack_rows(a, d.lda, ws, pl.lda, a_outer, a_inner, es, st)) != cudaSuccess)
+      return cuda_fail(e, "pack a");
+    a = ws;
+  }
+  if (pl.pack_b) {
+    if ((e = fwn::launch_pack_rows(b, d.ldb, ws + pl.off_b, pl.ldb, b_outer, b_inner, es, st)) != cudaSuccess)
+      return cuda_fail(e, "pack b");
+    b = ws + pl.off_b;
+  }
+  const int tm = fwn::linear_tile_m(pl.tile), tn = fwn::linear_tile_n(pl.tile);
+  p.m_tiles = static_cast<int>((d.m + tm - 1) / tm);
+  p.n_tiles = (d.n + tn - 1) / tn;
+  p.splits = pl.splits;
+  p.k_blocks = static_cast<int>((static_cast<int64_t>(d.k) * es + 127) / 128);
+  const int64_t items = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
+  if (items > INT32_MAX - 1024) return fail(FWN_ERR_UNSUPPORTED, "m=%lld n=%d too large", static_cast<long long>(d.m), d.n);
+  p.items = static_cast<int>(items);
+  CUtensorMap ta, tb, tx, to;
+  if ((s = make_map_ld(&ta, a, d.dtype, a_inner, a_outer, pl.lda, 128, p.a_mn ? 64 : 128)) != FWN_OK) return s;
+  if ((s = make_map_ld(&tb, b, d.dtype, b_inner, b_outer, pl.ldb, 128, p.b_mn ? 64 : fwn::linear_box_n(pl.tile))) != FWN_OK)
+    return s;
+  tx = to = ta;
+  if (p.splits > 1) {
+    // Parts in float32, then their sum with the epilogue.
+    const int64_t ldp = round_up(d.n, 4);
+    float* part = reinterpret_cast<float*>(ws + pl.off_part);
+    p.split_rows = static_cast<int64_t>(p.m_tiles) * tm;
+    if (p.split_rows * p.splits > INT32_MAX) return fail(FWN_ERR_UNSUPPORTED, "m=%lld too large", static_cast<long long>(d.m));
+    if ((s = make_map_ld(&to, part, FWN_DTYPE_F32, d.n, p.split_rows * p.splits, ldp, 128, 32)) != FWN_OK) return s;
+    fwn::LinearParams q = p;
+    q.bias = q.x = nullptr;
+    q.a_scale = q.b_scale = nullptr;
+    q.act = 0;
+    q.out = part;
+    q.ldo = ldp;
+    q.out_f32 = true;
+    if ((e = fwn::launch_linear_tiles(pl.tile, ta, tb, tx, to, q, sms, st)) != cudaSuccess) return cuda_fail(e, "linear");
+    if ((e = fwn::launch_linear_split_sum(part, ldp, p, st)) != cudaSuccess) return cuda_fail(e, "linear split sum");
+    return ok();
+  }
+  p.out_direct = !tma_rows(out, d.out_dtype, d.m, d.ldo);
+  if (!p.out_direct &&
+      (s = make_map_ld(&to, out, d.out_dtype, d.n, d.m, d.ldo, p.out_f32 ? 128 : 64, 32)) != FWN_OK)
+    return s;
+  if (x) {
+    p.x_direct = !tma_rows(x, d.x_dtype, d.m, d.ldx);
+    if (!p.x_direct && (s = make_map_ld(&tx, x, d.x_dtype, d.n, d.m, d.ldx, p.x_f32 ? 128 : 64, 32)) != FWN_OK) return s;
+  }
+  if (d_bias) p.colsum = reinterpret_cast<float*>(ws + pl.off_sum);
+  if ((e = fwn::launch_linear_tiles(pl.tile, ta, tb, tx, to, p, sms, st)) != cudaSuccess) return cuda_fail(e, "linear");
+  if (d_bias && (e = fwn::launch_column_sum(p.colsum, (d.m + 31) / 32, d.n, d_bias, p.bias_bf16, st)) != cudaSuccess)
+    return cuda_fail(e, "column sums");
+  return ok();
+}
+
+fwn_status fwn_linear_grad_cast_workspace_size(int64_t m, int32_t n, size_t* bytes) {
+  if (!bytes) return fail(FWN_ERR_INVALID_ARGUMENT, "bytes is null");
+  if (m < 0 || n <= 0) return fail(FWN_ERR_INVALID_ARGUMENT, "bad shape m=%lld n=%d", static_cast<long long>(m), n);
+  *bytes = static_cast<size_t>(fwn::grad_cast_blocks(m, n, num_sms())) * n * sizeof(float);
+  return ok();
+}
+
+fwn_status fwn_linear_grad_cast(const void* dy, int32_t dtype, int64_t ldy, int64_t m, int32_t n, void* cast, int64_t ldc,
+                                void* d_bias, int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (m < 0 || n <= 0 || m > INT32_MAX) return fail(FWN_ERR_INVALID_ARGUMENT, "bad shape m=%lld n=%d", static_cast<long long>(m), n);
+  if (!is_float_dtype(dtype) || !is_float_dtype(bias_dtype)) return fail(FWN_ERR_INVALID_ARGUMENT, "dy and d_bias are bf16 or float32");
+  if (m > 1 && (ldy < n || (cast && ldc < n))) return fail(FWN_ERR_INVALID_ARGUMENT, "a row stride is below n");
+  if (m > 0 && !dy) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!cast && !d_bias) return ok();
+  size_t need = 0;
+  fwn_linear_grad_cast_workspace_size(m, n, &need);
+  if (d_bias && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(FWN_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed", need);
+  const int blocks = fwn::grad_cast_blocks(m, n, num_sms());
+  const bool wide = n % 8 == 0 && tma_rows(dy, dtype, m, ldy) && (!cast || tma_rows(cast, FWN_DTYPE_BF16, m, ldc));
+  float* part = d_bias ? static_cast<float*>(workspace) : nullptr;
+  cudaError_t e = fwn::launch_grad_cast(dy, dtype == FWN_DTYPE_F32, ldy, m, n, cast, ldc, part, blocks, wide,
+                                        static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "grad_cast");
+  if (d_bias && (e = fwn::launch_column_sum(part, blocks, n, d_bias, bias_dtype == FWN_DTYPE_BF16,
+                                            static_cast<cudaStream_t>(stream))) != cudaSuccess)
+    return cuda_fail(e, "column sums");
   return ok();
 }
 

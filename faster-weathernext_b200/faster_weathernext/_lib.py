@@ -19,6 +19,7 @@ FWN_ERR_NO_DEVICE = 6
 
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+DTYPE_E4M3 = 2
 MODE_BF16 = 0
 MODE_TF32 = 1
 MODE_TF32X3 = 2
@@ -28,6 +29,10 @@ ACT_GELU_TANH = 1
 ACT_SWISH = 2
 ACT_GELU_TANH_AUX = 3
 ACT_GELU_TANH_GRAD = 4
+RMS_SCALE_ONLY = 1
+LINEAR_A_M_CONTIGUOUS = 1
+LINEAR_B_N_CONTIGUOUS = 2
+LINEAR_PRE_GRAD = 4
 
 # Every symbol include/fwn_attn.h declares.
 SYMBOLS = ("fwn_version", "fwn_last_error_string", "fwn_device_error", "fwn_lse_rows",
@@ -37,7 +42,9 @@ SYMBOLS = ("fwn_version", "fwn_last_error_string", "fwn_device_error", "fwn_lse_
            "fwn_bitset_words", "fwn_khop_bitset", "fwn_walk_bitset", "fwn_bitset_csr_count", "fwn_bitset_csr_fill",
            "fwn_cond_layernorm", "fwn_cond_layernorm_scatter", "fwn_cond_layernorm_residual",
            "fwn_cond_layernorm_add", "fwn_cond_layernorm_bwd_workspace", "fwn_cond_layernorm_bwd",
-           "fwn_gemm_bf16", "fwn_gemm_bf16_aux", "fwn_gemm_bf16_gather", "fwn_gnn_gather_add_act", "fwn_gnn_ln_segment_sum", "fwn_test_attn_fwd_timeout")
+           "fwn_gemm_bf16", "fwn_gemm_bf16_aux", "fwn_gemm_bf16_gather", "fwn_gnn_gather_add_act", "fwn_gnn_ln_segment_sum",
+           "fwn_rms_norm", "fwn_rms_norm_bwd_workspace_size", "fwn_rms_norm_bwd", "fwn_linear_workspace_size", "fwn_linear",
+           "fwn_linear_grad_cast_workspace_size", "fwn_linear_grad_cast", "fwn_test_attn_fwd_timeout")
 
 
 class AttnDesc(ctypes.Structure):
@@ -53,6 +60,20 @@ class TileList(ctypes.Structure):
   _fields_ = [("ptr", ctypes.c_void_p), ("kb", ctypes.c_void_p), ("bits", ctypes.c_void_p),
               ("n_blocks", ctypes.c_int32), ("n_tiles", ctypes.c_int32), ("block_rows", ctypes.c_int32),
               ("n_cols", ctypes.c_int32), ("cols", ctypes.c_void_p)]
+
+
+class RmsDesc(ctypes.Structure):
+  _fields_ = [("rows", ctypes.c_int64), ("d", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+              ("residual_dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
+              ("flags", ctypes.c_int32), ("eps", ctypes.c_float), ("reserved", ctypes.c_int32),
+              ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64)]
+
+
+class LinearDesc(ctypes.Structure):
+  _fields_ = [("m", ctypes.c_int64), ("n", ctypes.c_int32), ("k", ctypes.c_int32), ("dtype", ctypes.c_int32),
+              ("out_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+              ("act", ctypes.c_int32), ("flags", ctypes.c_int32), ("lda", ctypes.c_int64), ("ldb", ctypes.c_int64),
+              ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64)]
 
 
 class FwnError(RuntimeError):
@@ -99,6 +120,13 @@ def _declare(lib):
                                _I, _P],
       "fwn_gnn_gather_add_act": [_P, _P, _P, _P, _P, _P, ctypes.c_int64, _I, _I, _P, _P],
       "fwn_gnn_ln_segment_sum": [_P, _P, ctypes.c_int64, _I, _P, _P, ctypes.c_float, ctypes.c_float, _P, _P, _I, _P],
+      "fwn_rms_norm": [ctypes.POINTER(RmsDesc), _P, _P, _P, _P, _P, _P, _P],
+      "fwn_rms_norm_bwd_workspace_size": [ctypes.POINTER(RmsDesc), ctypes.POINTER(_SZ)],
+      "fwn_rms_norm_bwd": [ctypes.POINTER(RmsDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+      "fwn_linear_workspace_size": [ctypes.POINTER(LinearDesc), _P, _P, ctypes.POINTER(_SZ)],
+      "fwn_linear": [ctypes.POINTER(LinearDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+      "fwn_linear_grad_cast_workspace_size": [ctypes.c_int64, _I, ctypes.POINTER(_SZ)],
+      "fwn_linear_grad_cast": [_P, _I, ctypes.c_int64, ctypes.c_int64, _I, _P, ctypes.c_int64, _P, _I, _P, _SZ, _P],
       "fwn_bitset_csr_count": [_P, _I, _I, _P, _P, _SZ, _P],
       "fwn_bitset_csr_fill": [_P, _I, _I, _P, _P, _P],
       "fwn_attn_fwd": [ctypes.POINTER(AttnDesc), _P, _P, _P, ctypes.POINTER(TileList), _P, _P, _P],

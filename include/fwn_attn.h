@@ -53,7 +53,9 @@ typedef enum fwn_status {
   FWN_ERR_NO_DEVICE = 6         /* no sm_100 device is current */
 } fwn_status;
 
-typedef enum fwn_dtype { FWN_DTYPE_BF16 = 0, FWN_DTYPE_F32 = 1 } fwn_dtype;
+/* FWN_DTYPE_E4M3 (8-bit floats, 4 exponent and 3 mantissa bits, largest value 448): the RMS norm's 8-bit output and the
+ * 8-bit projection's operands only. */
+typedef enum fwn_dtype { FWN_DTYPE_BF16 = 0, FWN_DTYPE_F32 = 1, FWN_DTYPE_E4M3 = 2 } fwn_dtype;
 
 /* Arithmetic of the attention MMAs. BF16 takes bf16 tensors; TF32 and TF32X3 take float32 tensors.
  * TF32 <-> the reference's default precision (DotAlgorithmPreset.TF32_TF32_F32, pallas_attn.py:342);
@@ -269,6 +271,93 @@ FWN_API fwn_status fwn_gemm_bf16_aux(const void* a, const void* bt, const void* 
 FWN_API fwn_status fwn_gemm_bf16_gather(const void* a, const void* bt, const void* bias, void* c, const void* add0,
                                         const int32_t* idx0, int64_t rows0, const void* add1, const int32_t* idx1,
                                         int64_t rows1, int64_t m, int32_t n, int32_t k, int32_t act, void* stream);
+
+/* ---- pre-norm projections ------------------------------------------------------------------------------------
+ * No counterpart in the reference (its blocks use LayerNorm and plain projections, src/faster_weathernext/patch.py:
+ * 165-177, 238-252); the RMS form of the same sub-blocks, in bf16 for training and forecasts and in 8 bits for forecasts.
+ *
+ * Root-mean-square norm: s = x + residual (or x), h = s / sqrt(mean(s^2) + eps) * weight over rows of d values.
+ * Every tensor has its last dimension contiguous; x and residual have a row stride in elements, the outputs are
+ * contiguous and do not overlap the inputs. d up to 16,384; any alignment of whole elements (rows whose addresses and
+ * width allow it, 32 bytes and multiples of 8, move in wide accesses). */
+typedef struct fwn_rms_desc {
+  int64_t rows;
+  int32_t d;
+  int32_t x_dtype;         /* FWN_DTYPE_BF16 or FWN_DTYPE_F32: x, x_out, ds, dx */
+  int32_t residual_dtype;  /* residual, d_residual (read with a residual only) */
+  int32_t weight_dtype;    /* weight, d_weight */
+  int32_t out_dtype;       /* out: BF16, F32 or E4M3; dh (BF16 or F32) */
+  int32_t flags;           /* fwn_rms_flags */
+  float eps;
+  int32_t reserved;        /* 0 */
+  int64_t x_stride;
+  int64_t residual_stride;
+} fwn_rms_desc;
+
+/* FWN_RMS_SCALE_ONLY: no norm, h = s * weight: the rows of a tensor brought to 8 bits (eps is not read). */
+typedef enum fwn_rms_flags { FWN_RMS_SCALE_ONLY = 1 } fwn_rms_flags;
+
+/* Forward. weight [d] or NULL; residual NULL: s = x, x_out not written; else x_out [rows, d] receives s (rounded to
+ * x_dtype; h is computed from the unrounded s). out_dtype E4M3: scale [rows] receives max |h| / 448 per row and out the
+ * values h / scale, rounded to nearest even; a row whose max |h| is below 2^-100 gets scale 0 and values 0, one with a
+ * NaN a NaN scale. */
+FWN_API fwn_status fwn_rms_norm(const fwn_rms_desc* desc, const void* x, const void* residual, const void* weight,
+                                void* x_out, void* out, float* scale, void* stream);
+
+/* Backward. dh [rows, d] in out_dtype, the gradient of h; ds [rows, d] in x_dtype, the gradient of x_out (NULL: none).
+ * With g = dh weight and rstd = 1 / sqrt(mean(s^2) + eps):
+ *   dx = rstd g - s rstd^3 mean(g s) + ds,  d_residual = dx,  d_weight = sum over rows of dh s rstd (fixed order).
+ * x, residual: the forward's inputs, or x = the forward's x_out with residual = NULL. dx, d_residual, d_weight may be
+ * NULL (not computed). d_weight needs a workspace of fwn_rms_norm_bwd_workspace_size bytes, 16-byte aligned. */
+FWN_API fwn_status fwn_rms_norm_bwd_workspace_size(const fwn_rms_desc* desc, size_t* bytes);
+FWN_API fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, const void* residual, const void* weight,
+                                    const void* dh, const void* ds, void* dx, void* d_residual, void* d_weight,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Projection with bias, activation and residual in its epilogue: out[m, n] = act(a[m, k] b[n, k]^T + bias) + x, any
+ * m, n, k >= 1 (m = 0 does nothing); float32 accumulation on the tensor cores. Operands bf16, or e4m3 with one float32
+ * scale per row of a and of b (the product's element (i, j) is multiplied by a_scale[i] b_scale[j]). Either operand may
+ * be given with its other dimension contiguous (bf16). x, the residual, has the output's type. Rows whose stride or base
+ * is not a multiple of 16 bytes are allowed everywhere (such operands are copied into the workspace first). out
+ * overlaps no input. FWN_ACT_NONE, FWN_ACT_GELU_TANH or FWN_ACT_SWISH.
+ *
+ * FWN_LINEAR_PRE_GRAD: the backward's first step, out = x act'(a b^T + bias) in bf16 with x = the gradient of the
+ * forward's output ([m, n], bf16 or float32): the gradient of the pre-activation, which is computed again here rather
+ * than kept. d_bias (NULL, or [n] in bias_dtype) receives its column sums, taken in float32 before the rounding, in a
+ * fixed order. The gradients of a and b are products of the same kind with out as an operand. */
+typedef struct fwn_linear_desc {
+  int64_t m;
+  int32_t n;
+  int32_t k;
+  int32_t dtype;       /* operands: FWN_DTYPE_BF16 or FWN_DTYPE_E4M3 */
+  int32_t out_dtype;   /* BF16 or F32 */
+  int32_t bias_dtype;  /* BF16 or F32 */
+  int32_t x_dtype;     /* BF16 or F32 */
+  int32_t act;         /* fwn_act */
+  int32_t flags;       /* fwn_linear_flags */
+  int64_t lda;         /* row strides in elements: a [m, k] (or [k, m]) */
+  int64_t ldb;         /* b [n, k] (or [k, n]) */
+  int64_t ldx;
+  int64_t ldo;
+} fwn_linear_desc;
+typedef enum fwn_linear_flags {
+  FWN_LINEAR_A_M_CONTIGUOUS = 1, /* a is stored [k, m] */
+  FWN_LINEAR_B_N_CONTIGUOUS = 2, /* b is stored [k, n] */
+  FWN_LINEAR_PRE_GRAD = 4
+} fwn_linear_flags;
+
+/* Workspace of the call with these operands (their addresses matter, not their contents); 256-byte aligned. */
+FWN_API fwn_status fwn_linear_workspace_size(const fwn_linear_desc* desc, const void* a, const void* b, size_t* bytes);
+FWN_API fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const float* a_scale, const void* b,
+                              const float* b_scale, const void* bias, const void* x, void* out, void* d_bias,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* The backward's first step without an activation: cast (bf16 [m, n], row stride ldc, or NULL) = dy rounded, d_bias
+ * ([n] in bias_dtype, or NULL) = the column sums of dy (float32, fixed order). Workspace for d_bias, 16-byte aligned. */
+FWN_API fwn_status fwn_linear_grad_cast_workspace_size(int64_t m, int32_t n, size_t* bytes);
+FWN_API fwn_status fwn_linear_grad_cast(const void* dy, int32_t dtype, int64_t ldy, int64_t m, int32_t n, void* cast,
+                                        int64_t ldc, void* d_bias, int32_t bias_dtype, void* workspace,
+                                        size_t workspace_bytes, void* stream);
 
 /* ---- grid <-> mesh interaction networks -------------------------------------------------------------------
  * The blocked GNNs of the encoder / decoder (src/faster_weathernext/patch.py:347-509, ChunkedDeepGNN: edge MLP on
