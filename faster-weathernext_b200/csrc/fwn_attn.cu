@@ -1189,12 +1189,12 @@ LinearPlan plan_linear(const fwn_linear_desc& d, const void* a, const void* b, i
     at += static_cast<size_t>(round_up(b_outer * pl.ldb * es, 256));
   }
   const int64_t kb = (d.k * es + 127) / 128;
-  const int stage[3] = {29, 19, 15}, epilogue[3] = {200, 120, 80};
+  const int stage[fwn::kLinearTiles] = {29, 19, 15}, epilogue[fwn::kLinearTiles] = {200, 120, 80};
   int64_t best = INT64_MAX;
-  for (int t = 0; t < 3; ++t) {
+  for (int t = 0; t < fwn::kLinearTiles; ++t) {
     const int64_t tiles = ((d.m + fwn::linear_tile_m(t) - 1) / fwn::linear_tile_m(t)) *
                           ((d.n + fwn::linear_tile_n(t) - 1) / fwn::linear_tile_n(t));
-    const int64_t slots = t == fwn::kTile256 ? sms / 2 : sms;
+    const int64_t slots = fwn::linear_pair(t) ? sms / 2 : sms;
     for (int64_t s = 1; s <= 16 && s <= (kb + 3) / 4; ++s) {
       if (s > 1 && (pre || tiles * s > 4 * slots)) break;
       const int64_t waves = (tiles * s + slots - 1) / slots, mine = (kb + s - 1) / s * stage[t];
@@ -1297,6 +1297,7 @@ fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const float* a
   p.n_tiles = (d.n + tn - 1) / tn;
   p.splits = pl.splits;
   p.k_blocks = static_cast<int>((static_cast<int64_t>(d.k) * es + 127) / 128);
+  p.chunk = p.out_f32 ? fwn::kLinearChunk : p.k_blocks;
   const int64_t items = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
   if (items > INT32_MAX - 1024) return fail(FWN_ERR_UNSUPPORTED, "m=%lld n=%d too large", static_cast<long long>(d.m), d.n);
   p.items = static_cast<int>(items);
@@ -1323,13 +1324,16 @@ fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const float* a
     if ((e = fwn::launch_linear_split_sum(part, ldp, p, st)) != cudaSuccess) return cuda_fail(e, "linear split sum");
     return ok();
   }
+  const int cols = fwn::linear_chunk_cols(pl.tile, p.out_f32 || (x && p.x_f32));
   p.out_direct = !tma_rows(out, d.out_dtype, d.m, d.ldo);
   if (!p.out_direct &&
-      (s = make_map_ld(&to, out, d.out_dtype, d.n, d.m, d.ldo, p.out_f32 ? 128 : 64, 32)) != FWN_OK)
+      (s = make_map_ld(&to, out, d.out_dtype, d.n, d.m, d.ldo, cols * static_cast<int>(dtype_size(d.out_dtype)), 32)) != FWN_OK)
     return s;
   if (x) {
     p.x_direct = !tma_rows(x, d.x_dtype, d.m, d.ldx);
-    if (!p.x_direct && (s = make_map_ld(&tx, x, d.x_dtype, d.n, d.m, d.ldx, p.x_f32 ? 128 : 64, 32)) != FWN_OK) return s;
+    if (!p.x_direct &&
+        (s = make_map_ld(&tx, x, d.x_dtype, d.n, d.m, d.ldx, cols * static_cast<int>(dtype_size(d.x_dtype)), 32)) != FWN_OK)
+      return s;
   }
   if (d_bias) p.colsum = reinterpret_cast<float*>(ws + pl.off_sum);
   if ((e = fwn::launch_linear_tiles(pl.tile, ta, tb, tx, to, p, sms, st)) != cudaSuccess) return cuda_fail(e, "linear");

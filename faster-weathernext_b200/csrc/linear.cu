@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "linear.cuh"
@@ -37,8 +38,10 @@ __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+// No cluster-scope release: it orders tensor-memory reads, which tcgen05.fence has ordered before it, and took 1,000
+// cycles behind the thread's outstanding stores.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // Tile load; CG = 2: the barrier may be the pair's other CTA's (its bytes count there).
 template <int CG>
@@ -118,72 +121,159 @@ __device__ __forceinline__ float rcp(float x) {
 
 constexpr float kGeluC0 = 0.7978845608028654f, kGeluC1 = 0.044715f, kLog2e = 1.4426950408889634f;
 
-// -log2(e) times the logistic function's argument: GELU in its tanh form is x sigma(2 u), u = c0 (x + c1 x^3); swish is
-// x sigma(x). Written through sigma both keep their relative precision where they are small.
+// GELU in its tanh form is x sigma(2 u), u = c0 (x + c1 x^3), swish x sigma(x): written through the logistic function
+// sigma(z) = 1 / (1 + 2^-z') both keep their relative precision where they are small, which 1 + tanh does not.
+// Coefficients of z' = -z log2(e) = x (p0 + p1 x^2).
 template <int ACT>
-__device__ __forceinline__ float neg_arg(float x) {
-  if constexpr (ACT == 1) return (-2.f * kLog2e * kGeluC0) * fmaf(kGeluC1 * x, x * x, x);
-  return -kLog2e * x;
-}
+struct Logistic {
+  static constexpr float p0 = ACT == 1 ? -2.f * kLog2e * kGeluC0 : -kLog2e;
+  static constexpr float p1 = ACT == 1 ? p0 * kGeluC1 : 0.f;
+  // dz/dx = q0 + q1 x^2
+  static constexpr float q0 = ACT == 1 ? 2.f * kGeluC0 : 1.f, q1 = ACT == 1 ? 3.f * kGeluC1 * q0 : 0.f;
+  // Below `low` 2^z' passes 2^30: there the value is taken as that at `low` (-5e-9, for swish -2e-8) and so is the slope
+  // (-5e-8, for swish -2e-8); above `high` the slope is 1 to float32's last bit.
+  static constexpr float low = ACT == 1 ? -5.5f : -20.5f, high = ACT == 1 ? 10.f : 40.f;
+};
+// One value, to float32 precision over the whole range.
 template <int ACT>
 __device__ __forceinline__ float activate(float x) {
   if constexpr (ACT == 0) return x;
-  return x * rcp(1.f + ex2(neg_arg<ACT>(x)));
+  using L = Logistic<ACT>;
+  const float z = ACT == 1 ? x * fmaf(L::p1 * x, x, L::p0) : x * L::p0;
+  return x * rcp(1.f + ex2(z));
 }
-// d/dx: sigma + x sigma (1 - sigma) z', z' = 2 c0 (1 + 3 c1 x^2) or 1. x is clamped to where the slope has long reached
-// 0 or 1, and the exponent below overflow, so that the products stay finite.
-template <int ACT>
-__device__ __forceinline__ float activate_grad(float x) {
-  if constexpr (ACT == 0) return 1.f;
-  constexpr float kMost = ACT == 1 ? 30.f : 100.f;
-  const float xc = x != x ? x : fminf(fmaxf(x, -kMost), kMost);
-  const float e = ex2(fminf(neg_arg<ACT>(xc), 100.f));
-  const float s = rcp(1.f + e);
-  const float z1 = ACT == 1 ? 2.f * kGeluC0 * fmaf(3.f * kGeluC1 * xc, xc, 1.f) : 1.f;
-  const float r = fmaf(xc * s * z1, e * s, s);
-  return x != x ? x : r;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 pair(float a) { return make_float2(a, a); }
+// Four values for a bf16 result. The special-function unit, not the FP32 pipe, bounds an epilogue of two calls a value
+// (4,096 cycles for a 128 x 256 tile, as long as its MMAs at k = 512): the four denominators 1 + 2^z' (each at most 2^31,
+// so that their product stays in float32) share one reciprocal, 1.25 calls a value, and the rest runs in pairs.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ void activate4(float* v) {
+  using L = Logistic<ACT>;
+  float2 x[2], d[2], e[2], xx[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    x[i] = make_float2(max_nan(v[2 * i], L::low), max_nan(v[2 * i + 1], L::low));
+    if constexpr (SLOPE) x[i] = make_float2(min_nan(x[i].x, L::high), min_nan(x[i].y, L::high));
+    float2 z;
+    if constexpr (ACT == 1) {
+      xx[i] = fmul2(x[i], x[i]);
+      z = fmul2(x[i], ffma2(xx[i], pair(L::p1), pair(L::p0)));
+    } else {
+      z = fmul2(x[i], pair(L::p0));
+    }
+    e[i] = make_float2(ex2(z.x), ex2(z.y));
+    d[i] = fadd2(e[i], pair(1.f));
+  }
+  const float2 m = fmul2(d[0], d[1]);
+  const float r = rcp(m.x * m.y);
+  const float2 n = fmul2(pair(r), make_float2(m.y, m.x));  // 1 / (d0 d2), 1 / (d1 d3)
+  const float2 s[2] = {fmul2(n, d[1]), fmul2(n, d[0])};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float2 y;
+    if constexpr (SLOPE) {
+      // sigma + x sigma (1 - sigma) z_x = sigma (1 + (1 - sigma) x z_x), 1 - sigma = 2^z' sigma
+      const float2 w = ACT == 1 ? fmul2(x[i], ffma2(xx[i], pair(L::q1), pair(L::q0))) : x[i];
+      y = fmul2(s[i], ffma2(fmul2(e[i], s[i]), w, pair(1.f)));
+    } else {
+      y = fmul2(x[i], s[i]);
+    }
+    v[2 * i] = y.x;
+    v[2 * i + 1] = y.y;
+  }
 }
 
 // ---- tensor-core kernel --------------------------------------------------------------------------------------------
 
 // Persistent; a CTA (CG = 1) or a pair of CTAs on two SMs (CG = 2) takes output tiles of 128 CG x BN, walked with n
 // fastest so that the tiles in flight share their rows of a in L2. Warps:
-//   0      TMA producer: 128 bytes of k (64 bf16, 128 e4m3) of 128 rows of a and of BN / CG rows of b per stage (with
-//          m or n contiguous: 64 rows of k by 64 columns, one box per 64);
+//   0      TMA producer of a: 128 bytes of k (64 bf16, 128 e4m3) of 128 rows (b: BN / CG rows) per stage, or, with m
+//          (n) contiguous, 64 rows of k by 64 columns, one box per 64;
 //   1      MMA issuer (CG = 2: of the pair's first CTA, for both), into one of two TMEM accumulators;
-//   2-9    epilogue: warp w reads TMEM lanes 32 (w % 4) + [0, 32) (rows) and one half of the tile's columns, 32 at a
-//          time; the residual (or dy) chunk of 32 x 32 arrives by TMA in a slot of the warp's own, the result replaces
-//          it there and leaves by TMA, so that a tile's epilogue overlaps the next tile's MMAs.
+//   2      the same producer for b (one lane issues a load in about 200 cycles; two loads a stage held the MMAs);
+//   3      idle (it completes the warpgroup whose registers the epilogue takes);
+//   4-11   epilogue: warp w reads TMEM lanes 32 (w % 4) + [0, 32) (rows) and one half of the tile's columns, CC at a
+//          time (128 bytes of a row); the residual (or dy) chunk arrives by TMA one chunk ahead, the result leaves by
+//          TMA, and a tile's epilogue overlaps the next tile's MMAs.
 // Ragged edges: TMA fills rows and columns past the tensors with zeros and clips stores. Why a pair on 256 x 256: per
 // 64 of k an SM then takes in 32 KB for 512 cycles of MMA, half the L2 traffic per FLOP of 128 x 128 and two thirds of
-// 128 x 256, which held that form at 1.14 PFLOP/s. The small tiles spread products of few rows over the SMs.
-template <int TILE, bool F32>
+// 128 x 256. The small tiles spread products of few rows over the SMs. Why chunks of 128-byte rows: a TMA store of 32
+// rows took about 200 cycles whether its rows had 64 bytes or 128, which held a 163,848 x 2,048 bf16 result to 226 us.
+//
+// float32 results: the tensor core truncates its running sum at every step, an error that grows with k (measured 1.5e-6
+// of the result at k = 2,048). They take k in chunks (p.chunk stages) into alternate accumulators, which the epilogue
+// warps add in float32 registers (128 a thread: the epilogue warpgroups run with 224 registers).
+template <int TILE, bool X32, bool O32, bool PRE, bool SUM>
 struct LinearCfg {
-  static constexpr int CG = TILE == kTile256 ? 2 : 1;
+  static constexpr int CG = linear_pair(TILE) ? 2 : 1;
   static constexpr int BN = linear_tile_n(TILE);
   static constexpr int BNC = BN / CG;                    // rows of b per CTA
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BNC * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int HC = BN / 2, NCH = HC / 32;       // columns and chunks of an epilogue warp
-  static constexpr int SLOT = F32 ? 4096 : 2048;         // one 32 x 32 chunk (float32 if x or the output is)
-  static constexpr int NSLOT = F32 ? 2 : 3;
-  static constexpr int NS = TILE == kTile64 ? 6 : F32 ? 4 : 5;
+  static constexpr int HC = BN / 2;                      // columns of an epilogue warp
+  static constexpr int CC = linear_chunk_cols(TILE, X32 || O32);
+  static constexpr int NCH = HC / CC;
+  static constexpr int X_ROW = CC * (X32 ? 4 : 2), O_ROW = CC * (O32 ? 4 : 2);  // bytes: 128 or 64
+  static constexpr int SLOT = 32 * (X_ROW > O_ROW ? X_ROW : O_ROW);
+  static constexpr int NS = STAGE == 24576 ? (PRE ? 4 : 6) : PRE ? 3 : 4;
   static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int THREADS = 320;
-  static constexpr int N_BAR = 2 * NS + 4 + 1 + 8 * NSLOT;
-  static constexpr int OFF_SLOT = NS * STAGE;
-  static constexpr int OFF_VEC = OFF_SLOT + 8 * NSLOT * SLOT;  // per epilogue warp: HC biases and HC scales
+  static constexpr int THREADS = 384;
+  static constexpr int N_BAR = 2 * NS + 4 + 1 + 8;
+  static constexpr int OFF_SLOT = NS * STAGE;            // per epilogue warp: x (or a second output), output
+  static constexpr int OFF_RED = OFF_SLOT + 8 * 2 * SLOT;      // PRE: 32 x 32 float32 per warp, for the column sums
+  static constexpr int OFF_VEC = OFF_RED + (PRE ? 8 * 4096 : 0);  // per epilogue warp: HC biases and HC scales
   static constexpr int OFF_BAR = OFF_VEC + 8 * 2 * HC * 4;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16 + 1024;
+  static_assert(OFF_SLOT % 1024 == 0 && SLOT % 1024 == 0 && OFF_RED % 1024 == 0, "swizzle atoms");
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
 };
 
-// Offset of column c (0..31) of row r in a 32 x 32 chunk: rows of 64 (bf16, 64-byte swizzle) or 128 bytes (float32).
-template <bool F32>
-__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-  if constexpr (F32) return sw128_offset(r, c >> 2) + ((c & 3) << 2);
-  return sw64_offset(r, c >> 3) + ((c & 7) << 1);
+// Offset of 16-byte piece i of row r in a chunk of ROW-byte rows (128-byte or 64-byte swizzle), and of one byte in it.
+template <int ROW>
+__device__ __forceinline__ uint32_t piece_at(int r, int i) {
+  if constexpr (ROW == 128) return sw128_offset(r, i);
+  return sw64_offset(r, i);
 }
+template <int ROW>
+__device__ __forceinline__ uint32_t byte_at(int r, int b) { return piece_at<ROW>(r, b >> 4) + (b & 15); }
+// The tiles of a CTA (pair), n fastest, then m, then the splits of k; the step's parts come from the host, so that the
+// walk divides once (a division of 64 bits per tile held the MMA warp for 1,000 cycles).
+struct TileWalk {
+  int t, nt, mt, sp;
+  __device__ __forceinline__ TileWalk(const LinearParams& p, int first) : t(first) {
+    nt = first % p.n_tiles;
+    const int r = first / p.n_tiles;
+    mt = r % p.m_tiles;
+    sp = r / p.m_tiles;
+  }
+  __device__ __forceinline__ void next(const LinearParams& p, int step) {
+    t += step;
+    nt += p.step_n;
+    mt += p.step_m;
+    sp += p.step_s;
+    if (nt >= p.n_tiles) {
+      nt -= p.n_tiles;
+      ++mt;
+    }
+    if (mt >= p.m_tiles) {
+      mt -= p.m_tiles;
+      ++sp;
+    }
+  }
+  __device__ __forceinline__ int kb0(const LinearParams& p) const { return sp * p.kb_q + min(sp, p.kb_r); }
+  __device__ __forceinline__ int kb1(const LinearParams& p) const { return kb0(p) + p.kb_q + (sp < p.kb_r ? 1 : 0); }
+};
+
 __device__ __forceinline__ void st_shared_u16(uint32_t a, uint16_t v) {
   asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(v) : "memory");
 }
@@ -196,12 +286,14 @@ __device__ __forceinline__ uint16_t ld_shared_u16(uint32_t a) {
   return v;
 }
 
-template <int TILE, int ACT, bool X32, bool O32, bool PRE>
-__global__ void __maxnreg__(168)
+// 12 warps of 168 registers fill the register file; the epilogue's eight take 224 and leave 56 to the others:
+// 128 x 56 + 256 x 224 = 64,512 = 384 x 168.
+template <int TILE, int ACT, bool X32, bool O32, bool PRE, bool SUM>
+__global__ void __launch_bounds__(384, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                        const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_o,
                        const LinearParams p) {
-  using C = LinearCfg<TILE, X32 || O32>;
+  using C = LinearCfg<TILE, X32, O32, PRE, SUM>;
   constexpr int CG = C::CG;
   extern __shared__ uint8_t smem_linear[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_linear) + 1023) & ~uintptr_t(1023));
@@ -214,7 +306,7 @@ __global__ void __maxnreg__(168)
   auto acc_full = [&](int b) { return bar0 + 8 * (2 * C::NS + b); };
   auto acc_empty = [&](int b) { return bar0 + 8 * (2 * C::NS + 2 + b); };
   const uint32_t drain = bar0 + 8 * (2 * C::NS + 4);
-  auto slot_bar = [&](int w, int s) { return bar0 + 8 * (2 * C::NS + 5 + w * C::NSLOT + s); };
+  auto x_bar = [&](int w) { return bar0 + 8 * (2 * C::NS + 5 + w); };
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::OFF_BAR + C::N_BAR * 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_BAR + C::N_BAR * 8 + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -231,7 +323,7 @@ __global__ void __maxnreg__(168)
       mbar_init(acc_empty(b), 8 * CG);
     }
     mbar_init(drain, 1);
-    for (int i = 0; i < 8 * C::NSLOT; ++i) mbar_init(slot_bar(0, i), 1);
+    for (int w = 0; w < 8; ++w) mbar_init(x_bar(w), 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -249,31 +341,31 @@ __global__ void __maxnreg__(168)
   const uint32_t tmem = *tmem_holder;
   const int bk = p.fp8 ? 128 : 64;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer
-    // CG = 2: both CTAs' bytes count on the first CTA's barrier, whose producer expects them.
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------------ TMA producers (a: warp 0, b: warp 2)
+    // CG = 2: both CTAs' bytes count on the first CTA's barrier, whose warp 0 expects them.
+    const bool is_a = warp == 0;
+    const bool mn = is_a ? p.a_mn : p.b_mn;
+    const CUtensorMap* tm = is_a ? &tm_a : &tm_b;
+    const int base = is_a ? rank * 128 : rank * C::BNC, boxes = is_a ? 2 : C::BNC / 64;
     uint32_t g = 0;
     bool ok = true;
-    for (int t = first; t < p.items && ok; t += step) {
-      const int split = t / (p.m_tiles * p.n_tiles), mn = t % (p.m_tiles * p.n_tiles);
-      const int m0 = (mn / p.n_tiles) * 128 * CG + rank * 128, n0 = (mn % p.n_tiles) * C::BN + rank * C::BNC;
-      const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * split / p.splits);
-      const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (split + 1) / p.splits);
-      for (int kb = kb0; kb < kb1; ++kb, ++g) {
+    for (TileWalk w(p, first); w.t < p.items && ok; w.next(p, step)) {
+      const int at = (is_a ? w.mt * 128 * CG : w.nt * C::BN) + base;
+      const int kb1 = w.kb1(p);
+      for (int kb = w.kb0(p); kb < kb1; ++kb, ++g) {
         const int st = g % C::NS;
-        if (!(ok = mbar_wait(empty(st), ((g / C::NS) & 1) ^ 1, abort_flag))) break;
-        if (lane == 0) {
-          if (rank == 0) mbar_arrive_expect_tx(full(st), CG * C::STAGE);
-          const uint32_t bar = CG == 2 ? map_to(full(st), 0) : full(st);
-          if (p.a_mn) {
-            for (int i = 0; i < 2; ++i) tile_load<CG>(a_st(st) + i * 8192, &tm_a, m0 + 64 * i, kb * bk, bar);
+        if (!(ok = warp_wait(empty(st), ((g / C::NS) & 1) ^ 1, abort_flag))) break;
+        const uint32_t bar = CG == 2 ? map_to(full(st), 0) : full(st);
+        const uint32_t dst = is_a ? a_st(st) : b_st(st);
+        if (elect_one_sync()) {
+          if (is_a && rank == 0) mbar_arrive_expect_tx(full(st), CG * C::STAGE);
+          if (mn) {
+            for (int i = 0; i < boxes; ++i) tile_load<CG>(dst + i * 8192, tm, at + 64 * i, kb * bk, bar);
           } else {
-            tile_load<CG>(a_st(st), &tm_a, kb * bk, m0, bar);
-          }
-          if (p.b_mn) {
-            for (int i = 0; i < C::BNC / 64; ++i) tile_load<CG>(b_st(st) + i * 8192, &tm_b, n0 + 64 * i, kb * bk, bar);
-          } else {
-            tile_load<CG>(b_st(st), &tm_b, kb * bk, n0, bar);
+            tile_load<CG>(dst, tm, kb * bk, at, bar);
           }
         }
         __syncwarp();
@@ -283,7 +375,7 @@ __global__ void __maxnreg__(168)
     volatile int never = 0;
     if (ok) {
       for (uint32_t i = (g >= C::NS ? g - C::NS : 0); i < g; ++i) {
-        if (!mbar_wait(empty(i % C::NS), (i / C::NS) & 1, abort_flag)) break;
+        if (!warp_wait(empty(i % C::NS), (i / C::NS) & 1, abort_flag)) break;
       }
     } else if (rank == 0) {
       // Gave up: the copies in flight land before TMEM and shared memory are released (bounded, abort flag ignored).
@@ -301,15 +393,21 @@ __global__ void __maxnreg__(168)
       const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
       uint32_t g = 0, acc_i = 0;
       bool ok = true;
-      for (int t = first; t < p.items && ok; t += step, ++acc_i) {
-        const int split = t / (p.m_tiles * p.n_tiles);
-        const int kb0 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * split / p.splits);
-        const int kb1 = static_cast<int>(static_cast<int64_t>(p.k_blocks) * (split + 1) / p.splits);
-        const int buf = acc_i & 1;
-        if (!(ok = warp_wait(acc_empty(buf), ((acc_i >> 1) & 1) ^ 1, abort_flag))) break;
-        tc_fence_after();
-        const uint32_t d = tmem + buf * C::BN;
+      for (TileWalk w(p, first); w.t < p.items && ok; w.next(p, step)) {
+        const int kb0 = w.kb0(p), kb1 = w.kb1(p);
+        int buf = 0, left = 0;  // stages until the accumulator is handed over
+        uint32_t d = 0;
         for (int kb = kb0; kb < kb1; ++kb, ++g) {
+          const bool begin = left == 0;
+          if (begin) {
+            left = SUM ? min(p.chunk, kb1 - kb) : kb1 - kb;
+            buf = acc_i & 1;
+            if (!(ok = warp_wait(acc_empty(buf), ((acc_i >> 1) & 1) ^ 1, abort_flag))) break;
+            tc_fence_after();
+            d = tmem + buf * C::BN;
+            ++acc_i;
+          }
+          --left;
           const int st = g % C::NS;
           if (!(ok = warp_wait(full(st), (g / C::NS) & 1, abort_flag))) break;
           tc_fence_after();
@@ -317,14 +415,14 @@ __global__ void __maxnreg__(168)
           if (elect_one_sync()) {
             if (p.fp8) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) mma<CG, true>(d, ad + 2 * i, bd + 2 * i, idesc, (kb > kb0 || i > 0) ? 1u : 0u);
+              for (int i = 0; i < 4; ++i) mma<CG, true>(d, ad + 2 * i, bd + 2 * i, idesc, (!begin || i > 0) ? 1u : 0u);
             } else {
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                mma<CG, false>(d, ad + i * ka, bd + i * kbs, idesc, (kb > kb0 || i > 0) ? 1u : 0u);
+                mma<CG, false>(d, ad + i * ka, bd + i * kbs, idesc, (!begin || i > 0) ? 1u : 0u);
             }
             commit<CG>(empty(st));
-            if (kb == kb1 - 1) commit<CG>(acc_full(buf));
+            if (left == 0) commit<CG>(acc_full(buf));
           }
           __syncwarp();
         }
@@ -339,224 +437,285 @@ __global__ void __maxnreg__(168)
       volatile int never = 0;
       mbar_wait(drain, 0, &never);
     }
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     // ------------------------------------------------------------------ epilogue
-    const int ew = warp - 2, quarter = warp & 3, half = ew >> 2;
+    const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
+    constexpr int CC = C::CC;
     const uint32_t trow = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * C::HC;
-    const uint32_t slots = sbase + C::OFF_SLOT + ew * C::NSLOT * C::SLOT;
+    const uint32_t x_slot = sbase + C::OFF_SLOT + ew * 2 * C::SLOT, o_slot = x_slot + C::SLOT;
     float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC) + ew * 2 * C::HC;
     const uint32_t vec_s = smem_u32(vec);
     const bool has_x = p.x != nullptr;
     const bool x_tma = has_x && !p.x_direct;
-    const uint32_t my_items = p.items > first ? (p.items - first + step - 1) / step : 0;
-    const uint32_t chunks = my_items * C::NCH;
-    // First row and column of chunk q of this warp (its item's tile, the warp's half and quarter).
-    auto place = [&](uint32_t q, int64_t& row, int& col) {
-      const int t = first + static_cast<int>(q / C::NCH) * step;
-      const int mn = t % (p.m_tiles * p.n_tiles);
-      row = static_cast<int64_t>(mn / p.n_tiles) * 128 * CG + rank * 128 + quarter * 32;
-      col = (mn % p.n_tiles) * C::BN + half * C::HC + static_cast<int>(q % C::NCH) * 32;
+    // One lane issues all of a warp's copies (elect.sync: from uniform registers), so its waits cover its stores.
+    auto issue_x = [&](const TileWalk& w, int ch) {  // the residual (dy) of chunk ch of a tile into the slot
+      mbar_arrive_expect_tx(x_bar(ew), 32 * C::X_ROW);
+      tile_load<1>(x_slot, &tm_x, w.nt * C::BN + half * C::HC + ch * CC, w.mt * 128 * CG + rank * 128 + quarter * 32, x_bar(ew));
     };
-    auto issue_x = [&](uint32_t q) {  // lane 0: chunk q's residual (dy) into its slot
-      if (q >= chunks) return;
-      int64_t row;
-      int col;
-      place(q, row, col);
-      const int s = q % C::NSLOT;
-      mbar_arrive_expect_tx(slot_bar(ew, s), 32 * 32 * (X32 ? 4 : 2));
-      tile_load<1>(slots + s * C::SLOT, &tm_x, col, static_cast<int>(row), slot_bar(ew, s));
+    // Biases and scales of this warp's half of a tile's columns, HC / 32 a lane, read a tile ahead.
+    float next_bias[C::HC / 32], next_scale[C::HC / 32];
+    auto fetch_vec = [&](const TileWalk& w) {
+#pragma unroll
+      for (int i = 0; i < C::HC / 32; ++i) {
+        const int c = w.nt * C::BN + half * C::HC + 32 * i + lane;
+        next_bias[i] = 0.f;
+        next_scale[i] = 1.f;
+        if (w.t < p.items && c < p.n) {
+          if (p.bias != nullptr)
+            next_bias[i] = p.bias_bf16 ? __bfloat162float(static_cast<const bf16*>(p.bias)[c])
+                                       : static_cast<const float*>(p.bias)[c];
+          if (p.b_scale != nullptr) next_scale[i] = p.b_scale[c];
+        }
+      }
     };
-    uint32_t issued = 0;
-    if (x_tma) {
-      if (lane == 0)
-        for (int i = 0; i < C::NSLOT; ++i) issue_x(i);
-      issued = C::NSLOT;
-    }
+    auto release = [&](int buf) {  // this warp has read the accumulator: the MMAs may overwrite it
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2) mbar_arrive_cluster(map_to(acc_empty(buf), 0)); else mbar_arrive(acc_empty(buf));
+      }
+    };
+    float rs = 1.f;  // this row's scale
+    // N accumulated values of this lane's row, from column `at` of the warp's half: scales, bias, activation (its slope).
+    auto scaled = [&](float* v, int at, auto n) {
+      constexpr int N = decltype(n)::value;
+      if (p.b_scale != nullptr) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+          const float4 c = ld_shared_f32x4(vec_s + (C::HC + at + 4 * i) * 4);
+          v[4 * i] *= rs * c.x;
+          v[4 * i + 1] *= rs * c.y;
+          v[4 * i + 2] *= rs * c.z;
+          v[4 * i + 3] *= rs * c.w;
+        }
+      }
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+          const float4 b = ld_shared_f32x4(vec_s + (at + 4 * i) * 4);
+          v[4 * i] += b.x;
+          v[4 * i + 1] += b.y;
+          v[4 * i + 2] += b.z;
+          v[4 * i + 3] += b.w;
+        }
+      }
+      if constexpr (ACT != 0) {
+        if constexpr (O32) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[i] = activate<ACT>(v[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N / 4; ++i) activate4<ACT, PRE>(v + 4 * i);
+        }
+      }
+    };
+    TileWalk w(p, first);
+    if (x_tma && elect_one_sync()) issue_x(w, 0);
+    __syncwarp();
+    fetch_vec(w);
     uint32_t q = 0, acc_i = 0;
     bool ok = true;
-    for (int t = first; t < p.items && ok; t += step, ++acc_i) {
-      const int split = t / (p.m_tiles * p.n_tiles), mn = t % (p.m_tiles * p.n_tiles);
-      const int buf = acc_i & 1;
-      const int64_t row0 = static_cast<int64_t>(mn / p.n_tiles) * 128 * CG + rank * 128 + quarter * 32;
-      const int col0 = (mn % p.n_tiles) * C::BN + half * C::HC;
+    while (w.t < p.items) {
+      TileWalk after = w;
+      after.next(p, step);
+      const int64_t row0 = static_cast<int64_t>(w.mt) * 128 * CG + rank * 128 + quarter * 32;
+      const int col0 = w.nt * C::BN + half * C::HC;
       __syncwarp();  // the previous tile's reads of vec
 #pragma unroll
-      for (int j = lane; j < C::HC; j += 32) {
-        const int c = col0 + j;
-        float b = 0.f, s = 1.f;
-        if (c < p.n) {
-          if (p.bias != nullptr)
-            b = p.bias_bf16 ? __bfloat162float(static_cast<const bf16*>(p.bias)[c]) : static_cast<const float*>(p.bias)[c];
-          if (p.b_scale != nullptr) s = p.b_scale[c];
-        }
-        vec[j] = b;
-        vec[C::HC + j] = s;
+      for (int i = 0; i < C::HC / 32; ++i) {
+        vec[32 * i + lane] = next_bias[i];
+        vec[C::HC + 32 * i + lane] = next_scale[i];
       }
-      float rs = 1.f;
+      fetch_vec(after);
+      rs = 1.f;
       if (p.a_scale != nullptr && row0 + lane < p.m) rs = p.a_scale[row0 + lane];
       __syncwarp();
-      if (!(ok = warp_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) break;
-      tc_fence_after();
-#pragma unroll 1
+      int buf = acc_i & 1;
+      float sum[SUM ? C::HC : 1];
+      float v[SUM ? 1 : 2][SUM ? 32 : CC];  // a chunk in work and the next one on its way from TMEM
+      auto fetch = [&](int ch) {
+        if constexpr (!SUM) {
+#pragma unroll
+          for (int j = 0; j < CC; j += 32)
+            tmem_ld32(trow + buf * C::BN + CC * ch + j, *reinterpret_cast<float(*)[32]>(v[ch & 1] + j));
+        }
+      };
+      if constexpr (SUM) {
+#pragma unroll
+        for (int i = 0; i < C::HC; ++i) sum[i] = 0.f;
+        const int kb1 = w.kb1(p);
+        for (int kb = w.kb0(p); kb < kb1; kb += p.chunk, ++acc_i) {
+          buf = acc_i & 1;
+          if (!(ok = warp_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < C::HC; j += 32) {
+            tmem_ld32(trow + buf * C::BN + j, *reinterpret_cast<float(*)[32]>(v[0]));
+            tmem_wait_ld();
+            reg_fence(*reinterpret_cast<float(*)[32]>(v[0]));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[j + i] += v[0][i];
+          }
+          release(buf);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < C::HC; j += 32) scaled(sum + j, j, std::integral_constant<int, 32>());
+      } else {
+        if (!(ok = warp_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        ++acc_i;
+        fetch(0);
+      }
+#pragma unroll
       for (int ch = 0; ch < C::NCH; ++ch, ++q) {
-        const int s = q % C::NSLOT;
-        const uint32_t slot = slots + s * C::SLOT;
-        const int col = col0 + 32 * ch;
-        float v[32];
-        tmem_ld32(trow + buf * C::BN + 32 * ch, v);
+        const int col = col0 + CC * ch;
+        float* val = SUM ? sum + (SUM ? CC * ch : 0) : v[SUM ? 0 : ch & 1];
+        uint32_t xr[X32 ? CC : CC / 2];  // this lane's row of x
         if (has_x) {
           if (x_tma) {
-            if (!(ok = warp_wait(slot_bar(ew, s), (q / C::NSLOT) & 1, abort_flag))) break;
+            if (!(ok = warp_wait(x_bar(ew), q & 1, abort_flag))) goto done;
           } else {
-            if (lane == 0) store_wait_read<C::NSLOT - 1>();
-            __syncwarp();
-            // Rows that TMA cannot address: lane = column, so that a row's 32 values are one access.
-#pragma unroll 8
+            // Rows that TMA cannot address: lane = column, so that a row's values are one access.
+#pragma unroll(SUM ? 2 : 8)
             for (int r = 0; r < 32; ++r) {
-              const bool in = row0 + r < p.m && col + lane < p.n;
-              const int64_t at = (row0 + r) * p.ldx + col + lane;
-              if constexpr (X32)
-                st_shared_u32(slot + chunk_at<true>(r, lane), in ? static_cast<const uint32_t*>(p.x)[at] : 0u);
-              else
-                st_shared_u16(slot + chunk_at<false>(r, lane), in ? static_cast<const uint16_t*>(p.x)[at] : uint16_t(0));
-            }
-            __syncwarp();
-          }
-        } else {
-          if (lane == 0) store_wait_read<C::NSLOT - 1>();
-          __syncwarp();
-        }
-        tmem_wait_ld();
-        reg_fence(v);
-        if (ch == C::NCH - 1) {
-          // The accumulator has been read: the next tile but one may overwrite it.
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 2) mbar_arrive_cluster(map_to(acc_empty(buf), 0)); else mbar_arrive(acc_empty(buf));
-          }
-        }
-        if (p.b_scale != nullptr) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 c = ld_shared_f32x4(vec_s + (C::HC + 32 * ch + 4 * i) * 4);
-            v[4 * i] *= rs * c.x;
-            v[4 * i + 1] *= rs * c.y;
-            v[4 * i + 2] *= rs * c.z;
-            v[4 * i + 3] *= rs * c.w;
-          }
-        }
-        if (p.bias != nullptr) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 b = ld_shared_f32x4(vec_s + (32 * ch + 4 * i) * 4);
-            v[4 * i] += b.x;
-            v[4 * i + 1] += b.y;
-            v[4 * i + 2] += b.z;
-            v[4 * i + 3] += b.w;
-          }
-        }
-        if constexpr (!PRE) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
-        }
-        // x: the residual is added; dy is multiplied by the activation's slope.
-        if (has_x) {
-          auto take = [&](int i, float x) { v[i] = PRE ? x * activate_grad<ACT>(v[i]) : v[i] + x; };
-          if constexpr (X32) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float4 f = ld_shared_f32x4(slot + sw128_offset(lane, i));
-              take(4 * i, f.x);
-              take(4 * i + 1, f.y);
-              take(4 * i + 2, f.z);
-              take(4 * i + 3, f.w);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint4 u = ld_shared_u32x4(slot + sw64_offset(lane, i));
-              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
-                take(8 * i + 2 * e, f.x);
-                take(8 * i + 2 * e + 1, f.y);
+              for (int j = lane; j < CC; j += 32) {
+                const bool in = row0 + r < p.m && col + j < p.n;
+                const int64_t at = (row0 + r) * p.ldx + col + j;
+                if constexpr (X32)
+                  st_shared_u32(x_slot + byte_at<C::X_ROW>(r, 4 * j), in ? static_cast<const uint32_t*>(p.x)[at] : 0u);
+                else
+                  st_shared_u16(x_slot + byte_at<C::X_ROW>(r, 2 * j), in ? static_cast<const uint16_t*>(p.x)[at] : uint16_t(0));
               }
             }
+            __syncwarp();
           }
-          __syncwarp();  // every lane has read the chunk before any writes it
+#pragma unroll
+          for (int i = 0; i < C::X_ROW / 16; ++i) {
+            const uint4 u = ld_shared_u32x4(x_slot + piece_at<C::X_ROW>(lane, i));
+            xr[4 * i] = u.x;
+            xr[4 * i + 1] = u.y;
+            xr[4 * i + 2] = u.z;
+            xr[4 * i + 3] = u.w;
+          }
+          // The slot has been read by every lane, and the proxy fence orders those reads before the copy that overwrites it
+          // (without it loads were still on their way when the next chunk landed): the next chunk's.
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (x_tma && (ch + 1 < C::NCH || after.t < p.items)) {
+            if (elect_one_sync()) {
+              if (ch + 1 < C::NCH) issue_x(w, ch + 1); else issue_x(after, 0);
+            }
+            __syncwarp();
+          }
+        }
+        if constexpr (!SUM) {
+          tmem_wait_ld();
+          reg_fence(v[ch & 1]);
+          if (ch + 1 < C::NCH) fetch(ch + 1); else release(buf);
+          scaled(val, CC * ch, std::integral_constant<int, CC>());
+        }
+        // The residual is added; dy is multiplied by the activation's slope.
+        if (has_x) {
+#pragma unroll
+          for (int i = 0; i < CC; ++i) {
+            const float x = X32 ? __uint_as_float(xr[X32 ? i : 0])
+                                : __uint_as_float(i & 1 ? xr[i / 2] & 0xFFFF0000u : xr[i / 2] << 16);
+            val[i] = PRE ? val[i] * x : val[i] + x;
+          }
         }
         if constexpr (PRE) {
           if (p.colsum != nullptr) {
-            // Column sums of the 32 rows in float32: five exchanges that halve the columns a lane holds leave lane l
-            // with column l. Rows past m have dy = 0.
-            float c[32];
+            // Column sums of the 32 rows in float32, across lanes, through shared memory: lane l then adds rows
+            // 8 (l / 8) + [0, 8) of columns 4 (l % 8) + [0, 4), and two exchanges join the four groups of rows. Rows
+            // past m have dy = 0.
+            const uint32_t red = sbase + C::OFF_RED + ew * 4096;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) c[i] = v[i];
+            for (int j = 0; j < CC; j += 32) {
+              __syncwarp();
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
+              for (int i = 0; i < 8; ++i)
+                st_shared_v4(red + sw128_offset(lane, i), __float_as_uint(val[j + 4 * i]), __float_as_uint(val[j + 4 * i + 1]),
+                             __float_as_uint(val[j + 4 * i + 2]), __float_as_uint(val[j + 4 * i + 3]));
+              __syncwarp();
+              float2 c0 = make_float2(0.f, 0.f), c1 = c0;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                if (i < o) {
-                  const bool up = (lane & o) != 0;
-                  const float send = up ? c[i] : c[i + o], keep = up ? c[i + o] : c[i];
-                  c[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-                }
+              for (int i = 0; i < 8; ++i) {
+                const float4 f = ld_shared_f32x4(red + sw128_offset((lane & 24) + i, lane & 7));
+                c0 = fadd2(c0, make_float2(f.x, f.y));
+                c1 = fadd2(c1, make_float2(f.z, f.w));
               }
+#pragma unroll
+              for (int o = 8; o <= 16; o <<= 1) {
+                c0.x += __shfl_xor_sync(0xffffffffu, c0.x, o);
+                c0.y += __shfl_xor_sync(0xffffffffu, c0.y, o);
+                c1.x += __shfl_xor_sync(0xffffffffu, c1.x, o);
+                c1.y += __shfl_xor_sync(0xffffffffu, c1.y, o);
+              }
+              // Lane l stores column 4 (l % 8) + l / 8.
+              const float c = lane & 16 ? (lane & 8 ? c1.y : c1.x) : (lane & 8 ? c0.y : c0.x);
+              const int cc = col + j + 4 * (lane & 7) + (lane >> 3);
+              if (row0 < p.m && cc < p.n) p.colsum[(row0 >> 5) * p.n + cc] = c;
             }
-            if (row0 < p.m && col + lane < p.n) p.colsum[(row0 >> 5) * p.n + col + lane] = c[0];
           }
         }
+        // The result into the output slot (without x the two slots alternate) once its last store has been read.
+        const uint32_t slot = !has_x && (q & 1) ? x_slot : o_slot;
+        if (!p.out_direct && elect_one_sync()) {
+          if (has_x) store_wait_read<0>(); else store_wait_read<1>();
+        }
+        __syncwarp();
         if constexpr (O32) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            st_shared_v4(slot + sw128_offset(lane, i), __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
-                         __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+          for (int i = 0; i < CC / 4; ++i)
+            st_shared_v4(slot + piece_at<C::O_ROW>(lane, i), __float_as_uint(val[4 * i]), __float_as_uint(val[4 * i + 1]),
+                         __float_as_uint(val[4 * i + 2]), __float_as_uint(val[4 * i + 3]));
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            st_shared_v4(slot + sw64_offset(lane, i), pack_bf16(v[8 * i], v[8 * i + 1]), pack_bf16(v[8 * i + 2], v[8 * i + 3]),
-                         pack_bf16(v[8 * i + 4], v[8 * i + 5]), pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+          for (int i = 0; i < CC / 8; ++i)
+            st_shared_v4(slot + piece_at<C::O_ROW>(lane, i), pack_bf16(val[8 * i], val[8 * i + 1]),
+                         pack_bf16(val[8 * i + 2], val[8 * i + 3]), pack_bf16(val[8 * i + 4], val[8 * i + 5]),
+                         pack_bf16(val[8 * i + 6], val[8 * i + 7]));
         }
         if (p.out_direct) {
           __syncwarp();
-#pragma unroll 8
+#pragma unroll(SUM ? 2 : 8)
           for (int r = 0; r < 32; ++r) {
-            if (row0 + r < p.m && col + lane < p.n) {
-              const int64_t at = (row0 + r) * p.ldo + col + lane;
-              if constexpr (O32)
-                static_cast<uint32_t*>(p.out)[at] = ld_shared_u32(slot + chunk_at<true>(r, lane));
-              else
-                static_cast<uint16_t*>(p.out)[at] = ld_shared_u16(slot + chunk_at<false>(r, lane));
+#pragma unroll
+            for (int j = lane; j < CC; j += 32) {
+              if (row0 + r < p.m && col + j < p.n) {
+                const int64_t at = (row0 + r) * p.ldo + col + j;
+                if constexpr (O32)
+                  static_cast<uint32_t*>(p.out)[at] = ld_shared_u32(slot + byte_at<C::O_ROW>(r, 4 * j));
+                else
+                  static_cast<uint16_t*>(p.out)[at] = ld_shared_u16(slot + byte_at<C::O_ROW>(r, 2 * j));
+              }
             }
           }
-          fence_proxy_async_smem();  // these reads before the slot's next TMA load
           __syncwarp();
-          if (x_tma && lane == 0) issue_x(issued);
-          ++issued;
         } else {
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
+          if (elect_one_sync()) {
             if (row0 < p.m && col < p.n)
-              tile_store(&tm_o, col, static_cast<int>(row0 + split * p.split_rows), slot);
+              tile_store(&tm_o, col, static_cast<int>(row0 + w.sp * p.split_rows), slot);
             store_commit();
-            if (x_tma) {
-              // The chunk before this one has left its slot: load into it.
-              store_wait_read<1>();
-              if (q > 0) issue_x(issued);
-            }
           }
-          if (q > 0) ++issued;
+          __syncwarp();
         }
       }
+      w = after;
     }
-    if (lane == 0) store_wait_all();
-    if (!ok && x_tma && lane == 0) {
-      // Gave up with copies in flight: wait (bounded, abort flag ignored) until they have landed.
+  done:
+    if (elect_one_sync()) store_wait_all();
+    __syncwarp();
+    if (!ok && x_tma) {
+      // Gave up with a copy in flight: wait (bounded, abort flag ignored) until it has landed.
       volatile int never = 0;
-      for (uint32_t i = q; i < issued && i < chunks; ++i) mbar_wait(slot_bar(ew, i % C::NSLOT), (i / C::NSLOT) & 1, &never);
+      mbar_wait(x_bar(ew), q & 1, &never);
     }
   }
   tc_fence_before();
@@ -566,14 +725,20 @@ __global__ void __maxnreg__(168)
   if (warp == 1) tmem_dealloc_cg<CG>(tmem, C::TMEM_COLS);
 }
 
-template <int TILE, int ACT, bool X32, bool O32, bool PRE>
+template <int TILE, int ACT, bool X32, bool O32, bool PRE, bool SUM>
 cudaError_t launch_tile(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx, const CUtensorMap& to,
-                        const LinearParams& p, int sms, cudaStream_t stream) {
-  using C = LinearCfg<TILE, X32 || O32>;
-  auto kernel = linear_tile_kernel<TILE, ACT, X32, O32, PRE>;
+                        const LinearParams& given, int sms, cudaStream_t stream) {
+  LinearParams p = given;
+  using C = LinearCfg<TILE, X32, O32, PRE, SUM>;
+  auto kernel = linear_tile_kernel<TILE, ACT, X32, O32, PRE, SUM>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return e;
   const int groups = std::min(p.items, sms / C::CG);
+  p.kb_q = p.k_blocks / p.splits;
+  p.kb_r = p.k_blocks % p.splits;
+  p.step_n = groups % p.n_tiles;
+  p.step_m = groups / p.n_tiles % p.m_tiles;
+  p.step_s = groups / p.n_tiles / p.m_tiles;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(groups * C::CG);
   cfg.blockDim = dim3(C::THREADS);
@@ -589,25 +754,27 @@ cudaError_t launch_tile(const CUtensorMap& ta, const CUtensorMap& tb, const CUte
   return cudaLaunchKernelEx(&cfg, kernel, ta, tb, tx, to, p);
 }
 
-template <int TILE, bool X32, bool O32, bool PRE>
+template <int TILE, bool X32, bool O32, bool PRE, bool SUM>
 cudaError_t by_act(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx, const CUtensorMap& to,
                    const LinearParams& p, int sms, cudaStream_t st) {
-  if (p.act == 1) return launch_tile<TILE, 1, X32, O32, PRE>(ta, tb, tx, to, p, sms, st);
-  if (p.act == 2) return launch_tile<TILE, 2, X32, O32, PRE>(ta, tb, tx, to, p, sms, st);
+  if (p.act == 1) return launch_tile<TILE, 1, X32, O32, PRE, SUM>(ta, tb, tx, to, p, sms, st);
+  if (p.act == 2) return launch_tile<TILE, 2, X32, O32, PRE, SUM>(ta, tb, tx, to, p, sms, st);
   if constexpr (PRE)
     return cudaErrorInvalidValue;  // without an activation the gradient needs no product
   else
-    return launch_tile<TILE, 0, X32, O32, PRE>(ta, tb, tx, to, p, sms, st);
+    return launch_tile<TILE, 0, X32, O32, PRE, SUM>(ta, tb, tx, to, p, sms, st);
 }
 
 template <int TILE>
 cudaError_t by_type(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx, const CUtensorMap& to,
                     const LinearParams& p, int sms, cudaStream_t st) {
   if (p.pre_grad)
-    return p.x_f32 ? by_act<TILE, true, false, true>(ta, tb, tx, to, p, sms, st)
-                   : by_act<TILE, false, false, true>(ta, tb, tx, to, p, sms, st);
-  return p.out_f32 ? by_act<TILE, true, true, false>(ta, tb, tx, to, p, sms, st)
-                   : by_act<TILE, false, false, false>(ta, tb, tx, to, p, sms, st);
+    return p.x_f32 ? by_act<TILE, true, false, true, false>(ta, tb, tx, to, p, sms, st)
+                   : by_act<TILE, false, false, true, false>(ta, tb, tx, to, p, sms, st);
+  if (!p.out_f32) return by_act<TILE, false, false, false, false>(ta, tb, tx, to, p, sms, st);
+  // More than one chunk of k in a split: added in registers.
+  return (p.k_blocks + p.splits - 1) / p.splits > p.chunk ? by_act<TILE, true, true, false, true>(ta, tb, tx, to, p, sms, st)
+                                                          : by_act<TILE, true, true, false, false>(ta, tb, tx, to, p, sms, st);
 }
 
 // ---- the sum of a split product's parts, with the epilogue ----------------------------------------------------------

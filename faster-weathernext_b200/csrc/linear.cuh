@@ -8,11 +8,17 @@
 namespace fwn {
 
 // Shapes of the tensor-core kernel's output tile: two SMs on 256 x 256, one on 128 x 128 or 128 x 64.
-enum LinearTile { kTile256 = 0, kTile128 = 1, kTile64 = 2 };
-__host__ __device__ constexpr int linear_tile_m(int t) { return t == kTile256 ? 256 : 128; }
+enum LinearTile { kTile256 = 0, kTile128 = 1, kTile64 = 2, kLinearTiles = 3 };
+__host__ __device__ constexpr bool linear_pair(int t) { return t == kTile256; }
+__host__ __device__ constexpr int linear_tile_m(int t) { return linear_pair(t) ? 256 : 128; }
 __host__ __device__ constexpr int linear_tile_n(int t) { return t == kTile256 ? 256 : t == kTile128 ? 128 : 64; }
+// Columns of the output (and of x) that an epilogue warp takes at a time: 128 bytes of a row where the warp's half of
+// the tile has them; the boxes of the two tensor maps.
+__host__ __device__ constexpr int linear_chunk_cols(int t, bool f32) { return f32 || t == kTile64 ? 32 : 64; }
 // Rows of B that one CTA loads (and the box rows of its tensor map).
-__host__ __device__ constexpr int linear_box_n(int t) { return t == kTile64 ? 64 : 128; }
+__host__ __device__ constexpr int linear_box_n(int t) { return linear_tile_n(t) / (linear_pair(t) ? 2 : 1); }
+// Stages of k (128 bytes each) that a float32 result accumulates in the tensor core at a time; see linear.cu.
+constexpr int kLinearChunk = 8;
 
 struct LinearParams {
   const void* bias;      // [n] or null
@@ -30,6 +36,9 @@ struct LinearParams {
   bool a_mn, b_mn;       // the operand's m (n) is contiguous instead of its k
   bool x_direct, out_direct;  // rows that TMA cannot address (strides or base off 16 bytes): plain accesses
   int m_tiles, n_tiles, splits, k_blocks, items;
+  int chunk;             // stages of k per accumulation in the tensor core (float32 output)
+  // Set at the launch: the stages of k of a split (the first kb_r take one more), and the walk's step in tiles.
+  int kb_q, kb_r, step_n, step_m, step_s;
   int64_t split_rows;    // rows of one split's partial sums in the output (splits > 1)
 };
 

@@ -364,25 +364,29 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 1024 ? 1 : 2) rm
   }
 }
 
-// out[j] = sum over r of part[r, j], j < d: 32 columns per block, warps take every eighth row, then the eight partial
-// sums are added in order.
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ part, int64_t rows, int d,
-                                                          void* __restrict__ out, bool out_bf16) {
-  __shared__ float red[8][33];
+// out[j] = sum over r of part[r, j], j < d: a block takes 32 columns, its 32 warps every 32nd row (eight loads in
+// flight each), and their sums are added in order.
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, int64_t rows, int d,
+                                                           void* __restrict__ out, bool out_bf16) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int j = blockIdx.x * 32 + lane;
   float t = 0.f;
-  if (j < d)
-    for (int64_t r = warp; r < rows; r += 8) t += part[r * d + j];
+  if (j < d) {
+#pragma unroll 8
+    for (int64_t r = warp; r < rows; r += 32) t += part[r * d + j];
+  }
   red[warp][lane] = t;
   __syncthreads();
-  if (warp == 0 && j < d) {
+  t = red[lane][warp];  // column `warp` of the block, the sums of its warps across the lanes
 #pragma unroll
-    for (int w = 1; w < 8; ++w) t += red[w][lane];
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  const int c = blockIdx.x * 32 + warp;
+  if (lane == 0 && c < d) {
     if (out_bf16)
-      static_cast<bf16*>(out)[j] = __float2bfloat16_rn(t);
+      static_cast<bf16*>(out)[c] = __float2bfloat16_rn(t);
     else
-      static_cast<float*>(out)[j] = t;
+      static_cast<float*>(out)[c] = t;
   }
 }
 
@@ -471,7 +475,7 @@ cudaError_t launch_rms_norm_bwd(const RmsBwdParams& p, int blocks, cudaStream_t 
 }
 
 cudaError_t launch_column_sum(const float* part, int64_t rows, int d, void* out, bool out_bf16, cudaStream_t st) {
-  column_sum_kernel<<<(d + 31) / 32, 256, 0, st>>>(part, rows, d, out, out_bf16);
+  column_sum_kernel<<<(d + 31) / 32, 1024, 0, st>>>(part, rows, d, out, out_bf16);
   return cudaGetLastError();
 }
 
