@@ -1160,8 +1160,20 @@ struct LinearPlan {
   size_t off_b, off_part, off_sum, bytes;
 };
 
-// Time model of the tensor-core kernel, in units of 0.01 us: a stage (128 bytes of k) of a tile's MMAs, and a tile's
-// epilogue, which overlaps the next tile's MMAs; a split product adds a launch and its parts' way through L2.
+// Whether a 256 x 256 tile takes its form with eight epilogue warps and five stages (kTile256Long) or sixteen and four
+// (kTile256): the first feeds the MMAs better, the second hides an epilogue that takes longer than a short k's MMAs.
+// Measured at 163,848 x k x 1,024, long / short in us: plain k 256 90 / 97, k 1,024 275 / 328; GELU k 512 176 / 167,
+// k 768 219 / 260; e4m3 plain k 512 114 / 104, k 768 130 / 150; e4m3 GELU k 1,024 220 / 193, k 1,536 (n 512) 124 / 143;
+// act'() k 1,024 447 / 418, k 1,536 (n 512) 268 / 334.
+bool long_form(const fwn_linear_desc& d, int64_t kb) {
+  if (d.flags & FWN_LINEAR_PRE_GRAD) return kb >= 20;
+  if (d.act != FWN_ACT_NONE) return kb >= 10;
+  return d.dtype == FWN_DTYPE_E4M3 ? kb >= 6 : true;
+}
+
+// Time model of the tensor-core kernel, in units of 0.01 us, from measurements at 42 to 163,848 rows: a stage (128 bytes
+// of k) of a tile, and its epilogue, which overlaps the next tile's MMAs; a split product adds a launch and its parts'
+// way through L2 (about 2.5 TB/s).
 LinearPlan plan_linear(const fwn_linear_desc& d, const void* a, const void* b, int sms) {
   LinearPlan pl{};
   const int64_t es = dtype_size(d.dtype);
@@ -1189,9 +1201,10 @@ LinearPlan plan_linear(const fwn_linear_desc& d, const void* a, const void* b, i
     at += static_cast<size_t>(round_up(b_outer * pl.ldb * es, 256));
   }
   const int64_t kb = (d.k * es + 127) / 128;
-  const int stage[fwn::kLinearTiles] = {29, 19, 15}, epilogue[fwn::kLinearTiles] = {200, 120, 80};
+  const int stage[fwn::kLinearTiles] = {55, 47, 31, 28}, epilogue[fwn::kLinearTiles] = {150, 200, 120, 100};
   int64_t best = INT64_MAX;
   for (int t = 0; t < fwn::kLinearTiles; ++t) {
+    if (t == (long_form(d, kb) ? fwn::kTile256 : fwn::kTile256Long)) continue;
     const int64_t tiles = ((d.m + fwn::linear_tile_m(t) - 1) / fwn::linear_tile_m(t)) *
                           ((d.n + fwn::linear_tile_n(t) - 1) / fwn::linear_tile_n(t));
     const int64_t slots = fwn::linear_pair(t) ? sms / 2 : sms;
@@ -1199,7 +1212,7 @@ LinearPlan plan_linear(const fwn_linear_desc& d, const void* a, const void* b, i
       if (s > 1 && (pre || tiles * s > 4 * slots)) break;
       const int64_t waves = (tiles * s + slots - 1) / slots, mine = (kb + s - 1) / s * stage[t];
       int64_t cost = waves * std::max<int64_t>(mine, epilogue[t]) + epilogue[t];
-      if (s > 1) cost += 300 + static_cast<int64_t>(8.0 * s * d.m * d.n / 5e4);
+      if (s > 1) cost += 430 + static_cast<int64_t>(8.0 * s * d.m * d.n / 2.5e4);
       if (cost < best) {
         best = cost;
         pl.tile = t;

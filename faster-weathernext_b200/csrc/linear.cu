@@ -11,7 +11,6 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <type_traits>
 
 #include "common.cuh"
 #include "linear.cuh"
@@ -68,6 +67,67 @@ __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.com
 template <int N>
 __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// A bounded wait of a whole warp by polling (mbarrier.test_wait), for the producers and the MMA warp: mbarrier.try_wait
+// suspends the warp, and came back some 300 cycles after the arrival.
+__device__ __forceinline__ bool poll_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  auto attempt = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+  bool ok = attempt();
+  if (!ok) {
+    unsigned long long t0 = 0;
+    for (uint32_t i = 1; !(ok = attempt()); ++i) {
+      if ((i & 255u) == 0u) {
+        if (*abort) break;
+        const unsigned long long t = globaltimer();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitLimitNs) {
+          *abort = 1;
+          atomicOr(&g_device_error, 5u);
+          break;
+        }
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+// A bounded wait like warp_wait for warps that wait long (the epilogue's): each try may suspend the warp for up to 4 us,
+// so that sixteen warps do not take issue slots and power from the MMA warp by polling.
+__device__ __forceinline__ bool idle_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  auto attempt = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(4000u)
+        : "memory");
+    return ok != 0;
+  };
+  bool ok = attempt();
+  if (!ok) {
+    const unsigned long long t0 = globaltimer();
+    while (!(ok = attempt())) {
+      if (*abort) break;
+      if (globaltimer() - t0 > kWaitLimitNs) {
+        *abort = 1;
+        atomicOr(&g_device_error, 5u);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
 
 template <int CG>
 __device__ __forceinline__ void tmem_alloc_cg(uint32_t dst, uint32_t cols) {
@@ -202,9 +262,10 @@ __device__ __forceinline__ void activate4(float* v) {
 //   1      MMA issuer (CG = 2: of the pair's first CTA, for both), into one of two TMEM accumulators;
 //   2      the same producer for b (one lane issues a load in about 200 cycles; two loads a stage held the MMAs);
 //   3      idle (it completes the warpgroup whose registers the epilogue takes);
-//   4-11   epilogue: warp w reads TMEM lanes 32 (w % 4) + [0, 32) (rows) and one half of the tile's columns, CC at a
-//          time (128 bytes of a row); the residual (or dy) chunk arrives by TMA one chunk ahead, the result leaves by
-//          TMA, and a tile's epilogue overlaps the next tile's MMAs.
+//   4-     epilogue, 16 warps (8 on the small tiles): warp w reads TMEM lanes 32 (w % 4) + [0, 32) (rows) and 64 of
+//          the tile's columns, in chunks of 128 bytes of a row; the residual (or dy) chunk arrives by TMA in the warp's
+//          slot, the result replaces it there and leaves by TMA, and a tile's epilogue overlaps the next tile's MMAs.
+//          With 8 warps the chain TMEM -> arithmetic -> shared memory -> store of two warps per scheduler left it idle.
 // Ragged edges: TMA fills rows and columns past the tensors with zeros and clips stores. Why a pair on 256 x 256: per
 // 64 of k an SM then takes in 32 KB for 512 cycles of MMA, half the L2 traffic per FLOP of 128 x 128 and two thirds of
 // 128 x 256. The small tiles spread products of few rows over the SMs. Why chunks of 128-byte rows: a TMA store of 32
@@ -212,7 +273,7 @@ __device__ __forceinline__ void activate4(float* v) {
 //
 // float32 results: the tensor core truncates its running sum at every step, an error that grows with k (measured 1.5e-6
 // of the result at k = 2,048). They take k in chunks (p.chunk stages) into alternate accumulators, which the epilogue
-// warps add in float32 registers (128 a thread: the epilogue warpgroups run with 224 registers).
+// warps add in float32 registers (64 a thread).
 template <int TILE, bool X32, bool O32, bool PRE, bool SUM>
 struct LinearCfg {
   static constexpr int CG = linear_pair(TILE) ? 2 : 1;
@@ -220,19 +281,24 @@ struct LinearCfg {
   static constexpr int BNC = BN / CG;                    // rows of b per CTA
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BNC * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int HC = BN / 2;                      // columns of an epilogue warp
+  static constexpr int EW = TILE == kTile256 ? 16 : 8;   // epilogue warps
+  static constexpr int HC = BN / (EW / 4);               // columns of an epilogue warp
   static constexpr int CC = linear_chunk_cols(TILE, X32 || O32);
   static constexpr int NCH = HC / CC;
   static constexpr int X_ROW = CC * (X32 ? 4 : 2), O_ROW = CC * (O32 ? 4 : 2);  // bytes: 128 or 64
   static constexpr int SLOT = 32 * (X_ROW > O_ROW ? X_ROW : O_ROW);
-  static constexpr int NS = STAGE == 24576 ? (PRE ? 4 : 6) : PRE ? 3 : 4;
+  static constexpr int RED = 32 * 64;                    // PRE: 32 rows x 16 columns in float32, for the column sums
+  static constexpr int NS = TILE == kTile256 ? (PRE ? 3 : 4) : TILE == kTile64 ? 6 : 5;
   static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int THREADS = 384;
-  static constexpr int N_BAR = 2 * NS + 4 + 1 + 8;
-  static constexpr int OFF_SLOT = NS * STAGE;            // per epilogue warp: x (or a second output), output
-  static constexpr int OFF_RED = OFF_SLOT + 8 * 2 * SLOT;      // PRE: 32 x 32 float32 per warp, for the column sums
-  static constexpr int OFF_VEC = OFF_RED + (PRE ? 8 * 4096 : 0);  // per epilogue warp: HC biases and HC scales
-  static constexpr int OFF_BAR = OFF_VEC + 8 * 2 * HC * 4;
+  static constexpr int THREADS = 128 + 32 * EW;
+  // Registers at launch (65,536 over the threads, in steps of 8) and after the warpgroups have traded: 128 x 32 + 512 x
+  // 112 = 640 x 96, 128 x 56 + 256 x 224 = 384 x 168.
+  static constexpr int REGS_LOW = TILE == kTile256 ? 40 : 56, REGS_HIGH = TILE == kTile256 ? 104 : 224;
+  static constexpr int N_BAR = 2 * NS + 4 + 1 + EW;
+  static constexpr int OFF_SLOT = NS * STAGE;            // per epilogue warp
+  static constexpr int OFF_RED = OFF_SLOT + EW * SLOT;
+  static constexpr int OFF_VEC = OFF_RED + (PRE ? EW * RED : 0);  // per epilogue warp: HC biases and HC scales
+  static constexpr int OFF_BAR = OFF_VEC + EW * 2 * HC * 4;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16 + 1024;
   static_assert(OFF_SLOT % 1024 == 0 && SLOT % 1024 == 0 && OFF_RED % 1024 == 0, "swizzle atoms");
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
@@ -286,10 +352,8 @@ __device__ __forceinline__ uint16_t ld_shared_u16(uint32_t a) {
   return v;
 }
 
-// 12 warps of 168 registers fill the register file; the epilogue's eight take 224 and leave 56 to the others:
-// 128 x 56 + 256 x 224 = 64,512 = 384 x 168.
 template <int TILE, int ACT, bool X32, bool O32, bool PRE, bool SUM>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 1)
     linear_tile_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                        const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_o,
                        const LinearParams p) {
@@ -320,10 +384,10 @@ __global__ void __launch_bounds__(384, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full(b), 1);
-      mbar_init(acc_empty(b), 8 * CG);
+      mbar_init(acc_empty(b), C::EW * CG);
     }
     mbar_init(drain, 1);
-    for (int w = 0; w < 8; ++w) mbar_init(x_bar(w), 1);
+    for (int w = 0; w < C::EW; ++w) mbar_init(x_bar(w), 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -342,7 +406,7 @@ __global__ void __launch_bounds__(384, 1)
   const int bk = p.fp8 ? 128 : 64;
 
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_LOW));
   if (warp == 0 || warp == 2) {
     // ------------------------------------------------------------------ TMA producers (a: warp 0, b: warp 2)
     // CG = 2: both CTAs' bytes count on the first CTA's barrier, whose warp 0 expects them.
@@ -357,7 +421,7 @@ __global__ void __launch_bounds__(384, 1)
       const int kb1 = w.kb1(p);
       for (int kb = w.kb0(p); kb < kb1; ++kb, ++g) {
         const int st = g % C::NS;
-        if (!(ok = warp_wait(empty(st), ((g / C::NS) & 1) ^ 1, abort_flag))) break;
+        if (!(ok = poll_wait(empty(st), ((g / C::NS) & 1) ^ 1, abort_flag))) break;
         const uint32_t bar = CG == 2 ? map_to(full(st), 0) : full(st);
         const uint32_t dst = is_a ? a_st(st) : b_st(st);
         if (elect_one_sync()) {
@@ -402,14 +466,14 @@ __global__ void __launch_bounds__(384, 1)
           if (begin) {
             left = SUM ? min(p.chunk, kb1 - kb) : kb1 - kb;
             buf = acc_i & 1;
-            if (!(ok = warp_wait(acc_empty(buf), ((acc_i >> 1) & 1) ^ 1, abort_flag))) break;
+            if (!(ok = poll_wait(acc_empty(buf), ((acc_i >> 1) & 1) ^ 1, abort_flag))) break;
             tc_fence_after();
             d = tmem + buf * C::BN;
             ++acc_i;
           }
           --left;
           const int st = g % C::NS;
-          if (!(ok = warp_wait(full(st), (g / C::NS) & 1, abort_flag))) break;
+          if (!(ok = poll_wait(full(st), (g / C::NS) & 1, abort_flag))) break;
           tc_fence_after();
           const uint64_t ad = smem_desc(a_st(st), a_lbo, 1024), bd = smem_desc(b_st(st), b_lbo, 1024);
           if (elect_one_sync()) {
@@ -439,12 +503,12 @@ __global__ void __launch_bounds__(384, 1)
     }
   }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_HIGH));
     // ------------------------------------------------------------------ epilogue
-    const int ew = warp - 4, quarter = warp & 3, half = ew >> 2;
+    const int ew = warp - 4, quarter = warp & 3, part = ew >> 2;
     constexpr int CC = C::CC;
-    const uint32_t trow = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + half * C::HC;
-    const uint32_t x_slot = sbase + C::OFF_SLOT + ew * 2 * C::SLOT, o_slot = x_slot + C::SLOT;
+    const uint32_t trow = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * C::HC;
+    const uint32_t slot = sbase + C::OFF_SLOT + ew * C::SLOT;
     float* vec = reinterpret_cast<float*>(smem + C::OFF_VEC) + ew * 2 * C::HC;
     const uint32_t vec_s = smem_u32(vec);
     const bool has_x = p.x != nullptr;
@@ -452,14 +516,14 @@ __global__ void __launch_bounds__(384, 1)
     // One lane issues all of a warp's copies (elect.sync: from uniform registers), so its waits cover its stores.
     auto issue_x = [&](const TileWalk& w, int ch) {  // the residual (dy) of chunk ch of a tile into the slot
       mbar_arrive_expect_tx(x_bar(ew), 32 * C::X_ROW);
-      tile_load<1>(x_slot, &tm_x, w.nt * C::BN + half * C::HC + ch * CC, w.mt * 128 * CG + rank * 128 + quarter * 32, x_bar(ew));
+      tile_load<1>(slot, &tm_x, w.nt * C::BN + part * C::HC + ch * CC, w.mt * 128 * CG + rank * 128 + quarter * 32, x_bar(ew));
     };
-    // Biases and scales of this warp's half of a tile's columns, HC / 32 a lane, read a tile ahead.
+    // Biases and scales of this warp's columns of a tile, HC / 32 a lane, read a tile ahead.
     float next_bias[C::HC / 32], next_scale[C::HC / 32];
     auto fetch_vec = [&](const TileWalk& w) {
 #pragma unroll
       for (int i = 0; i < C::HC / 32; ++i) {
-        const int c = w.nt * C::BN + half * C::HC + 32 * i + lane;
+        const int c = w.nt * C::BN + part * C::HC + 32 * i + lane;
         next_bias[i] = 0.f;
         next_scale[i] = 1.f;
         if (w.t < p.items && c < p.n) {
@@ -478,39 +542,44 @@ __global__ void __launch_bounds__(384, 1)
       }
     };
     float rs = 1.f;  // this row's scale
-    // N accumulated values of this lane's row, from column `at` of the warp's half: scales, bias, activation (its slope).
-    auto scaled = [&](float* v, int at, auto n) {
-      constexpr int N = decltype(n)::value;
+    // 32 accumulated values of this lane's row, from column `at` of the warp's: scales, bias, activation (its slope).
+    auto finish32 = [&](float* v, int at) {
       if (p.b_scale != nullptr) {
+        const float2 r2 = pair(rs);
 #pragma unroll
-        for (int i = 0; i < N / 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
           const float4 c = ld_shared_f32x4(vec_s + (C::HC + at + 4 * i) * 4);
-          v[4 * i] *= rs * c.x;
-          v[4 * i + 1] *= rs * c.y;
-          v[4 * i + 2] *= rs * c.z;
-          v[4 * i + 3] *= rs * c.w;
-        }
-      }
-      if (p.bias != nullptr) {
-#pragma unroll
-        for (int i = 0; i < N / 4; ++i) {
           const float4 b = ld_shared_f32x4(vec_s + (at + 4 * i) * 4);
-          v[4 * i] += b.x;
-          v[4 * i + 1] += b.y;
-          v[4 * i + 2] += b.z;
-          v[4 * i + 3] += b.w;
+          const float2 lo = ffma2(make_float2(v[4 * i], v[4 * i + 1]), fmul2(r2, make_float2(c.x, c.y)), make_float2(b.x, b.y));
+          const float2 hi = ffma2(make_float2(v[4 * i + 2], v[4 * i + 3]), fmul2(r2, make_float2(c.z, c.w)), make_float2(b.z, b.w));
+          v[4 * i] = lo.x;
+          v[4 * i + 1] = lo.y;
+          v[4 * i + 2] = hi.x;
+          v[4 * i + 3] = hi.y;
+        }
+      } else if (p.bias != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 b = ld_shared_f32x4(vec_s + (at + 4 * i) * 4);
+          const float2 lo = fadd2(make_float2(v[4 * i], v[4 * i + 1]), make_float2(b.x, b.y));
+          const float2 hi = fadd2(make_float2(v[4 * i + 2], v[4 * i + 3]), make_float2(b.z, b.w));
+          v[4 * i] = lo.x;
+          v[4 * i + 1] = lo.y;
+          v[4 * i + 2] = hi.x;
+          v[4 * i + 3] = hi.y;
         }
       }
       if constexpr (ACT != 0) {
         if constexpr (O32) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = activate<ACT>(v[i]);
+          for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
         } else {
 #pragma unroll
-          for (int i = 0; i < N / 4; ++i) activate4<ACT, PRE>(v + 4 * i);
+          for (int i = 0; i < 8; ++i) activate4<ACT, PRE>(v + 4 * i);
         }
       }
     };
+    auto combine = [&](float& v, float x) { v = PRE ? v * x : v + x; };  // dy times the slope; the residual is added
     TileWalk w(p, first);
     if (x_tma && elect_one_sync()) issue_x(w, 0);
     __syncwarp();
@@ -521,7 +590,7 @@ __global__ void __launch_bounds__(384, 1)
       TileWalk after = w;
       after.next(p, step);
       const int64_t row0 = static_cast<int64_t>(w.mt) * 128 * CG + rank * 128 + quarter * 32;
-      const int col0 = w.nt * C::BN + half * C::HC;
+      const int col0 = w.nt * C::BN + part * C::HC;
       __syncwarp();  // the previous tile's reads of vec
 #pragma unroll
       for (int i = 0; i < C::HC / 32; ++i) {
@@ -534,155 +603,142 @@ __global__ void __launch_bounds__(384, 1)
       __syncwarp();
       int buf = acc_i & 1;
       float sum[SUM ? C::HC : 1];
-      float v[SUM ? 1 : 2][SUM ? 32 : CC];  // a chunk in work and the next one on its way from TMEM
-      auto fetch = [&](int ch) {
-        if constexpr (!SUM) {
-#pragma unroll
-          for (int j = 0; j < CC; j += 32)
-            tmem_ld32(trow + buf * C::BN + CC * ch + j, *reinterpret_cast<float(*)[32]>(v[ch & 1] + j));
-        }
-      };
       if constexpr (SUM) {
 #pragma unroll
         for (int i = 0; i < C::HC; ++i) sum[i] = 0.f;
         const int kb1 = w.kb1(p);
         for (int kb = w.kb0(p); kb < kb1; kb += p.chunk, ++acc_i) {
           buf = acc_i & 1;
-          if (!(ok = warp_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) break;
+          if (!(ok = idle_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) goto done;
           tc_fence_after();
 #pragma unroll
-          for (int j = 0; j < C::HC; j += 32) {
-            tmem_ld32(trow + buf * C::BN + j, *reinterpret_cast<float(*)[32]>(v[0]));
+          for (int j = 0; j < C::HC; j += 16) {
+            float u[16];
+            tmem_ld16(trow + buf * C::BN + j, u);
             tmem_wait_ld();
-            reg_fence(*reinterpret_cast<float(*)[32]>(v[0]));
+            reg_fence(u);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sum[j + i] += v[0][i];
+            for (int i = 0; i < 16; ++i) sum[j + i] += u[i];
           }
           release(buf);
         }
-        if (!ok) break;
-#pragma unroll
-        for (int j = 0; j < C::HC; j += 32) scaled(sum + j, j, std::integral_constant<int, 32>());
       } else {
-        if (!(ok = warp_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) break;
+        if (!(ok = idle_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) goto done;
         tc_fence_after();
         ++acc_i;
-        fetch(0);
       }
 #pragma unroll
       for (int ch = 0; ch < C::NCH; ++ch, ++q) {
         const int col = col0 + CC * ch;
-        float* val = SUM ? sum + (SUM ? CC * ch : 0) : v[SUM ? 0 : ch & 1];
-        uint32_t xr[X32 ? CC : CC / 2];  // this lane's row of x
-        if (has_x) {
-          if (x_tma) {
-            if (!(ok = warp_wait(x_bar(ew), q & 1, abort_flag))) goto done;
-          } else {
+        if (x_tma) {
+          if (!(ok = idle_wait(x_bar(ew), q & 1, abort_flag))) goto done;
+        } else {
+          if (!p.out_direct && elect_one_sync()) store_wait_read<0>();  // the slot's last store
+          __syncwarp();
+          if (has_x) {
             // Rows that TMA cannot address: lane = column, so that a row's values are one access.
-#pragma unroll(SUM ? 2 : 8)
+#pragma unroll 4
             for (int r = 0; r < 32; ++r) {
 #pragma unroll
               for (int j = lane; j < CC; j += 32) {
                 const bool in = row0 + r < p.m && col + j < p.n;
                 const int64_t at = (row0 + r) * p.ldx + col + j;
                 if constexpr (X32)
-                  st_shared_u32(x_slot + byte_at<C::X_ROW>(r, 4 * j), in ? static_cast<const uint32_t*>(p.x)[at] : 0u);
+                  st_shared_u32(slot + byte_at<C::X_ROW>(r, 4 * j), in ? static_cast<const uint32_t*>(p.x)[at] : 0u);
                 else
-                  st_shared_u16(x_slot + byte_at<C::X_ROW>(r, 2 * j), in ? static_cast<const uint16_t*>(p.x)[at] : uint16_t(0));
+                  st_shared_u16(slot + byte_at<C::X_ROW>(r, 2 * j), in ? static_cast<const uint16_t*>(p.x)[at] : uint16_t(0));
               }
             }
             __syncwarp();
           }
-#pragma unroll
-          for (int i = 0; i < C::X_ROW / 16; ++i) {
-            const uint4 u = ld_shared_u32x4(x_slot + piece_at<C::X_ROW>(lane, i));
-            xr[4 * i] = u.x;
-            xr[4 * i + 1] = u.y;
-            xr[4 * i + 2] = u.z;
-            xr[4 * i + 3] = u.w;
-          }
-          // The slot has been read by every lane, and the proxy fence orders those reads before the copy that overwrites it
-          // (without it loads were still on their way when the next chunk landed): the next chunk's.
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (x_tma && (ch + 1 < C::NCH || after.t < p.items)) {
-            if (elect_one_sync()) {
-              if (ch + 1 < C::NCH) issue_x(w, ch + 1); else issue_x(after, 0);
-            }
-            __syncwarp();
-          }
         }
-        if constexpr (!SUM) {
-          tmem_wait_ld();
-          reg_fence(v[ch & 1]);
-          if (ch + 1 < C::NCH) fetch(ch + 1); else release(buf);
-          scaled(val, CC * ch, std::integral_constant<int, CC>());
-        }
-        // The residual is added; dy is multiplied by the activation's slope.
-        if (has_x) {
 #pragma unroll
-          for (int i = 0; i < CC; ++i) {
-            const float x = X32 ? __uint_as_float(xr[X32 ? i : 0])
-                                : __uint_as_float(i & 1 ? xr[i / 2] & 0xFFFF0000u : xr[i / 2] << 16);
-            val[i] = PRE ? val[i] * x : val[i] + x;
+        for (int h = 0; h < CC; h += 32) {
+          float acc[32];
+          float* v = acc;
+          if constexpr (SUM) {
+            v = sum + (SUM ? CC * ch + h : 0);
+          } else {
+            tmem_ld32(trow + buf * C::BN + CC * ch + h, acc);
+            tmem_wait_ld();
+            reg_fence(acc);
+            if (ch == C::NCH - 1 && h == CC - 32) release(buf);
           }
-        }
-        if constexpr (PRE) {
-          if (p.colsum != nullptr) {
-            // Column sums of the 32 rows in float32, across lanes, through shared memory: lane l then adds rows
-            // 8 (l / 8) + [0, 8) of columns 4 (l % 8) + [0, 4), and two exchanges join the four groups of rows. Rows
-            // past m have dy = 0.
-            const uint32_t red = sbase + C::OFF_RED + ew * 4096;
-#pragma unroll
-            for (int j = 0; j < CC; j += 32) {
-              __syncwarp();
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                st_shared_v4(red + sw128_offset(lane, i), __float_as_uint(val[j + 4 * i]), __float_as_uint(val[j + 4 * i + 1]),
-                             __float_as_uint(val[j + 4 * i + 2]), __float_as_uint(val[j + 4 * i + 3]));
-              __syncwarp();
-              float2 c0 = make_float2(0.f, 0.f), c1 = c0;
+          finish32(v, CC * ch + h);
+          if (has_x) {
+            if constexpr (X32) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float4 f = ld_shared_f32x4(red + sw128_offset((lane & 24) + i, lane & 7));
-                c0 = fadd2(c0, make_float2(f.x, f.y));
-                c1 = fadd2(c1, make_float2(f.z, f.w));
+                const float4 f = ld_shared_f32x4(slot + piece_at<C::X_ROW>(lane, i));
+                combine(v[4 * i], f.x);
+                combine(v[4 * i + 1], f.y);
+                combine(v[4 * i + 2], f.z);
+                combine(v[4 * i + 3], f.w);
               }
+              if constexpr (!O32) __syncwarp();  // the result's rows are shorter than x's: every lane has read its own
+            } else {
 #pragma unroll
-              for (int o = 8; o <= 16; o <<= 1) {
-                c0.x += __shfl_xor_sync(0xffffffffu, c0.x, o);
-                c0.y += __shfl_xor_sync(0xffffffffu, c0.y, o);
-                c1.x += __shfl_xor_sync(0xffffffffu, c1.x, o);
-                c1.y += __shfl_xor_sync(0xffffffffu, c1.y, o);
+              for (int i = 0; i < 4; ++i) {
+                const uint4 u = ld_shared_u32x4(slot + piece_at<C::X_ROW>(lane, h / 8 + i));
+                const uint32_t t[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  combine(v[8 * i + 2 * e], __uint_as_float(t[e] << 16));
+                  combine(v[8 * i + 2 * e + 1], __uint_as_float(t[e] & 0xFFFF0000u));
+                }
               }
-              // Lane l stores column 4 (l % 8) + l / 8.
-              const float c = lane & 16 ? (lane & 8 ? c1.y : c1.x) : (lane & 8 ? c0.y : c0.x);
-              const int cc = col + j + 4 * (lane & 7) + (lane >> 3);
-              if (row0 < p.m && cc < p.n) p.colsum[(row0 >> 5) * p.n + cc] = c;
             }
           }
-        }
-        // The result into the output slot (without x the two slots alternate) once its last store has been read.
-        const uint32_t slot = !has_x && (q & 1) ? x_slot : o_slot;
-        if (!p.out_direct && elect_one_sync()) {
-          if (has_x) store_wait_read<0>(); else store_wait_read<1>();
-        }
-        __syncwarp();
-        if constexpr (O32) {
+          if constexpr (PRE) {
+            if (p.colsum != nullptr) {
+              // Column sums of the 32 rows in float32, across lanes, 16 columns at a time through shared memory: lane l
+              // adds rows 4 (l / 4) + [0, 4) of columns 4 (l % 4) + [0, 4), and three exchanges join the eight groups
+              // of rows, the first two of which also share out the columns. Rows past m have dy = 0.
+              const uint32_t red = sbase + C::OFF_RED + ew * C::RED;
 #pragma unroll
-          for (int i = 0; i < CC / 4; ++i)
-            st_shared_v4(slot + piece_at<C::O_ROW>(lane, i), __float_as_uint(val[4 * i]), __float_as_uint(val[4 * i + 1]),
-                         __float_as_uint(val[4 * i + 2]), __float_as_uint(val[4 * i + 3]));
-        } else {
+              for (int j = 0; j < 32; j += 16) {
+                __syncwarp();
 #pragma unroll
-          for (int i = 0; i < CC / 8; ++i)
-            st_shared_v4(slot + piece_at<C::O_ROW>(lane, i), pack_bf16(val[8 * i], val[8 * i + 1]),
-                         pack_bf16(val[8 * i + 2], val[8 * i + 3]), pack_bf16(val[8 * i + 4], val[8 * i + 5]),
-                         pack_bf16(val[8 * i + 6], val[8 * i + 7]));
+                for (int i = 0; i < 4; ++i)
+                  st_shared_v4(red + sw64_offset(lane, i), __float_as_uint(v[j + 4 * i]), __float_as_uint(v[j + 4 * i + 1]),
+                               __float_as_uint(v[j + 4 * i + 2]), __float_as_uint(v[j + 4 * i + 3]));
+                __syncwarp();
+                float2 c0 = make_float2(0.f, 0.f), c1 = c0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float4 f = ld_shared_f32x4(red + sw64_offset((lane & 28) + i, lane & 3));
+                  c0 = fadd2(c0, make_float2(f.x, f.y));
+                  c1 = fadd2(c1, make_float2(f.z, f.w));
+                }
+                const bool up = lane & 4, odd = lane & 8;
+                const float2 send = up ? c0 : c1;
+                float2 keep = up ? c1 : c0;
+                keep.x += __shfl_xor_sync(0xffffffffu, send.x, 4);
+                keep.y += __shfl_xor_sync(0xffffffffu, send.y, 4);
+                float c = odd ? keep.y : keep.x;
+                c += __shfl_xor_sync(0xffffffffu, odd ? keep.x : keep.y, 8);
+                c += __shfl_xor_sync(0xffffffffu, c, 16);
+                const int cc = col + h + j + 4 * (lane & 3) + 2 * up + odd;
+                if (lane < 16 && row0 < p.m && cc < p.n) p.colsum[(row0 >> 5) * p.n + cc] = c;
+              }
+            }
+          }
+          if constexpr (O32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              st_shared_v4(slot + piece_at<C::O_ROW>(lane, i), __float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                           __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              st_shared_v4(slot + piece_at<C::O_ROW>(lane, h / 8 + i), pack_bf16(v[8 * i], v[8 * i + 1]),
+                           pack_bf16(v[8 * i + 2], v[8 * i + 3]), pack_bf16(v[8 * i + 4], v[8 * i + 5]),
+                           pack_bf16(v[8 * i + 6], v[8 * i + 7]));
+          }
         }
         if (p.out_direct) {
           __syncwarp();
-#pragma unroll(SUM ? 2 : 8)
+#pragma unroll 4
           for (int r = 0; r < 32; ++r) {
 #pragma unroll
             for (int j = lane; j < CC; j += 32) {
@@ -695,17 +751,23 @@ __global__ void __launch_bounds__(384, 1)
               }
             }
           }
-          __syncwarp();
-        } else {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (elect_one_sync()) {
+        }
+        // The slot's writes before the store that reads them, its reads before the copy that overwrites them (without
+        // the proxy fence loads were still on their way when the next chunk landed).
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (elect_one_sync()) {
+          if (!p.out_direct) {
             if (row0 < p.m && col < p.n)
               tile_store(&tm_o, col, static_cast<int>(row0 + w.sp * p.split_rows), slot);
             store_commit();
           }
-          __syncwarp();
+          if (x_tma && (ch + 1 < C::NCH || after.t < p.items)) {
+            if (!p.out_direct) store_wait_read<0>();
+            if (ch + 1 < C::NCH) issue_x(w, ch + 1); else issue_x(after, 0);
+          }
         }
+        __syncwarp();
       }
       w = after;
     }
@@ -972,6 +1034,7 @@ __global__ void __launch_bounds__(256) grad_cast_kernel(const void* __restrict__
 cudaError_t launch_linear_tiles(int tile, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx,
                                 const CUtensorMap& to, const LinearParams& p, int sms, cudaStream_t st) {
   if (tile == kTile256) return by_type<kTile256>(ta, tb, tx, to, p, sms, st);
+  if (tile == kTile256Long) return by_type<kTile256Long>(ta, tb, tx, to, p, sms, st);
   if (tile == kTile128) return by_type<kTile128>(ta, tb, tx, to, p, sms, st);
   return by_type<kTile64>(ta, tb, tx, to, p, sms, st);
 }

@@ -7,11 +7,12 @@
 
 namespace fwn {
 
-// Shapes of the tensor-core kernel's output tile: two SMs on 256 x 256, one on 128 x 128 or 128 x 64.
-enum LinearTile { kTile256 = 0, kTile128 = 1, kTile64 = 2, kLinearTiles = 3 };
-__host__ __device__ constexpr bool linear_pair(int t) { return t == kTile256; }
+// Shapes of the tensor-core kernel's output tile: two SMs on 256 x 256 (two forms: sixteen epilogue warps and four
+// stages, or eight and five), one on 128 x 128 or 128 x 64.
+enum LinearTile { kTile256 = 0, kTile256Long = 1, kTile128 = 2, kTile64 = 3, kLinearTiles = 4 };
+__host__ __device__ constexpr bool linear_pair(int t) { return t == kTile256 || t == kTile256Long; }
 __host__ __device__ constexpr int linear_tile_m(int t) { return linear_pair(t) ? 256 : 128; }
-__host__ __device__ constexpr int linear_tile_n(int t) { return t == kTile256 ? 256 : t == kTile128 ? 128 : 64; }
+__host__ __device__ constexpr int linear_tile_n(int t) { return linear_pair(t) ? 256 : t == kTile128 ? 128 : 64; }
 // Columns of the output (and of x) that an epilogue warp takes at a time: 128 bytes of a row where the warp's half of
 // the tile has them; the boxes of the two tensor maps.
 __host__ __device__ constexpr int linear_chunk_cols(int t, bool f32) { return f32 || t == kTile64 ? 32 : 64; }
