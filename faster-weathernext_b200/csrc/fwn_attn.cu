@@ -996,10 +996,15 @@ fwn_status check_rms(const fwn_rms_desc* d, bool residual, bool weight, bool bwd
   return FWN_OK;
 }
 
-// Whether a [rows, d] tensor's rows allow 8 values per access: 32 bytes of float32, 16 of bf16, 8 of e4m3.
-bool wide_rows(const void* p, int32_t dtype, int64_t stride, int64_t rows) {
-  const int64_t bytes = 8 * dtype_size(dtype);
-  return p == nullptr || (aligned_to(p, bytes) && (rows <= 1 || stride % 8 == 0));
+// Whether a tensor starts where 8 values are one access: 32 bytes of float32, 16 of bf16, 8 of e4m3.
+bool starts_wide(const void* p, int32_t dtype) { return p == nullptr || aligned_to(p, 8 * dtype_size(dtype)); }
+
+int rms_row_mode(const fwn_rms_desc& d, bool starts, bool residual, const void* weight) {
+  const bool one = d.rows <= 1;
+  const bool wide = starts && d.d % 8 == 0 && (one || d.x_stride % 8 == 0) &&
+                    (!residual || one || d.residual_stride % 8 == 0) && (!weight || aligned16(weight));
+  const bool packed = starts && (one || d.x_stride == d.d) && (!residual || one || d.residual_stride == d.d);
+  return fwn::rms_mode(wide, packed, d.d);
 }
 
 }  // namespace
@@ -1031,9 +1036,10 @@ fwn_status fwn_rms_norm(const fwn_rms_desc* desc, const void* x, const void* res
   p.residual_bf16 = d.residual_dtype == FWN_DTYPE_BF16;
   p.weight_bf16 = d.weight_dtype == FWN_DTYPE_BF16;
   p.normalize = !(d.flags & FWN_RMS_SCALE_ONLY);
-  p.wide = d.d % 8 == 0 && wide_rows(x, d.x_dtype, d.x_stride, d.rows) &&
-           wide_rows(residual, d.residual_dtype, d.residual_stride, d.rows) && wide_rows(x_out, d.x_dtype, d.d, d.rows) &&
-           wide_rows(out, d.out_dtype, d.d, d.rows) && (!weight || aligned16(weight));
+  const bool starts = starts_wide(x, d.x_dtype) && starts_wide(residual, d.residual_dtype) &&
+                      starts_wide(x_out, d.x_dtype) && starts_wide(out, d.out_dtype);
+  p.mode = rms_row_mode(d, starts, residual != nullptr, weight);
+  p.sms = num_sms();
   cudaError_t e = fwn::launch_rms_norm(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "rms_norm");
   return ok();
@@ -1043,7 +1049,11 @@ fwn_status fwn_rms_norm_bwd_workspace_size(const fwn_rms_desc* desc, size_t* byt
   if (!bytes) return fail(FWN_ERR_INVALID_ARGUMENT, "bytes is null");
   fwn_status s = check_rms(desc, false, false, true);
   if (s != FWN_OK) return s;
-  *bytes = static_cast<size_t>(fwn::rms_bwd_blocks(desc->rows, desc->d, num_sms())) * desc->d * sizeof(float);
+  // The mode goes by the operands' addresses too: the most that any of them needs.
+  int blocks = 0;
+  const int sms = num_sms();
+  for (int mode = 0; mode < 3; ++mode) blocks = std::max(blocks, fwn::rms_bwd_blocks(desc->rows, desc->d, sms, mode));
+  *bytes = static_cast<size_t>(blocks) * desc->d * sizeof(float);
   if (*bytes < 16) *bytes = 16;
   return ok();
 }
@@ -1085,11 +1095,12 @@ fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, const void*
   p.weight_bf16 = d.weight_dtype == FWN_DTYPE_BF16;
   p.dh_bf16 = d.out_dtype == FWN_DTYPE_BF16;
   p.dw_bf16 = p.weight_bf16;
-  p.wide = d.d % 8 == 0 && wide_rows(x, d.x_dtype, d.x_stride, d.rows) &&
-           wide_rows(residual, d.residual_dtype, d.residual_stride, d.rows) && wide_rows(dh, d.out_dtype, d.d, d.rows) &&
-           wide_rows(ds, d.x_dtype, d.d, d.rows) && wide_rows(dx, d.x_dtype, d.d, d.rows) &&
-           wide_rows(d_residual, d.residual_dtype, d.d, d.rows) && (!weight || aligned16(weight));
-  cudaError_t e = fwn::launch_rms_norm_bwd(p, fwn::rms_bwd_blocks(d.rows, d.d, num_sms()), static_cast<cudaStream_t>(stream));
+  const bool starts = starts_wide(x, d.x_dtype) && starts_wide(residual, d.residual_dtype) &&
+                      starts_wide(dh, d.out_dtype) && starts_wide(ds, d.x_dtype) && starts_wide(dx, d.x_dtype) &&
+                      starts_wide(d_residual, d.residual_dtype);
+  p.mode = rms_row_mode(d, starts, residual != nullptr, weight);
+  cudaError_t e = fwn::launch_rms_norm_bwd(p, fwn::rms_bwd_blocks(d.rows, d.d, num_sms(), p.mode),
+                                           static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "rms_norm_bwd");
   return ok();
 }

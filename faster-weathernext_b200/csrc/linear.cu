@@ -253,6 +253,25 @@ __device__ __forceinline__ void activate4(float* v) {
   }
 }
 
+// Four values through the hardware's tanh, one special-function call each: off by at most 2^-12 of |x| absolutely, so that
+// the tail (x < -2) keeps few digits of its own. For 8-bit operands, whose own rounding is 2^-4: the e4m3 GELU
+// up-projection (163,848 x 512 x 2,048) went from 309 to 234 us, the bf16 one, which stays exact, would from 317 to 302.
+template <int ACT>
+__device__ __forceinline__ void activate4_short(float* v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 x = make_float2(v[2 * i], v[2 * i + 1]);
+    const float2 h = fmul2(x, pair(0.5f));
+    const float2 z = ACT == 1 ? fmul2(x, ffma2(fmul2(x, x), pair(kGeluC0 * kGeluC1), pair(kGeluC0))) : h;
+    float2 t;
+    asm("tanh.approx.f32 %0, %1;" : "=f"(t.x) : "f"(z.x));
+    asm("tanh.approx.f32 %0, %1;" : "=f"(t.y) : "f"(z.y));
+    const float2 y = ffma2(h, t, h);
+    v[2 * i] = y.x;
+    v[2 * i + 1] = y.y;
+  }
+}
+
 // ---- tensor-core kernel --------------------------------------------------------------------------------------------
 
 // Persistent; a CTA (CG = 1) or a pair of CTAs on two SMs (CG = 2) takes output tiles of 128 CG x BN, walked with n
@@ -573,6 +592,9 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
         if constexpr (O32) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
+        } else if (!PRE && p.b_scale != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) activate4_short<ACT>(v + 4 * i);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) activate4<ACT, PRE>(v + 4 * i);

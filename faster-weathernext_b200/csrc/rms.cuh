@@ -23,7 +23,7 @@ struct RmsParams {
   int out_type;
   bool x_bf16, residual_bf16, weight_bf16;
   bool normalize;        // false: the sum itself (scaled by weight, if any) is written
-  bool wide;             // every row and tensor allows 8 values per access
+  int mode, sms;         // rms_mode; multiprocessors
 };
 
 struct RmsBwdParams {
@@ -39,11 +39,15 @@ struct RmsBwdParams {
   int64_t rows, x_stride, residual_stride;
   int d;
   float eps;
-  bool x_bf16, residual_bf16, weight_bf16, dh_bf16, dw_bf16, wide;
+  bool x_bf16, residual_bf16, weight_bf16, dh_bf16, dw_bf16;
+  int mode;
 };
 
+// How rows are laid over threads. wide: every row of every tensor allows 8 values per access; packed: all tensors are
+// contiguous, from a base that allows 8 values per access.
+int rms_mode(bool wide, bool packed, int d);
 cudaError_t launch_rms_norm(const RmsParams& p, cudaStream_t stream);
-int rms_bwd_blocks(int64_t rows, int d, int sms);
+int rms_bwd_blocks(int64_t rows, int d, int sms, int mode);
 cudaError_t launch_rms_norm_bwd(const RmsBwdParams& p, int blocks, cudaStream_t stream);
 cudaError_t launch_column_sum(const float* part, int64_t rows, int d, void* out, bool out_bf16, cudaStream_t stream);
 

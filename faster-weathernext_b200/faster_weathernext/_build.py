@@ -3,6 +3,7 @@
     python -m faster_weathernext._build            # from faster-weathernext_b200/
 """
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -45,14 +46,18 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
   out_dir = os.path.join(ROOT, "_build")
   os.makedirs(out_dir, exist_ok=True)
-  objs = []
-  for src in SOURCES:
+
+
+  def compile_one(src):
     obj = os.path.join(out_dir, src.replace(".cu", ".o"))
     cmd = [nvcc(), *ARCH, *FLAGS, "-I", INCLUDE, "-c", os.path.join(CSRC, src), "-o", obj]
     if verbose:
       cmd.insert(1, "-Xptxas=-v")
     subprocess.run(cmd, check=True)
-    objs.append(obj)
+    return obj
+
+  with concurrent.futures.ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+    objs = list(pool.map(compile_one, SOURCES))
   tmp = LIB + ".tmp"
   subprocess.run([nvcc(), *ARCH, "-shared", "-o", tmp, *objs, "-lcudart_static", "-ldl",
                   "-lrt", "-lpthread"], check=True)

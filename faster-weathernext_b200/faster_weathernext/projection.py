@@ -214,6 +214,19 @@ def _orient(t):
   return t.contiguous(), c, False
 
 
+def _padded(t):
+  """t, or a copy of t [r, c] in its own order with rows of whole 16 bytes, which TMA can address: an operand of three
+  products (odd widths) is laid out once instead of by each."""
+  src, ld, turned = _orient(t)
+  if (ld % 8 == 0 and src.data_ptr() % 16 == 0) or src.shape[0] <= 8:
+    return t
+  if turned:
+    src = src.t()
+  out = src.new_empty((src.shape[0], -(-src.shape[1] // 8) * 8))[:, :src.shape[1]]
+  out.copy_(src)
+  return out.t() if turned else out
+
+
 # Workspace bytes by a call's shape, types, strides and the alignment of its operands (asked once for each).
 _WORKSPACE = {}
 
@@ -295,9 +308,11 @@ class _Linear(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, a, weight, bias, residual, act, out_dtype):
-    ctx.act = act
-    ctx.save_for_backward(a, weight, bias)
-    return _linear_forward(a, weight, bias, residual, act, out_dtype)
+    ctx.act, ctx.shape = act, a.shape
+    a2, w2 = _padded(_rows(a)), _padded(weight)
+    ctx.save_for_backward(a2, w2, bias)
+    y = _linear_forward(a2, w2, bias, None if residual is None else _rows(residual), act, out_dtype)
+    return y if a.dim() == 2 else y.view(*a.shape[:-1], weight.shape[0])
 
   @staticmethod
   def backward(ctx, dy):
@@ -305,30 +320,29 @@ class _Linear(torch.autograd.Function):
     need_a, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     d_a = d_w = d_b = None
     if a.numel() == 0:
-      d_a = torch.zeros_like(a) if need_a else None
+      d_a = a.new_zeros(ctx.shape) if need_a else None
       d_w = torch.zeros_like(weight) if need_w else None
       d_b = torch.zeros_like(bias) if need_b else None
     elif need_a or need_w or need_b:
       d_a, d_w, d_b = _on_device(a, _Linear._launch, a, weight, bias, ctx.act, dy, need_a, need_w, need_b)
+      if need_a and len(ctx.shape) != 2:
+        d_a = d_a.view(ctx.shape)
     return d_a, d_w, d_b, dy if need_r else None, None, None
 
   @staticmethod
   def _launch(stream, a, weight, bias, act, dy, need_a, need_w, need_b):
-    n, k = weight.shape
-    a2 = _rows(a)
+    n = weight.shape[0]
     d_a = d_w = None
-    d_pre, d_b = _pre_gradient(stream, a2, weight, None if bias is None else bias.contiguous(), act,
+    d_pre, d_b = _pre_gradient(stream, a, weight, None if bias is None else bias.contiguous(), act,
                                dy if dy.dim() == 2 else dy.reshape(-1, n), need_b)
     if need_a:
       d_a = _product(stream, d_pre, weight.t(), None, None, _lib.ACT_NONE, _BF16)
-      if a.dim() != 2:
-        d_a = d_a.view(a.shape)
     if need_w:
       # In the weight's own orientation, so that the gradient's rows are written as they lie.
       if weight.stride(0) == 1 and weight.stride(1) != 1:
-        d_w = _product(stream, a2.t(), d_pre.t(), None, None, _lib.ACT_NONE, _BF16).t()
+        d_w = _product(stream, a.t(), d_pre.t(), None, None, _lib.ACT_NONE, _BF16).t()
       else:
-        d_w = _product(stream, d_pre.t(), a2.t(), None, None, _lib.ACT_NONE, _BF16)
+        d_w = _product(stream, d_pre.t(), a.t(), None, None, _lib.ACT_NONE, _BF16)
     return d_a, d_w, d_b
 
 
