@@ -1366,33 +1366,109 @@ fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const float* a
   return ok();
 }
 
-fwn_status fwn_linear_grad_cast_workspace_size(int64_t m, int32_t n, size_t* bytes) {
+namespace {
+
+// The backward of a projection as three steps on one stream: the gradient of the pre-activation, which the other two
+// read, and their workspace, which they take in turn.
+struct LinearBwdPlan {
+  bool cast;                    // d_pre is written (an activation, or dy is not bf16 rows that TMA can address)
+  int64_t ldp;                  // d_pre's row stride
+  fwn_linear_desc pre, da, db;
+  bool db_turned;               // d_b is written as [k, n]
+  int cast_blocks;
+  size_t off_ws, ws, bytes;
+};
+
+LinearBwdPlan plan_linear_bwd(const fwn_linear_desc& d, const void* a, const void* b, const void* dy, int sms) {
+  LinearBwdPlan pl{};
+  const bool act = d.act != FWN_ACT_NONE;
+  const bool a_mn = d.flags & FWN_LINEAR_A_M_CONTIGUOUS, b_mn = d.flags & FWN_LINEAR_B_N_CONTIGUOUS;
+  pl.cast = act || d.x_dtype != FWN_DTYPE_BF16 || !tma_rows(dy, d.x_dtype, d.m, d.ldx);
+  pl.ldp = pl.cast ? round_up(d.n, 8) : d.ldx;
+  pl.pre = d;
+  pl.pre.flags = d.flags | FWN_LINEAR_PRE_GRAD;
+  pl.pre.out_dtype = FWN_DTYPE_BF16;
+  pl.pre.ldo = pl.ldp;
+  const void* aligned = nullptr;  // d_pre: the workspace's start, or dy, which TMA can address
+  // d_a [m, k] = d_pre [m, n] b: b as [k, n] rows.
+  pl.da = fwn_linear_desc{d.m, d.k, d.n, FWN_DTYPE_BF16, FWN_DTYPE_BF16, 0, 0, FWN_ACT_NONE,
+                          b_mn ? 0 : FWN_LINEAR_B_N_CONTIGUOUS, pl.ldp, d.ldb, 0, d.k};
+  // d_b: [n, k] = d_pre^T a, or [k, n] = a^T d_pre.
+  pl.db_turned = b_mn;
+  const int a_mc = FWN_LINEAR_A_M_CONTIGUOUS, b_nc = FWN_LINEAR_B_N_CONTIGUOUS;
+  if (b_mn)
+    pl.db = fwn_linear_desc{d.k, d.n, static_cast<int32_t>(d.m), FWN_DTYPE_BF16, FWN_DTYPE_BF16, 0, 0, FWN_ACT_NONE,
+                            (a_mn ? 0 : a_mc) | b_nc, d.lda, pl.ldp, 0, d.n};
+  else
+    pl.db = fwn_linear_desc{d.n, d.k, static_cast<int32_t>(d.m), FWN_DTYPE_BF16, FWN_DTYPE_BF16, 0, 0, FWN_ACT_NONE,
+                            a_mc | (a_mn ? 0 : b_nc), pl.ldp, d.lda, 0, d.k};
+  pl.off_ws = pl.cast ? static_cast<size_t>(round_up(d.m * pl.ldp * 2, 256)) : 0;
+  pl.cast_blocks = fwn::grad_cast_blocks(d.m, d.n, sms);
+  pl.ws = act ? plan_linear(pl.pre, a, b, sms).bytes
+              : static_cast<size_t>(round_up(static_cast<int64_t>(pl.cast_blocks) * d.n * sizeof(float), 256));
+  pl.ws = std::max(pl.ws, plan_linear(pl.da, aligned, b, sms).bytes);
+  pl.ws = std::max(pl.ws, b_mn ? plan_linear(pl.db, a, aligned, sms).bytes : plan_linear(pl.db, aligned, a, sms).bytes);
+  pl.bytes = pl.off_ws + pl.ws;
+  return pl;
+}
+
+fwn_status check_linear_bwd(const fwn_linear_desc* d) {
+  fwn_status s = check_linear(d);
+  if (s != FWN_OK) return s;
+  if (d->m < 1) return fail(FWN_ERR_INVALID_ARGUMENT, "m must be positive");
+  if (d->dtype != FWN_DTYPE_BF16 || (d->flags & FWN_LINEAR_PRE_GRAD))
+    return fail(FWN_ERR_UNSUPPORTED, "the backward takes bf16 operands and no FWN_LINEAR_PRE_GRAD");
+  if (d->m > 1 && d->ldx < d->n) return fail(FWN_ERR_INVALID_ARGUMENT, "ldx is below n");
+  return FWN_OK;
+}
+
+}  // namespace
+
+fwn_status fwn_linear_bwd_workspace_size(const fwn_linear_desc* desc, const void* a, const void* b, const void* dy,
+                                         size_t* bytes) {
   if (!bytes) return fail(FWN_ERR_INVALID_ARGUMENT, "bytes is null");
-  if (m < 0 || n <= 0) return fail(FWN_ERR_INVALID_ARGUMENT, "bad shape m=%lld n=%d", static_cast<long long>(m), n);
-  *bytes = static_cast<size_t>(fwn::grad_cast_blocks(m, n, num_sms())) * n * sizeof(float);
+  fwn_status s = check_linear_bwd(desc);
+  if (s != FWN_OK) return s;
+  *bytes = plan_linear_bwd(*desc, a, b, dy, num_sms()).bytes;
   return ok();
 }
 
-fwn_status fwn_linear_grad_cast(const void* dy, int32_t dtype, int64_t ldy, int64_t m, int32_t n, void* cast, int64_t ldc,
-                                void* d_bias, int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  if (m < 0 || n <= 0 || m > INT32_MAX) return fail(FWN_ERR_INVALID_ARGUMENT, "bad shape m=%lld n=%d", static_cast<long long>(m), n);
-  if (!is_float_dtype(dtype) || !is_float_dtype(bias_dtype)) return fail(FWN_ERR_INVALID_ARGUMENT, "dy and d_bias are bf16 or float32");
-  if (m > 1 && (ldy < n || (cast && ldc < n))) return fail(FWN_ERR_INVALID_ARGUMENT, "a row stride is below n");
-  if (m > 0 && !dy) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
-  if (!cast && !d_bias) return ok();
-  size_t need = 0;
-  fwn_linear_grad_cast_workspace_size(m, n, &need);
-  if (d_bias && (!workspace || workspace_bytes < need || !aligned16(workspace)))
-    return fail(FWN_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed", need);
-  const int blocks = fwn::grad_cast_blocks(m, n, num_sms());
-  const bool wide = n % 8 == 0 && tma_rows(dy, dtype, m, ldy) && (!cast || tma_rows(cast, FWN_DTYPE_BF16, m, ldc));
-  float* part = d_bias ? static_cast<float*>(workspace) : nullptr;
-  cudaError_t e = fwn::launch_grad_cast(dy, dtype == FWN_DTYPE_F32, ldy, m, n, cast, ldc, part, blocks, wide,
-                                        static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return cuda_fail(e, "grad_cast");
-  if (d_bias && (e = fwn::launch_column_sum(part, blocks, n, d_bias, bias_dtype == FWN_DTYPE_BF16,
-                                            static_cast<cudaStream_t>(stream))) != cudaSuccess)
-    return cuda_fail(e, "column sums");
+fwn_status fwn_linear_bwd(const fwn_linear_desc* desc, const void* a, const void* b, const void* bias, const void* dy,
+                          void* d_a, void* d_b, void* d_bias, void* workspace, size_t workspace_bytes, void* stream) {
+  fwn_status s = check_linear_bwd(desc);
+  if (s != FWN_OK) return s;
+  const fwn_linear_desc& d = *desc;
+  if (!a || !b || !dy) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
+  if (d_bias && !bias) return fail(FWN_ERR_INVALID_ARGUMENT, "d_bias needs the bias");
+  const LinearBwdPlan pl = plan_linear_bwd(d, a, b, dy, num_sms());
+  if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned_to(workspace, 256)))
+    return fail(FWN_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) needed", pl.bytes);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const void* d_pre = pl.cast ? ws : dy;
+  ws += pl.off_ws;
+  if (d.act != FWN_ACT_NONE) {
+    s = fwn_linear(&pl.pre, a, nullptr, b, nullptr, bias, dy, workspace, d_bias, ws, pl.ws, stream);
+    if (s != FWN_OK) return s;
+  } else if (pl.cast || d_bias) {
+    const bool wide = d.n % 8 == 0 && tma_rows(dy, d.x_dtype, d.m, d.ldx);
+    float* part = d_bias ? reinterpret_cast<float*>(ws) : nullptr;
+    cudaError_t e = fwn::launch_grad_cast(dy, d.x_dtype == FWN_DTYPE_F32, d.ldx, d.m, d.n, pl.cast ? workspace : nullptr,
+                                          pl.ldp, part, pl.cast_blocks, wide, st);
+    if (e != cudaSuccess) return cuda_fail(e, "grad_cast");
+    if (d_bias && (e = fwn::launch_column_sum(part, pl.cast_blocks, d.n, d_bias, d.bias_dtype == FWN_DTYPE_BF16, st)) != cudaSuccess)
+      return cuda_fail(e, "column sums");
+  }
+  if (d_a) {
+    s = fwn_linear(&pl.da, d_pre, nullptr, b, nullptr, nullptr, nullptr, d_a, nullptr, ws, pl.ws, stream);
+    if (s != FWN_OK) return s;
+  }
+  if (d_b) {
+    const void* first = pl.db_turned ? a : d_pre;
+    const void* second = pl.db_turned ? d_pre : a;
+    s = fwn_linear(&pl.db, first, nullptr, second, nullptr, nullptr, nullptr, d_b, nullptr, ws, pl.ws, stream);
+    if (s != FWN_OK) return s;
+  }
   return ok();
 }
 

@@ -158,13 +158,11 @@ class _RmsNorm(torch.autograd.Function):
     desc = _lib.RmsDesc(rows, d, _CODE[x.dtype], 0 if ctx.residual_dtype is None else _CODE[ctx.residual_dtype],
                         0 if w is None else _CODE[w.dtype], _CODE[dh.dtype], 0, ctx.eps, 0, x.stride(0),
                         0 if r is None else r.stride(0))
-    lib, ws, size = _lib.lib(), None, ctypes.c_size_t(0)
-    if need_w:
-      _lib.check(lib.fwn_rms_norm_bwd_workspace_size(desc, size))
-      ws = x.new_empty((size.value,), dtype=torch.uint8)
+    lib = _lib.lib()
+    ws, size = _workspace(x, desc, lib.fwn_rms_norm_bwd_workspace_size) if need_w else (None, 0)
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     _lib.check(lib.fwn_rms_norm_bwd(desc, x.data_ptr(), ptr(r), ptr(w), dh.data_ptr(), ptr(ds), ptr(dx), ptr(dr), ptr(dw),
-                                    ptr(ws), size.value, stream))
+                                    ptr(ws), size, stream))
     return dx, dw, dr
 
 
@@ -231,9 +229,21 @@ def _padded(t):
 _WORKSPACE = {}
 
 
-def _product(stream, a, b, bias, x, act, out_dtype, a_scale=None, b_scale=None, pre_grad=False, d_bias=None, pad=False):
-  """act(a b^T + bias) + x for 2D a [m, k], b [n, k] in either orientation; pre_grad: x act'(a b^T + bias) with d_bias's
-  column sums. pad: the output's row stride is rounded up to 16 bytes (an operand of the next product)."""
+def _workspace(like, desc, size_of, *ptrs):
+  """(tensor or None, bytes) that `size_of` wants for a call with these operands."""
+  key = (bytes(desc), *[p & 15 for p in ptrs])
+  size = _WORKSPACE.get(key)
+  if size is None:
+    need = ctypes.c_size_t(0)
+    _lib.check(size_of(desc, *ptrs, need))
+    if len(_WORKSPACE) >= 4096:
+      _WORKSPACE.clear()
+    size = _WORKSPACE[key] = need.value
+  return like.new_empty((size,), dtype=torch.uint8) if size else None, size
+
+
+def _forward_launch(stream, a, b, bias, x, act, out_dtype, a_scale=None, b_scale=None):
+  """act(a b^T + bias) + x for 2D a [m, k], b [n, k] in either orientation."""
   m, k = a.shape
   n = b.shape[0]
   dtype = a.dtype
@@ -244,74 +254,36 @@ def _product(stream, a, b, bias, x, act, out_dtype, a_scale=None, b_scale=None, 
       a, lda, a_t = a.contiguous(), k, False
     if b_t:
       b, ldb, b_t = b.contiguous(), k, False
-  if pad and n % 8:
-    ldo = -(-n // 8) * 8
-    out = a.new_empty((m, ldo), dtype=out_dtype)[:, :n]
-  else:
-    ldo = n
-    out = a.new_empty((m, n), dtype=out_dtype)
-  flags = ((_lib.LINEAR_A_M_CONTIGUOUS if a_t else 0) | (_lib.LINEAR_B_N_CONTIGUOUS if b_t else 0) |
-           (_lib.LINEAR_PRE_GRAD if pre_grad else 0))
-  ap, bp, xp, x_code, ldx = a.data_ptr(), b.data_ptr(), None, 0, 0
-  if x is not None:
-    x = _rows(x)
-    xp, x_code, ldx = x.data_ptr(), _CODE[x.dtype], max(x.stride(0), n)
-  desc = _lib.LinearDesc(m, n, k, _CODE[dtype], _CODE[out_dtype], 0 if bias is None else _CODE[bias.dtype], x_code, act,
-                         flags, lda, ldb, ldx, ldo)
+  out = a.new_empty((m, n), dtype=out_dtype)
+  flags = (_lib.LINEAR_A_M_CONTIGUOUS if a_t else 0) | (_lib.LINEAR_B_N_CONTIGUOUS if b_t else 0)
+  ap, bp = a.data_ptr(), b.data_ptr()
+  desc = _lib.LinearDesc(m, n, k, _CODE[dtype], _CODE[out_dtype], 0 if bias is None else _CODE[bias.dtype],
+                         0 if x is None else _CODE[x.dtype], act, flags, lda, ldb,
+                         0 if x is None else max(x.stride(0), n), n)
   lib = _lib.lib()
-  key = (bytes(desc), ap & 15, bp & 15)
-  size = _WORKSPACE.get(key)
-  if size is None:
-    need = ctypes.c_size_t(0)
-    _lib.check(lib.fwn_linear_workspace_size(desc, ap, bp, need))
-    if len(_WORKSPACE) >= 4096:
-      _WORKSPACE.clear()
-    size = _WORKSPACE[key] = need.value
-  ws = a.new_empty((size,), dtype=torch.uint8) if size else None
+  ws, size = _workspace(a, desc, lib.fwn_linear_workspace_size, ap, bp)
   status = lib.fwn_linear(desc, ap, None if a_scale is None else a_scale.data_ptr(), bp,
-                          None if b_scale is None else b_scale.data_ptr(), None if bias is None else bias.data_ptr(), xp,
-                          out.data_ptr(), None if d_bias is None else d_bias.data_ptr(),
+                          None if b_scale is None else b_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+                          None if x is None else x.data_ptr(), out.data_ptr(), None,
                           None if ws is None else ws.data_ptr(), size, stream)
   if status:
     _lib.check(status)
   return out
 
 
-def _pre_gradient(stream, a, weight, bias, act, dy, need_bias):
-  """(gradient of the pre-activation in bf16, gradient of the bias or None) for dy [m, n]."""
-  m, n = dy.shape
-  d_bias = torch.empty_like(bias) if need_bias else None
-  if act != _lib.ACT_NONE:
-    return _product(stream, a, weight, bias, dy, act, _BF16, pre_grad=True, d_bias=d_bias, pad=True), d_bias
-  dy = _rows(dy)
-  cast = None
-  if dy.dtype is not _BF16:
-    cast = dy.new_empty((m, -(-n // 8) * 8), dtype=_BF16)[:, :n]
-  if cast is not None or need_bias:
-    lib, size, ws = _lib.lib(), ctypes.c_size_t(0), None
-    if need_bias:
-      _lib.check(lib.fwn_linear_grad_cast_workspace_size(m, n, size))
-      ws = dy.new_empty((size.value,), dtype=torch.uint8)
-    _lib.check(lib.fwn_linear_grad_cast(dy.data_ptr(), _CODE[dy.dtype], max(dy.stride(0), n), m, n,
-                                        None if cast is None else cast.data_ptr(),
-                                        0 if cast is None else cast.stride(0),
-                                        None if d_bias is None else d_bias.data_ptr(),
-                                        0 if bias is None else _CODE[bias.dtype], None if ws is None else ws.data_ptr(),
-                                        size.value, stream))
-  return dy if cast is None else cast, d_bias
-
-
 class _Linear(torch.autograd.Function):
-  """linear with gradients. The backward recomputes the pre-activation inside the product that turns dy into its
-  gradient (x act'(a w^T + bias), with the bias gradient's column sums), then takes d_a = d_pre w and
+  """linear with gradients. The backward (fwn_linear_bwd) recomputes the pre-activation inside the product that turns dy
+  into its gradient (x act'(a w^T + bias), with the bias gradient's column sums), then takes d_a = d_pre w and
   d_weight = d_pre^T a on the same kernel; the residual's gradient is dy."""
 
   @staticmethod
   def forward(ctx, a, weight, bias, residual, act, out_dtype):
     ctx.act, ctx.shape = act, a.shape
     a2, w2 = _padded(_rows(a)), _padded(weight)
+    if bias is not None and not bias.is_contiguous():
+      bias = bias.contiguous()
     ctx.save_for_backward(a2, w2, bias)
-    y = _linear_forward(a2, w2, bias, None if residual is None else _rows(residual), act, out_dtype)
+    y = _on_device(a2, _forward_launch, a2, w2, bias, None if residual is None else _rows(residual), act, out_dtype)
     return y if a.dim() == 2 else y.view(*a.shape[:-1], weight.shape[0])
 
   @staticmethod
@@ -319,37 +291,44 @@ class _Linear(torch.autograd.Function):
     a, weight, bias = ctx.saved_tensors
     need_a, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     d_a = d_w = d_b = None
-    if a.numel() == 0:
+    if a.shape[0] == 0:
       d_a = a.new_zeros(ctx.shape) if need_a else None
       d_w = torch.zeros_like(weight) if need_w else None
       d_b = torch.zeros_like(bias) if need_b else None
     elif need_a or need_w or need_b:
-      d_a, d_w, d_b = _on_device(a, _Linear._launch, a, weight, bias, ctx.act, dy, need_a, need_w, need_b)
+      d_a, d_w, d_b = _on_device(a, _Linear._launch, a, weight, bias, ctx.act,
+                                 _rows(dy if dy.dim() == 2 else dy.reshape(a.shape[0], -1)), need_a, need_w, need_b)
       if need_a and len(ctx.shape) != 2:
         d_a = d_a.view(ctx.shape)
     return d_a, d_w, d_b, dy if need_r else None, None, None
 
   @staticmethod
   def _launch(stream, a, weight, bias, act, dy, need_a, need_w, need_b):
+    m, k = a.shape
     n = weight.shape[0]
-    d_a = d_w = None
-    d_pre, d_b = _pre_gradient(stream, a, weight, None if bias is None else bias.contiguous(), act,
-                               dy if dy.dim() == 2 else dy.reshape(-1, n), need_b)
-    if need_a:
-      d_a = _product(stream, d_pre, weight.t(), None, None, _lib.ACT_NONE, _BF16)
-    if need_w:
-      # In the weight's own orientation, so that the gradient's rows are written as they lie.
-      if weight.stride(0) == 1 and weight.stride(1) != 1:
-        d_w = _product(stream, a.t(), d_pre.t(), None, None, _lib.ACT_NONE, _BF16).t()
-      else:
-        d_w = _product(stream, d_pre.t(), a.t(), None, None, _lib.ACT_NONE, _BF16)
-    return d_a, d_w, d_b
+    a, lda, a_t = _orient(a)
+    b, ldb, b_t = _orient(weight)
+    d_a = a.new_empty((m, k)) if need_a else None
+    d_w = a.new_empty((k, n) if b_t else (n, k)) if need_w else None
+    d_b = torch.empty_like(bias) if need_b else None
+    flags = (_lib.LINEAR_A_M_CONTIGUOUS if a_t else 0) | (_lib.LINEAR_B_N_CONTIGUOUS if b_t else 0)
+    ap, bp, dp = a.data_ptr(), b.data_ptr(), dy.data_ptr()
+    desc = _lib.LinearDesc(m, n, k, _lib.DTYPE_BF16, _CODE[dy.dtype], 0 if bias is None else _CODE[bias.dtype],
+                           _CODE[dy.dtype], act, flags, lda, ldb, max(dy.stride(0), n), n)
+    lib = _lib.lib()
+    ws, size = _workspace(a, desc, lib.fwn_linear_bwd_workspace_size, ap, bp, dp)
+    status = lib.fwn_linear_bwd(desc, ap, bp, None if bias is None else bias.data_ptr(), dp,
+                                None if d_a is None else d_a.data_ptr(), None if d_w is None else d_w.data_ptr(),
+                                None if d_b is None else d_b.data_ptr(), None if ws is None else ws.data_ptr(), size, stream)
+    if status:
+      _lib.check(status)
+    return d_a, d_w.t() if b_t and need_w else d_w, d_b
 
 
 def _linear_forward(a, weight, bias, residual, act, out_dtype, a_scale=None, b_scale=None):
   if bias is not None and not bias.is_contiguous():
     bias = bias.contiguous()
-  out = _on_device(a, _product, _rows(a), weight, bias, None if residual is None else _rows(residual), act, out_dtype,
+  out = _on_device(a, _forward_launch, _rows(a), weight, bias, None if residual is None else _rows(residual), act, out_dtype,
                    a_scale, b_scale)
   return out if a.dim() == 2 else out.view(*a.shape[:-1], weight.shape[0])
 

@@ -324,7 +324,7 @@ FWN_API fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, con
  * FWN_LINEAR_PRE_GRAD: the backward's first step, out = x act'(a b^T + bias) in bf16 with x = the gradient of the
  * forward's output ([m, n], bf16 or float32): the gradient of the pre-activation, which is computed again here rather
  * than kept. d_bias (NULL, or [n] in bias_dtype) receives its column sums, taken in float32 before the rounding, in a
- * fixed order. The gradients of a and b are products of the same kind with out as an operand. */
+ * fixed order. fwn_linear_bwd does it and the two products that follow. */
 typedef struct fwn_linear_desc {
   int64_t m;
   int32_t n;
@@ -352,12 +352,15 @@ FWN_API fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const 
                               const float* b_scale, const void* bias, const void* x, void* out, void* d_bias,
                               void* workspace, size_t workspace_bytes, void* stream);
 
-/* The backward's first step without an activation: cast (bf16 [m, n], row stride ldc, or NULL) = dy rounded, d_bias
- * ([n] in bias_dtype, or NULL) = the column sums of dy (float32, fixed order). Workspace for d_bias, 16-byte aligned. */
-FWN_API fwn_status fwn_linear_grad_cast_workspace_size(int64_t m, int32_t n, size_t* bytes);
-FWN_API fwn_status fwn_linear_grad_cast(const void* dy, int32_t dtype, int64_t ldy, int64_t m, int32_t n, void* cast,
-                                        int64_t ldc, void* d_bias, int32_t bias_dtype, void* workspace,
-                                        size_t workspace_bytes, void* stream);
+/* The whole backward: desc as the forward's (bf16 operands, flags without FWN_LINEAR_PRE_GRAD), with x_dtype and ldx of dy
+ * [m, n], the gradient of the output. d_pre = dy act'(a b^T + bias) (dy itself without an activation) in bf16, then
+ * d_a [m, k] = d_pre b, d_b = d_pre^T a in b's own orientation (both bf16, contiguous) and d_bias [n] in bias_dtype; each
+ * may be NULL (d_bias: must be without a bias). The residual's gradient is dy. Deterministic. m >= 1. */
+FWN_API fwn_status fwn_linear_bwd_workspace_size(const fwn_linear_desc* desc, const void* a, const void* b, const void* dy,
+                                                 size_t* bytes);
+FWN_API fwn_status fwn_linear_bwd(const fwn_linear_desc* desc, const void* a, const void* b, const void* bias,
+                                  const void* dy, void* d_a, void* d_b, void* d_bias, void* workspace,
+                                  size_t workspace_bytes, void* stream);
 
 /* ---- grid <-> mesh interaction networks -------------------------------------------------------------------
  * The blocked GNNs of the encoder / decoder (src/faster_weathernext/patch.py:347-509, ChunkedDeepGNN: edge MLP on
