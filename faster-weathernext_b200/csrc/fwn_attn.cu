@@ -1178,6 +1178,7 @@ struct LinearPlan {
 // act'() k 1,024 447 / 418, k 1,536 (n 512) 268 / 334.
 bool long_form(const fwn_linear_desc& d, int64_t kb) {
   if (d.flags & FWN_LINEAR_PRE_GRAD) return kb >= 20;
+  if (d.ldo * dtype_size(d.out_dtype) % 16 != 0) return kb >= 20;  // an epilogue of plain stores (odd widths)
   if (d.act != FWN_ACT_NONE) return kb >= 10;
   return d.dtype == FWN_DTYPE_E4M3 ? kb >= 6 : true;
 }
@@ -1321,7 +1322,7 @@ fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const float* a
   p.n_tiles = (d.n + tn - 1) / tn;
   p.splits = pl.splits;
   p.k_blocks = static_cast<int>((static_cast<int64_t>(d.k) * es + 127) / 128);
-  p.chunk = p.out_f32 ? fwn::kLinearChunk : p.k_blocks;
+  p.chunk = p.out_f32 || (d_bias && !p.bias_bf16) ? fwn::kLinearChunk : p.k_blocks;
   const int64_t items = static_cast<int64_t>(p.m_tiles) * p.n_tiles * p.splits;
   if (items > INT32_MAX - 1024) return fail(FWN_ERR_UNSUPPORTED, "m=%lld n=%d too large", static_cast<long long>(d.m), d.n);
   p.items = static_cast<int>(items);

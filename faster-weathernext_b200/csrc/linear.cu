@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "linear.cuh"
@@ -292,7 +293,7 @@ __device__ __forceinline__ void activate4_short(float* v) {
 //
 // float32 results: the tensor core truncates its running sum at every step, an error that grows with k (measured 1.5e-6
 // of the result at k = 2,048). They take k in chunks (p.chunk stages) into alternate accumulators, which the epilogue
-// warps add in float32 registers (64 a thread).
+// warps add in float32 registers (64 a thread); so does act'(), where it makes a float32 bias gradient.
 template <int TILE, bool X32, bool O32, bool PRE, bool SUM>
 struct LinearCfg {
   static constexpr int CG = linear_pair(TILE) ? 2 : 1;
@@ -601,6 +602,65 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
         }
       }
     };
+    auto free_slot = [&] {  // the slot's last store has read it
+      if (!p.out_direct && elect_one_sync()) store_wait_read<0>();
+      __syncwarp();
+    };
+    // Rows that TMA cannot address (x or the output): lane = column, so that a row's 32 values are one access; eight
+    // rows in flight, one pointer a row.
+    auto gather_x = [&](int64_t row0, int col) {
+      using T = std::conditional_t<X32, uint32_t, uint16_t>;
+      const T* src = static_cast<const T*>(p.x) + row0 * p.ldx + col + lane;
+      const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - row0));
+      const bool in0 = col + lane < p.n, in1 = CC == 64 && col + 32 + lane < p.n;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += 8) {
+        T t[8][2];
+#pragma unroll
+        for (int r = 0; r < 8; ++r, src += p.ldx) {
+          const bool in = r0 + r < rows;
+          t[r][0] = in && in0 ? __ldg(src) : T(0);
+          if (CC == 64) t[r][1] = in && in1 ? __ldg(src + 32) : T(0);
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const uint32_t at = slot + r0 * C::X_ROW + byte_at<C::X_ROW>(r, static_cast<int>(sizeof(T)) * lane);
+          if constexpr (X32) {
+            st_shared_u32(at, t[r][0]);
+          } else {
+            st_shared_u16(at, t[r][0]);
+            if (CC == 64) st_shared_u16(at ^ 64u, t[r][1]);
+          }
+        }
+      }
+      __syncwarp();
+    };
+    auto scatter_out = [&](int64_t row0, int col) {
+      using T = std::conditional_t<O32, uint32_t, uint16_t>;
+      T* dst = static_cast<T*>(p.out) + row0 * p.ldo + col + lane;
+      const int rows = static_cast<int>(min(static_cast<int64_t>(32), p.m - row0));
+      const bool in0 = col + lane < p.n, in1 = CC == 64 && col + 32 + lane < p.n;
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 8) {
+        T t[8][2];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const uint32_t at = slot + r0 * C::O_ROW + byte_at<C::O_ROW>(r, static_cast<int>(sizeof(T)) * lane);
+          if constexpr (O32) {
+            t[r][0] = ld_shared_u32(at);
+          } else {
+            t[r][0] = ld_shared_u16(at);
+            if (CC == 64) t[r][1] = ld_shared_u16(at ^ 64u);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r, dst += p.ldo) {
+          const bool in = r0 + r < rows;
+          if (in && in0) *dst = t[r][0];
+          if (CC == 64 && in && in1) dst[32] = t[r][1];
+        }
+      }
+    };
     auto combine = [&](float& v, float x) { v = PRE ? v * x : v + x; };  // dy times the slope; the residual is added
     TileWalk w(p, first);
     if (x_tma && elect_one_sync()) issue_x(w, 0);
@@ -623,6 +683,10 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
       rs = 1.f;
       if (p.a_scale != nullptr && row0 + lane < p.m) rs = p.a_scale[row0 + lane];
       __syncwarp();
+      if (has_x && !x_tma) {  // the first chunk's x while the MMAs run
+        free_slot();
+        gather_x(row0, col0);
+      }
       int buf = acc_i & 1;
       float sum[SUM ? C::HC : 1];
       if constexpr (SUM) {
@@ -654,25 +718,9 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
         const int col = col0 + CC * ch;
         if (x_tma) {
           if (!(ok = idle_wait(x_bar(ew), q & 1, abort_flag))) goto done;
-        } else {
-          if (!p.out_direct && elect_one_sync()) store_wait_read<0>();  // the slot's last store
-          __syncwarp();
-          if (has_x) {
-            // Rows that TMA cannot address: lane = column, so that a row's values are one access.
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r) {
-#pragma unroll
-              for (int j = lane; j < CC; j += 32) {
-                const bool in = row0 + r < p.m && col + j < p.n;
-                const int64_t at = (row0 + r) * p.ldx + col + j;
-                if constexpr (X32)
-                  st_shared_u32(slot + byte_at<C::X_ROW>(r, 4 * j), in ? static_cast<const uint32_t*>(p.x)[at] : 0u);
-                else
-                  st_shared_u16(slot + byte_at<C::X_ROW>(r, 2 * j), in ? static_cast<const uint16_t*>(p.x)[at] : uint16_t(0));
-              }
-            }
-            __syncwarp();
-          }
+        } else if (ch > 0 || !has_x) {
+          free_slot();
+          if (has_x) gather_x(row0, col);
         }
 #pragma unroll
         for (int h = 0; h < CC; h += 32) {
@@ -760,19 +808,7 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
         }
         if (p.out_direct) {
           __syncwarp();
-#pragma unroll 4
-          for (int r = 0; r < 32; ++r) {
-#pragma unroll
-            for (int j = lane; j < CC; j += 32) {
-              if (row0 + r < p.m && col + j < p.n) {
-                const int64_t at = (row0 + r) * p.ldo + col + j;
-                if constexpr (O32)
-                  static_cast<uint32_t*>(p.out)[at] = ld_shared_u32(slot + byte_at<C::O_ROW>(r, 4 * j));
-                else
-                  static_cast<uint16_t*>(p.out)[at] = ld_shared_u16(slot + byte_at<C::O_ROW>(r, 2 * j));
-              }
-            }
-          }
+          scatter_out(row0, col);
         }
         // The slot's writes before the store that reads them, its reads before the copy that overwrites them (without
         // the proxy fence loads were still on their way when the next chunk landed).
@@ -852,12 +888,16 @@ cudaError_t by_act(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
 template <int TILE>
 cudaError_t by_type(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx, const CUtensorMap& to,
                     const LinearParams& p, int sms, cudaStream_t st) {
-  if (p.pre_grad)
+  const bool sum = (p.k_blocks + p.splits - 1) / p.splits > p.chunk;  // more than one chunk of k: added in registers
+  if (p.pre_grad) {
+    if (sum)
+      return p.x_f32 ? by_act<TILE, true, false, true, true>(ta, tb, tx, to, p, sms, st)
+                     : by_act<TILE, false, false, true, true>(ta, tb, tx, to, p, sms, st);
     return p.x_f32 ? by_act<TILE, true, false, true, false>(ta, tb, tx, to, p, sms, st)
                    : by_act<TILE, false, false, true, false>(ta, tb, tx, to, p, sms, st);
+  }
   if (!p.out_f32) return by_act<TILE, false, false, false, false>(ta, tb, tx, to, p, sms, st);
-  // More than one chunk of k in a split: added in registers.
-  return (p.k_blocks + p.splits - 1) / p.splits > p.chunk ? by_act<TILE, true, true, false, true>(ta, tb, tx, to, p, sms, st)
+  return sum ? by_act<TILE, true, true, false, true>(ta, tb, tx, to, p, sms, st)
                                                           : by_act<TILE, true, true, false, false>(ta, tb, tx, to, p, sms, st);
 }
 
