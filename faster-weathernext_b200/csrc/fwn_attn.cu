@@ -1052,7 +1052,7 @@ fwn_status fwn_rms_norm_bwd_workspace_size(const fwn_rms_desc* desc, size_t* byt
   // The mode goes by the operands' addresses too: the most that any of them needs.
   int blocks = 0;
   const int sms = num_sms();
-  for (int mode = 0; mode < 3; ++mode) blocks = std::max(blocks, fwn::rms_bwd_blocks(desc->rows, desc->d, sms, mode));
+  for (int mode = 0; mode < 3; ++mode) blocks = std::max(blocks, fwn::rms_bwd_blocks(desc->rows, desc->d, sms, mode, desc->x_dtype == FWN_DTYPE_BF16));
   *bytes = static_cast<size_t>(blocks) * desc->d * sizeof(float);
   if (*bytes < 16) *bytes = 16;
   return ok();
@@ -1099,7 +1099,7 @@ fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, const void*
                       starts_wide(dh, d.out_dtype) && starts_wide(ds, d.x_dtype) && starts_wide(dx, d.x_dtype) &&
                       starts_wide(d_residual, d.residual_dtype);
   p.mode = rms_row_mode(d, starts, residual != nullptr, weight);
-  cudaError_t e = fwn::launch_rms_norm_bwd(p, fwn::rms_bwd_blocks(d.rows, d.d, num_sms(), p.mode),
+  cudaError_t e = fwn::launch_rms_norm_bwd(p, fwn::rms_bwd_blocks(d.rows, d.d, num_sms(), p.mode, p.x_bf16),
                                            static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "rms_norm_bwd");
   return ok();

@@ -6,16 +6,16 @@
 // where it is stored.
 //
 // Bound: HBM. A row is read once, kept in registers (at most 32 values per thread) through the sum of squares (and the
-// row maximum of the 8-bit output) and written once. A row of up to 1,024 values belongs to one warp, of up to 8,192
-// to a block of 256 threads, of up to 16,384 to one of 1,024: the smallest group that holds the row in registers
-// needs the fewest exchanges. Three ways to lay a row over its threads:
+// row maximum of the 8-bit output) and written once. 8 to 512 threads take a row (the gradient: to 1,024), the smallest
+// group that holds it in registers: it needs the fewest exchanges and has the most bytes on their way per thread; where
+// those are few (bf16 rows), a group takes up to four rows at once. Three ways to lay a row over its threads:
 //   kWide    8 values per thread and access (16 bytes of bf16, 32 of float32, the widest accesses of sm_100): widths
 //            and strides that are multiples of 8;
 //   kShift   the same accesses for rows of any width that follow one another without gaps: groups of 8 start at the
 //            aligned address before the row, and only the two that its ends cut go by single values. A group of threads
 //            takes rows eight apart, whose starts are off alike, so that a thread keeps its columns (its weights, its
 //            share of the weight's gradient) from row to row, and the next row's loads are issued before the work on
-//            one. 10,242 x 1,001 bf16 with a bf16 residual, forward / backward: kScalar 41 / 165 us, kShift 22 / 35;
+//            one. 10,242 x 1,001 bf16 with a bf16 residual, forward / backward: kScalar 41 / 165 us, kShift 19 / 36;
 //   kScalar  one value per thread and access: other strides and addresses.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -148,26 +148,36 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// Sum (or NaN-keeping maximum) over the TPR threads of a row, the same in each. `red` holds one value per warp and is
-// used once per call site and row, so the block form needs a barrier before the next row's use (two alternate).
-template <int TPR, bool MAX>
-__device__ __forceinline__ float row_reduce(float v, float* red) {
+// Threads of a block whose rows take TPR threads: eight rows or more where a row is at most a warp's, else one.
+constexpr int block_of(int tpr) { return tpr <= 32 ? 256 : tpr; }
+
+// Sums (or NaN-keeping maxima) of N values over the TPR threads of a row, the same in each. `red` (N x 32) holds one value
+// per warp and is written once per row, so that rows alternate between two of them.
+template <int TPR, bool MAX, int N>
+__device__ __forceinline__ void row_reduce(float (&v)[N], float (*red)[32]) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? max_nan(v, u) : v + u;
-  }
-  if constexpr (TPR > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[threadIdx.x & (TPR / 32 - 1)];
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
 #pragma unroll
-    for (int o = TPR / 64; o > 0; o >>= 1) {
-      const float u = __shfl_xor_sync(0xffffffffu, v, o);
-      v = MAX ? max_nan(v, u) : v + u;
+    for (int i = 0; i < N; ++i) {
+      const float u = __shfl_xor_sync(0xffffffffu, v[i], o);
+      v[i] = MAX ? max_nan(v[i], u) : v[i] + u;
     }
   }
-  return v;
+  if constexpr (TPR > 32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((threadIdx.x & 31) == 0) red[i][threadIdx.x >> 5] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = red[i][threadIdx.x & (TPR / 32 - 1)];
+#pragma unroll
+      for (int o = TPR / 64; o > 0; o >>= 1) {
+        const float u = __shfl_xor_sync(0xffffffffu, v[i], o);
+        v[i] = MAX ? max_nan(v[i], u) : v[i] + u;
+      }
+    }
+  }
 }
 
 enum RowMode { kScalar = 0, kWide = 1, kShift = 2 };
@@ -175,8 +185,7 @@ enum RowMode { kScalar = 0, kWide = 1, kShift = 2 };
 // Column of a thread's i-th group of V values; `off` (kShift) is how far the row starts past an aligned address.
 template <int TPR, int V>
 __device__ __forceinline__ int group_at(int i, int off) {
-  const int t = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
-  return (i * TPR + t) * V - off;
+  return (i * TPR + static_cast<int>(threadIdx.x & (TPR - 1))) * V - off;
 }
 // The group of values from column j of the row at p. `more`: rows follow, so that a group which the row's end cuts may be
 // read whole (kShift: what lies before a row is the row before); the last row's goes by single values.
@@ -252,15 +261,36 @@ constexpr float kE4m3Max = 448.f;
 // A row whose largest value is below this has scale 0 and values 0 (its scale's reciprocal would leave float32).
 constexpr float kTinyRow = 7.8886090522101181e-31f;  // 2^-100
 
-// TPR threads per row (32: a warp, eight rows per block of 256; else the block), NV groups of V values per thread. The
-// grid covers the rows, or (kShift) a multiple of eight blocks walks them.
+// The rows of a group of TPR threads: `row`, then `step` further on each time. Groups of one warp have adjacent rows and
+// leave together (`base`, the row of the warp's first group, decides); kShift: `step` is a multiple of eight.
+template <int TPR>
+struct Rows {
+  int64_t row, base, step;
+  __device__ __forceinline__ Rows() {
+    constexpr int GROUPS = block_of(TPR) / TPR, PER_WARP = TPR < 32 ? 32 / TPR : 1;
+    const int g = threadIdx.x / TPR;
+    row = static_cast<int64_t>(blockIdx.x) * GROUPS + g;
+    base = row - g % PER_WARP;
+    step = static_cast<int64_t>(gridDim.x) * GROUPS;
+  }
+};
+
+// Rows that a group works on at once, so that a thread has some 64 bytes on their way: bf16 rows of few values per thread.
+template <class X, class R, int MODE>
+constexpr int rows_at_once(int nv) {
+  if (MODE != kWide) return MODE == kShift && nv == 1 && sizeof(X) == 2 ? 2 : 1;
+  const int bytes = nv * 8 * (static_cast<int>(sizeof(X)) + (is_none<R> ? 0 : static_cast<int>(sizeof(R))));
+  return bytes <= 16 ? 4 : bytes <= 32 ? 2 : 1;
+}
+
+// TPR threads per row, NV groups of V values per thread.
 template <class X, class R, class O, int TPR, int MODE, int NV>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 1024 ? 1 : 2) rms_norm_kernel(const RmsParams p) {
+__global__ void __launch_bounds__(block_of(TPR), TPR > 512 ? 1 : 512 / block_of(TPR)) rms_norm_kernel(const RmsParams p) {
   constexpr int V = MODE == kScalar ? 1 : 8;
-  __shared__ float red[4][32];
-  const int64_t first = TPR == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (TPR == 32 ? 8 : 1);
-  const int off = MODE == kShift ? static_cast<int>(first * p.d & 7) : 0;  // of all this group's rows
+  constexpr int U = rows_at_once<X, R, MODE>(NV);
+  __shared__ float red[2][2][U][32];
+  Rows<TPR> at;
+  const int off = MODE == kShift ? static_cast<int>(at.row * p.d & 7) : 0;  // of all this group's rows
   const int d = p.d;
   float w[MODE == kShift ? NV : 1][V];
   if constexpr (MODE == kShift) {
@@ -276,109 +306,145 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, TPR == 1024 ? 1 : 2) rm
   }
   using RR = std::conditional_t<is_none<R>, float, R>;
   constexpr int NR = is_none<R> ? 1 : NV;
-  constexpr bool kAhead = MODE == kShift;  // the next row is on its way while one is worked on
-  Raw<X, V> xs[kAhead ? NV : 1];
-  Raw<RR, V> rs[kAhead ? NR : 1];
+  // kShift: the next rows are on their way while some are worked on.
+  constexpr bool kAhead = MODE == kShift;
+  Raw<X, V> xs[kAhead ? U : 1][kAhead ? NV : 1];
+  Raw<RR, V> rs[kAhead ? U : 1][kAhead ? NR : 1];
   auto fetch = [&](int64_t row, int i, Raw<X, V>& a, Raw<RR, V>& b) {
-    const int j = group_at<TPR, V>(i, off);
-    load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, d, row + 1 < p.rows, a);
+    const int j = group_at<TPR, V>(i, off), n = row < p.rows ? d : 0;
+    load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, row + 1 < p.rows, a);
     if constexpr (!is_none<R>)
-      load_group<MODE>(static_cast<const R*>(p.residual) + row * p.residual_stride, j, d, row + 1 < p.rows, b);
+      load_group<MODE>(static_cast<const R*>(p.residual) + row * p.residual_stride, j, n, row + 1 < p.rows, b);
   };
-  auto fetch_row = [&](int64_t row) {
-    if (!kAhead || row >= p.rows) return;
+  auto fetch_rows = [&](int64_t row) {
+    if constexpr (kAhead) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) fetch(row, i, xs[kAhead ? i : 0], rs[kAhead && !is_none<R> ? i : 0]);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) fetch(row + u * at.step, i, xs[u][i], rs[u][is_none<R> ? 0 : i]);
+    }
   };
-  fetch_row(first);
+  fetch_rows(at.row);
   int flip = 0;
-  for (int64_t row = first; row < p.rows; row += step, flip ^= 2) {  // whole warps (blocks) leave together
-    float s[NV][V], r[NR][V];
+  for (; at.base < p.rows; at.base += U * at.step, at.row += U * at.step, flip ^= 1) {
+    float s[U][NV][V], ss[U];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, V>(i, off);
-      Raw<X, V> a;
-      Raw<RR, V> b;
-      if constexpr (kAhead) {
-        a = xs[i];
-        b = rs[is_none<R> ? 0 : i];
-      } else {
-        fetch(row, i, a, b);
+    for (int u = 0; u < U; ++u) {
+      const int n = at.row + u * at.step < p.rows ? d : 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = group_at<TPR, V>(i, off);
+        Raw<X, V> a;
+        Raw<RR, V> b;
+        if constexpr (kAhead) {
+          a = xs[u][i];
+          b = rs[u][is_none<R> ? 0 : i];
+        } else {
+          fetch(at.row + u * at.step, i, a, b);
+        }
+        expand<MODE>(a, j, n, s[u][i]);
+        if constexpr (!is_none<R>) {
+          float r[V];
+          expand<MODE>(b, j, n, r);
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[u][i][e] += r[e];
+        }
       }
-      expand<MODE>(a, j, d, s[i]);
-      if constexpr (!is_none<R>) expand<MODE>(b, j, d, r[i]);
     }
-    fetch_row(row + step);
-    float ss = 0.f;
+    if constexpr (kAhead) {
+      if (at.base + U * at.step < p.rows) fetch_rows(at.row + U * at.step);
+    }
+    float rstd[U];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if constexpr (!is_none<R>) {
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = at.row + u * at.step;
+      const int n = row < p.rows ? d : 0;
+      ss[u] = 0.f;
+      rstd[u] = 1.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] += r[i][e];
-        store_group<MODE>(static_cast<X*>(p.x_out) + row * d, group_at<TPR, V>(i, off), d, s[i]);
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (!is_none<R>) store_group<MODE>(static_cast<X*>(p.x_out) + row * d, group_at<TPR, V>(i, off), n, s[u][i]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) ss[u] = fmaf(s[u][i][e], s[u][i][e], ss[u]);
       }
-#pragma unroll
-      for (int e = 0; e < V; ++e) ss = fmaf(s[i][e], s[i][e], ss);
     }
-    float rstd = 1.f;
     if (p.normalize) {
-      ss = row_reduce<TPR, false>(ss, red[flip]);
-      rstd = rsqrtf(ss / static_cast<float>(d) + p.eps);
+      row_reduce<TPR, false>(ss, red[flip][0]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) rstd[u] = rsqrtf(ss[u] / static_cast<float>(d) + p.eps);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if constexpr (MODE == kShift) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] = s[i][e] * rstd * w[i][e];
-      } else if (p.weight != nullptr) {
+      if (MODE != kShift && p.weight != nullptr)
         weight_group<MODE>(p.weight, p.weight_bf16, group_at<TPR, V>(i, off), d, w[0]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] = s[i][e] * rstd * w[0][e];
-      } else {
+      for (int u = 0; u < U; ++u) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] *= rstd;
+        for (int e = 0; e < V; ++e) {
+          s[u][i][e] *= rstd[u];
+          if (MODE == kShift || p.weight != nullptr) s[u][i][e] *= w[MODE == kShift ? i : 0][e];
+        }
       }
     }
     if constexpr (sizeof(O) == 1) {
-      float m = 0.f;
+      float m[U];
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+      for (int u = 0; u < U; ++u) {
+        m[u] = 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) m = max_nan(m, fabsf(s[i][e]));
-      m = row_reduce<TPR, true>(m, red[flip + 1]);
-      const bool tiny = m < kTinyRow;  // false for NaN, which the scale and the values keep
-      const float inv = tiny ? 0.f : kE4m3Max / m;
-      if ((TPR == 32 ? (threadIdx.x & 31) : threadIdx.x) == 0) p.scale[row] = tiny ? 0.f : m / kE4m3Max;
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+          for (int e = 0; e < V; ++e) m[u] = max_nan(m[u], fabsf(s[u][i][e]));
+      }
+      row_reduce<TPR, true>(m, red[flip][1]);
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] *= inv;
+      for (int u = 0; u < U; ++u) {
+        const int64_t row = at.row + u * at.step;
+        const bool tiny = m[u] < kTinyRow;  // false for NaN, which the scale and the values keep
+        const float inv = tiny ? 0.f : kE4m3Max / m[u];
+        if ((threadIdx.x & (TPR - 1)) == 0 && row < p.rows) p.scale[row] = tiny ? 0.f : m[u] / kE4m3Max;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[u][i][e] *= inv;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store_group<MODE>(static_cast<O*>(p.out) + row * d, group_at<TPR, V>(i, off), d, s[i]);
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = at.row + u * at.step;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        store_group<MODE>(static_cast<O*>(p.out) + row * d, group_at<TPR, V>(i, off), row < p.rows ? d : 0, s[u][i]);
+    }
   }
 }
 
-// Blocks of the gradient's kernel that an SM holds, by the threads of a row and the values of a thread: five arrays of
-// values and some 30 registers a thread.
-constexpr int bwd_resident(int tpr, int values) {
-  return tpr == 1024 ? 1 : tpr == 128 ? 4 : values <= 8 && tpr == 32 ? 3 : 2;
+// Blocks of the gradient's kernel that an SM holds: five arrays of a thread's values and some 40 registers a thread, or
+// fewer where no row is read ahead.
+template <class X, int MODE>
+constexpr bool bwd_ahead(int nv) { return nv == 1 && (MODE == kShift || sizeof(X) == 2); }
+template <class X, int MODE>
+constexpr int bwd_at_once(int nv) { return MODE == kWide && nv == 1 && sizeof(X) == 2 ? 2 : 1; }  // rows, as rows_at_once
+template <class X, int MODE>
+constexpr int bwd_resident(int tpr, int nv) {
+  return tpr > 512 ? 1 : (MODE == kWide && nv == 1 && !bwd_ahead<X, MODE>(nv) ? 768 : 512) / block_of(tpr);
 }
 
 // Gradient, with g = dh weight, s the normalised row (x, or x + residual), ds the gradient of the stored sum:
 //   dx = rstd g - s rstd^3 mean(g s) + ds,  d_residual = dx,  dweight = sum over rows of dh s rstd.
-// A group of TPR threads walks rows (grid-stride); its columns' share of dweight stays in registers and leaves as one
-// row of partials per block (the warps of a block are added through shared memory), summed in order by
-// column_sum_kernel: no atomics, the same bits every time. All of a row's loads are issued before its sums are needed.
+// A group of TPR threads walks rows; its columns' share of dweight stays in registers and leaves as one row of partials
+// per block (a block's groups are added through shared memory), summed in order by column_sum_kernel: no atomics, the
+// same bits every time. All of a row's loads are issued before its sums are needed.
 template <class X, class R, class G, int TPR, int MODE, int NV>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, bwd_resident(TPR, NV * (MODE == kScalar ? 1 : 8)))
+__global__ void __launch_bounds__(block_of(TPR), (bwd_resident<X, MODE>(TPR, NV)))
     rms_norm_bwd_kernel(const RmsBwdParams p) {
   constexpr int V = MODE == kScalar ? 1 : 8;
-  extern __shared__ float part_smem[];  // TPR == 32 with a weight: 8 rows of d
-  __shared__ float red[4][32];
-  const int64_t first = TPR == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (TPR == 32 ? 8 : 1);
-  const int off = MODE == kShift ? static_cast<int>(first * p.d & 7) : 0;
+  constexpr int GROUPS = block_of(TPR) / TPR;
+  extern __shared__ float part_smem[];  // more than one group, with a weight: a row of d each
+  constexpr int U = bwd_at_once<X, MODE>(NV);
+  __shared__ float red[2][2 * U][32];
+  Rows<TPR> at;
+  const int off = MODE == kShift ? static_cast<int>(at.row * p.d & 7) : 0;
   const int d = p.d;
   float w[NV][V], dw[NV][V];
 #pragma unroll
@@ -393,81 +459,102 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, bwd_resident(TPR, NV * 
     for (int e = 0; e < V; ++e) dw[i][e] = 0.f;
   }
   using RR = std::conditional_t<is_none<R>, float, R>;
-  constexpr bool kAhead = MODE == kShift && NV == 1;  // the next row is on its way while one is worked on
+  constexpr bool kAhead = bwd_ahead<X, MODE>(NV);  // the next rows are on their way while some are worked on
   struct Loads {
     Raw<X, V> x, ds;
     Raw<G, V> g;
     Raw<RR, V> r;
   };
-  Loads next;
+  Loads next[U];
   auto fetch = [&](int64_t row, int i, Loads& l) {
     const bool more = row + 1 < p.rows;
-    const int j = group_at<TPR, V>(i, off);
-    load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, d, more, l.x);
-    load_group<MODE>(static_cast<const G*>(p.dh) + row * d, j, d, more, l.g);
-    if (p.ds != nullptr) load_group<MODE>(static_cast<const X*>(p.ds) + row * d, j, d, more, l.ds);
+    const int j = group_at<TPR, V>(i, off), n = row < p.rows ? d : 0;
+    load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, more, l.x);
+    load_group<MODE>(static_cast<const G*>(p.dh) + row * d, j, n, more, l.g);
+    if (p.ds != nullptr) load_group<MODE>(static_cast<const X*>(p.ds) + row * d, j, n, more, l.ds);
     if constexpr (!is_none<R>) {
       if (p.residual != nullptr)
-        load_group<MODE>(static_cast<const R*>(p.residual) + row * p.residual_stride, j, d, more, l.r);
+        load_group<MODE>(static_cast<const R*>(p.residual) + row * p.residual_stride, j, n, more, l.r);
     }
   };
-  if (kAhead && first < p.rows) fetch(first, 0, next);
+  if constexpr (kAhead) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) fetch(at.row + u * at.step, 0, next[u]);
+  }
   int flip = 0;
-  for (int64_t row = first; row < p.rows; row += step, flip ^= 2) {
-    float s[NV][V], g[NV][V], ds[NV][V];
+  for (; at.base < p.rows; at.base += U * at.step, at.row += U * at.step, flip ^= 1) {
+    float s[U][NV][V], g[U][NV][V], ds[U][NV][V], sums[2 * U];  // sums: s^2 and g s of each row
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, V>(i, off);
-      Loads l;
-      if constexpr (kAhead) l = next; else fetch(row, i, l);
-      expand<MODE>(l.x, j, d, s[i]);
-      expand<MODE>(l.g, j, d, g[i]);
-      if (p.ds != nullptr) {
-        expand<MODE>(l.ds, j, d, ds[i]);
-      } else {
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = at.row + u * at.step;
+      const int n = row < p.rows ? d : 0;
 #pragma unroll
-        for (int e = 0; e < V; ++e) ds[i][e] = 0.f;
-      }
-      if constexpr (!is_none<R>) {
-        if (p.residual != nullptr) {
-          float r[V];
-          expand<MODE>(l.r, j, d, r);
+      for (int i = 0; i < NV; ++i) {
+        const int j = group_at<TPR, V>(i, off);
+        Loads l;
+        if constexpr (kAhead) l = next[u]; else fetch(row, i, l);
+        expand<MODE>(l.x, j, n, s[u][i]);
+        expand<MODE>(l.g, j, n, g[u][i]);
+        if (p.ds != nullptr) {
+          expand<MODE>(l.ds, j, n, ds[u][i]);
+        } else {
 #pragma unroll
-          for (int e = 0; e < V; ++e) s[i][e] += r[e];
+          for (int e = 0; e < V; ++e) ds[u][i][e] = 0.f;
+        }
+        if constexpr (!is_none<R>) {
+          if (p.residual != nullptr) {
+            float r[V];
+            expand<MODE>(l.r, j, n, r);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[u][i][e] += r[e];
+          }
         }
       }
     }
-    if (kAhead && row + step < p.rows) fetch(row + step, 0, next);
-    float ss = 0.f, sg = 0.f;
+    if constexpr (kAhead) {
+      if (at.base + U * at.step < p.rows) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        ss = fmaf(s[i][e], s[i][e], ss);
-        sg = fmaf(g[i][e] * w[i][e], s[i][e], sg);
+        for (int u = 0; u < U; ++u) fetch(at.row + (U + u) * at.step, 0, next[u]);
       }
     }
-    ss = row_reduce<TPR, false>(ss, red[flip]);
-    sg = row_reduce<TPR, false>(sg, red[flip + 1]);
-    const float rstd = rsqrtf(ss / static_cast<float>(d) + p.eps);
-    const float c = sg / static_cast<float>(d) * rstd * rstd;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, V>(i, off);
-      float dx[V];
+    for (int u = 0; u < U; ++u) {
+      sums[2 * u] = sums[2 * u + 1] = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        dw[i][e] = fmaf(g[i][e], s[i][e] * rstd, dw[i][e]);
-        dx[e] = fmaf(rstd, g[i][e] * w[i][e] - s[i][e] * c, ds[i][e]);
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          sums[2 * u] = fmaf(s[u][i][e], s[u][i][e], sums[2 * u]);
+          sums[2 * u + 1] = fmaf(g[u][i][e] * w[i][e], s[u][i][e], sums[2 * u + 1]);
+        }
       }
-      if (p.dx != nullptr) store_group<MODE>(static_cast<X*>(p.dx) + row * d, j, d, dx);
-      if constexpr (!is_none<R>) {
-        if (p.dr != nullptr) store_group<MODE>(static_cast<R*>(p.dr) + row * d, j, d, dx);
+    }
+    row_reduce<TPR, false>(sums, red[flip]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t row = at.row + u * at.step;
+      const int n = row < p.rows ? d : 0;
+      // A row past the end adds nothing (its g and s are 0; with eps = 0 its rstd would be infinite).
+      const float rstd = n > 0 ? rsqrtf(sums[2 * u] / static_cast<float>(d) + p.eps) : 0.f;
+      const float c = sums[2 * u + 1] / static_cast<float>(d) * rstd * rstd;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = group_at<TPR, V>(i, off);
+        float dx[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          dw[i][e] = fmaf(g[u][i][e], s[u][i][e] * rstd, dw[i][e]);
+          dx[e] = fmaf(rstd, g[u][i][e] * w[i][e] - s[u][i][e] * c, ds[u][i][e]);
+        }
+        if (p.dx != nullptr) store_group<MODE>(static_cast<X*>(p.dx) + row * d, j, n, dx);
+        if constexpr (!is_none<R>) {
+          if (p.dr != nullptr) store_group<MODE>(static_cast<R*>(p.dr) + row * d, j, n, dx);
+        }
       }
     }
   }
   if (p.part == nullptr) return;
-  float* mine = TPR == 32 ? part_smem + (threadIdx.x >> 5) * d : p.part + static_cast<int64_t>(blockIdx.x) * d;
+  float* mine = GROUPS > 1 ? part_smem + threadIdx.x / TPR * d : p.part + static_cast<int64_t>(blockIdx.x) * d;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = group_at<TPR, V>(i, off);
@@ -475,12 +562,12 @@ __global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, bwd_resident(TPR, NV * 
     for (int e = 0; e < V; ++e)
       if (j + e >= 0 && j + e < d) mine[j + e] = dw[i][e];
   }
-  if constexpr (TPR == 32) {
+  if constexpr (GROUPS > 1) {
     __syncthreads();
     for (int j = threadIdx.x; j < d; j += blockDim.x) {
       float t = 0.f;
-#pragma unroll
-      for (int v = 0; v < 8; ++v) t += part_smem[v * d + j];
+#pragma unroll 8
+      for (int v = 0; v < GROUPS; ++v) t += part_smem[v * d + j];
       p.part[static_cast<int64_t>(blockIdx.x) * d + j] = t;
     }
   }
@@ -512,48 +599,64 @@ __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restric
   }
 }
 
-// Calls f with the threads per row and the groups per thread that hold `room` values. LEAN: at most 16 values per thread
-// up to 8,192 of a row (the gradient keeps five arrays of them, kShift three).
-template <int MODE, bool LEAN, class F>
+// Calls f with the threads per row and the groups of values per thread that hold `room` values. The gradient (GRAD,
+// which keeps five arrays of a thread's values) and kShift (which reads ahead) take at most two groups, both together one up to 2,048.
+template <int MODE, bool GRAD, class F>
 cudaError_t by_width(int room, F f) {
   using std::integral_constant;
+#define FWN_ROW(TPR, NV) \
+  if (room <= TPR * NV * (MODE == kScalar ? 1 : 8)) return f(integral_constant<int, TPR>(), integral_constant<int, NV>())
   if constexpr (MODE == kScalar) {
-    if (room <= 2048) return f(integral_constant<int, 256>(), integral_constant<int, 8>());
-    if (room <= 4096) return f(integral_constant<int, 256>(), integral_constant<int, 16>());
-    return f(integral_constant<int, 1024>(), integral_constant<int, 16>());
+    FWN_ROW(256, 8);
+    FWN_ROW(256, 16);
+    FWN_ROW(1024, 16);
   } else {
-    if (room <= 256) return f(integral_constant<int, 32>(), integral_constant<int, 1>());
-    if (room <= 512) return f(integral_constant<int, 32>(), integral_constant<int, 2>());
-    if constexpr (LEAN) {
-      if (room <= 1024) return f(integral_constant<int, 128>(), integral_constant<int, 1>());
+    FWN_ROW(8, 1);
+    FWN_ROW(16, 1);
+    FWN_ROW(32, 1);
+    if constexpr (MODE != kShift || !GRAD) FWN_ROW(32, 2);
+    if constexpr (MODE == kShift && GRAD) {
+      FWN_ROW(64, 1);
+      FWN_ROW(128, 1);
+      FWN_ROW(256, 1);
+      FWN_ROW(256, 2);
+      FWN_ROW(512, 2);
+      FWN_ROW(1024, 2);
+    } else if constexpr (GRAD || MODE == kShift) {
+      FWN_ROW(64, 2);
+      FWN_ROW(128, 2);
+      FWN_ROW(256, 2);
+      FWN_ROW(512, 2);
+      FWN_ROW(1024, 2);
     } else {
-      if (room <= 1024) return f(integral_constant<int, 32>(), integral_constant<int, 4>());
+      FWN_ROW(32, 3);
+      FWN_ROW(32, 4);
+      FWN_ROW(64, 3);
+      FWN_ROW(64, 4);
+      FWN_ROW(128, 3);
+      FWN_ROW(128, 4);
+      FWN_ROW(256, 4);
+      FWN_ROW(512, 4);
     }
-    if (room <= 2048) return f(integral_constant<int, 256>(), integral_constant<int, 1>());
-    if (room <= 4096) return f(integral_constant<int, 256>(), integral_constant<int, 2>());
-    if constexpr (LEAN) {
-      if (room <= 8192) return f(integral_constant<int, 1024>(), integral_constant<int, 1>());
-    } else {
-      if (room <= 8192) return f(integral_constant<int, 256>(), integral_constant<int, 4>());
-    }
-    return f(integral_constant<int, 1024>(), integral_constant<int, 2>());
   }
+#undef FWN_ROW
+  return cudaErrorInvalidValue;
 }
 int room_of(int mode, int d) { return mode == kShift ? d + 7 : d; }
 
 template <class X, class R, class O, int MODE>
 cudaError_t go(const RmsParams& p, cudaStream_t st) {
-  return by_width<MODE, MODE == kShift>(room_of(MODE, p.d), [&](auto tpr, auto nv) {
-    constexpr int TPR = decltype(tpr)::value;
-    int64_t blocks = TPR == 32 ? (p.rows + 7) / 8 : p.rows;
+  return by_width<MODE, false>(room_of(MODE, p.d), [&](auto tpr, auto nv) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, GROUPS = block_of(TPR) / TPR;
+    constexpr int U = rows_at_once<X, R, MODE>(NV);
+    // kWide, kScalar: the grid covers the rows. kShift: as many blocks as are resident walk them, so that the weights are
+    // read once per group of threads; a multiple of eight rows at a step.
+    int64_t blocks = (p.rows + GROUPS * U - 1) / (GROUPS * U);
     if (MODE == kShift) {
-      // A multiple of eight, several rows each: the weights are read once per group of threads.
-      const int64_t resident = static_cast<int64_t>(p.sms) * (TPR == 1024 ? 1 : TPR == 128 ? 6 : 2);
-      blocks = std::min(blocks, resident);
-      if (TPR != 32) blocks = (blocks + 7) / 8 * 8;
+      blocks = std::min<int64_t>(blocks, static_cast<int64_t>(p.sms) * (TPR > 512 ? 1 : 512 / block_of(TPR)));
+      if (GROUPS < 8) blocks = (blocks + 7) / 8 * 8;
     }
-    rms_norm_kernel<X, R, O, TPR, MODE, decltype(nv)::value>
-        <<<static_cast<unsigned>(blocks), TPR == 32 ? 256 : TPR, 0, st>>>(p);
+    rms_norm_kernel<X, R, O, TPR, MODE, NV><<<static_cast<unsigned>(blocks), block_of(TPR), 0, st>>>(p);
     return cudaGetLastError();
   });
 }
@@ -579,8 +682,9 @@ template <class X, class R, class G, int MODE>
 cudaError_t go_bwd(const RmsBwdParams& p, int blocks, cudaStream_t st) {
   cudaError_t e = by_width<MODE, true>(room_of(MODE, p.d), [&](auto tpr, auto nv) {
     constexpr int TPR = decltype(tpr)::value;
-    const size_t smem = TPR == 32 && p.part != nullptr ? 8 * sizeof(float) * static_cast<size_t>(p.d) : 0;
-    rms_norm_bwd_kernel<X, R, G, TPR, MODE, decltype(nv)::value><<<blocks, TPR == 32 ? 256 : TPR, smem, st>>>(p);
+    constexpr int GROUPS = block_of(TPR) / TPR;
+    const size_t smem = GROUPS > 1 && p.part != nullptr ? GROUPS * sizeof(float) * static_cast<size_t>(p.d) : 0;
+    rms_norm_bwd_kernel<X, R, G, TPR, MODE, decltype(nv)::value><<<blocks, block_of(TPR), smem, st>>>(p);
     return cudaGetLastError();
   });
   if (e != cudaSuccess || p.part == nullptr) return e;
@@ -613,20 +717,26 @@ cudaError_t launch_rms_norm(const RmsParams& p, cudaStream_t st) {
 
 // Blocks of the gradient's kernel: as many as are resident, which leaves the most rows to spread the cost of a block's row
 // of partials over; a multiple of eight where a block is a row's (mode kShift needs it).
-template <int MODE>
+template <class X, int MODE>
 int bwd_blocks(int64_t rows, int d, int sms) {
   int blocks = 0;
   by_width<MODE, true>(room_of(MODE, d), [&](auto tpr, auto nv) {
-    constexpr int TPR = decltype(tpr)::value;
-    const int64_t most = TPR == 32 ? (rows + 7) / 8 : rows;
-    const int64_t some = std::min<int64_t>(most, static_cast<int64_t>(sms) * bwd_resident(TPR, decltype(nv)::value * (MODE == kScalar ? 1 : 8)));
-    blocks = static_cast<int>(TPR == 32 ? some : (some + 7) / 8 * 8);
+    constexpr int TPR = decltype(tpr)::value, GROUPS = block_of(TPR) / TPR;
+    const int64_t most = (rows + GROUPS - 1) / GROUPS;
+    const int64_t some = std::min<int64_t>(most, static_cast<int64_t>(sms) * bwd_resident<X, MODE>(TPR, decltype(nv)::value));
+    blocks = static_cast<int>(GROUPS >= 8 ? some : (some + 7) / 8 * 8);
     return cudaSuccess;
   });
   return blocks;
 }
-int rms_bwd_blocks(int64_t rows, int d, int sms, int mode) {
-  return mode == kWide ? bwd_blocks<kWide>(rows, d, sms) : mode == kShift ? bwd_blocks<kShift>(rows, d, sms) : bwd_blocks<kScalar>(rows, d, sms);
+template <class X>
+int bwd_blocks_of(int64_t rows, int d, int sms, int mode) {
+  return mode == kWide    ? bwd_blocks<X, kWide>(rows, d, sms)
+         : mode == kShift ? bwd_blocks<X, kShift>(rows, d, sms)
+                          : bwd_blocks<X, kScalar>(rows, d, sms);
+}
+int rms_bwd_blocks(int64_t rows, int d, int sms, int mode, bool x_bf16) {
+  return x_bf16 ? bwd_blocks_of<bf16>(rows, d, sms, mode) : bwd_blocks_of<float>(rows, d, sms, mode);
 }
 
 cudaError_t launch_rms_norm_bwd(const RmsBwdParams& p, int blocks, cudaStream_t st) {

@@ -47,7 +47,7 @@ struct RmsBwdParams {
 // contiguous, from a base that allows 8 values per access.
 int rms_mode(bool wide, bool packed, int d);
 cudaError_t launch_rms_norm(const RmsParams& p, cudaStream_t stream);
-int rms_bwd_blocks(int64_t rows, int d, int sms, int mode);
+int rms_bwd_blocks(int64_t rows, int d, int sms, int mode, bool x_bf16);
 cudaError_t launch_rms_norm_bwd(const RmsBwdParams& p, int blocks, cudaStream_t stream);
 cudaError_t launch_column_sum(const float* part, int64_t rows, int d, void* out, bool out_bf16, cudaStream_t stream);
 
