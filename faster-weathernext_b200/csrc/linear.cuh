@@ -19,7 +19,7 @@ __host__ __device__ constexpr int linear_chunk_cols(int t, bool f32) { return f3
 // Rows of B that one CTA loads (and the box rows of its tensor map).
 __host__ __device__ constexpr int linear_box_n(int t) { return linear_tile_n(t) / (linear_pair(t) ? 2 : 1); }
 // Stages of k (128 bytes each) that a float32 result accumulates in the tensor core at a time; see linear.cu.
-constexpr int kLinearChunk = 8;
+constexpr int kLinearChunk = 12;
 
 struct LinearParams {
   const void* bias;      // [n] or null

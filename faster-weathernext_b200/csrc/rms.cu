@@ -187,8 +187,8 @@ template <int TPR, int V>
 __device__ __forceinline__ int group_at(int i, int off) {
   return (i * TPR + static_cast<int>(threadIdx.x & (TPR - 1))) * V - off;
 }
-// The group of values from column j of the row at p. `more`: rows follow, so that a group which the row's end cuts may be
-// read whole (kShift: what lies before a row is the row before); the last row's goes by single values.
+// The group of values from column j of the row at p. `more`: V - 1 values or more follow the row, so that a group which
+// its end cuts may be read whole (kShift: what lies before a row is the row before); the last rows' go by single values.
 template <int MODE, class T, int V>
 __device__ __forceinline__ void load_group(const T* p, int j, int d, bool more, Raw<T, V>& r) {
   constexpr int W = sizeof(r.u) / 4;
@@ -285,7 +285,8 @@ constexpr int rows_at_once(int nv) {
 
 // TPR threads per row, NV groups of V values per thread.
 template <class X, class R, class O, int TPR, int MODE, int NV>
-__global__ void __launch_bounds__(block_of(TPR), TPR > 512 ? 1 : 512 / block_of(TPR)) rms_norm_kernel(const RmsParams p) {
+__global__ void __launch_bounds__(block_of(TPR), TPR > 512 ? 1 : (MODE == kWide && TPR <= 32 && NV <= 2 ? 1024 : 512) / block_of(TPR))
+    rms_norm_kernel(const RmsParams p) {
   constexpr int V = MODE == kScalar ? 1 : 8;
   constexpr int U = rows_at_once<X, R, MODE>(NV);
   __shared__ float red[2][2][U][32];
@@ -312,9 +313,9 @@ __global__ void __launch_bounds__(block_of(TPR), TPR > 512 ? 1 : 512 / block_of(
   Raw<RR, V> rs[kAhead ? U : 1][kAhead ? NR : 1];
   auto fetch = [&](int64_t row, int i, Raw<X, V>& a, Raw<RR, V>& b) {
     const int j = group_at<TPR, V>(i, off), n = row < p.rows ? d : 0;
-    load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, row + 1 < p.rows, a);
-    if constexpr (!is_none<R>)
-      load_group<MODE>(static_cast<const R*>(p.residual) + row * p.residual_stride, j, n, row + 1 < p.rows, b);
+    const bool more = (p.rows - 1 - row) * d >= V - 1;
+    load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, more, a);
+    if constexpr (!is_none<R>) load_group<MODE>(static_cast<const R*>(p.residual) + row * p.residual_stride, j, n, more, b);
   };
   auto fetch_rows = [&](int64_t row) {
     if constexpr (kAhead) {
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(block_of(TPR), (bwd_resident<X, MODE>(TPR, NV)
   };
   Loads next[U];
   auto fetch = [&](int64_t row, int i, Loads& l) {
-    const bool more = row + 1 < p.rows;
+    const bool more = (p.rows - 1 - row) * d >= V - 1;
     const int j = group_at<TPR, V>(i, off), n = row < p.rows ? d : 0;
     load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, more, l.x);
     load_group<MODE>(static_cast<const G*>(p.dh) + row * d, j, n, more, l.g);
