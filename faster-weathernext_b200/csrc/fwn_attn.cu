@@ -1425,6 +1425,19 @@ fwn_status check_linear_bwd(const fwn_linear_desc* d) {
 
 }  // namespace
 
+fwn_status fwn_linear_pack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, int32_t dtype,
+                           void* stream) {
+  if (dtype != FWN_DTYPE_BF16 && dtype != FWN_DTYPE_E4M3) return fail(FWN_ERR_INVALID_ARGUMENT, "rows of bf16 or e4m3 (got %d)", dtype);
+  if (rows < 0 || cols <= 0 || (rows > 1 && lds < cols) || ldd < cols || ldd * dtype_size(dtype) % 16 != 0)
+    return fail(FWN_ERR_INVALID_ARGUMENT, "bad shape or stride");
+  if (rows == 0) return ok();
+  if (!src || !dst || !aligned16(dst)) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer or dst off 16 bytes");
+  cudaError_t e = fwn::launch_pack_rows(src, lds, dst, ldd, rows, cols, static_cast<int>(dtype_size(dtype)),
+                                        static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "pack");
+  return ok();
+}
+
 fwn_status fwn_linear_bwd_workspace_size(const fwn_linear_desc* desc, const void* a, const void* b, const void* dy,
                                          size_t* bytes) {
   if (!bytes) return fail(FWN_ERR_INVALID_ARGUMENT, "bytes is null");

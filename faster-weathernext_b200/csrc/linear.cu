@@ -69,8 +69,8 @@ template <int N>
 __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-// A bounded wait of a whole warp by polling (mbarrier.test_wait), for the producers and the MMA warp: mbarrier.try_wait
-// suspends the warp, and came back some 300 cycles after the arrival.
+// A bounded wait of a whole warp by polling (mbarrier.test_wait), for the producers and the MMA warp: 20.3 us at 10,242 x
+// 512 x 2,048 against 21.2 with mbarrier.try_wait, which may suspend the warp. The epilogue's warps wait with try_wait.
 __device__ __forceinline__ bool poll_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
   auto attempt = [&] {
     uint32_t ok;
@@ -101,35 +101,6 @@ __device__ __forceinline__ bool poll_wait(uint32_t bar, uint32_t parity, volatil
   }
   return __all_sync(0xffffffffu, ok);
 }
-// A bounded wait like warp_wait for warps that wait long (the epilogue's): each try may suspend the warp for up to 4 us,
-// so that sixteen warps do not take issue slots and power from the MMA warp by polling.
-__device__ __forceinline__ bool idle_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  auto attempt = [&] {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(4000u)
-        : "memory");
-    return ok != 0;
-  };
-  bool ok = attempt();
-  if (!ok) {
-    const unsigned long long t0 = globaltimer();
-    while (!(ok = attempt())) {
-      if (*abort) break;
-      if (globaltimer() - t0 > kWaitLimitNs) {
-        *abort = 1;
-        atomicOr(&g_device_error, 5u);
-        break;
-      }
-    }
-  }
-  return __all_sync(0xffffffffu, ok);
-}
-
 template <int CG>
 __device__ __forceinline__ void tmem_alloc_cg(uint32_t dst, uint32_t cols) {
   if constexpr (CG == 2) {
@@ -293,7 +264,16 @@ __device__ __forceinline__ void activate4_short(float* v) {
 //
 // float32 results: the tensor core truncates its running sum at every step, an error that grows with k (measured 1.5e-6
 // of the result at k = 2,048). They take k in chunks (p.chunk stages) into alternate accumulators, which the epilogue
-// warps add in float32 registers (64 a thread); so does act'(), where it makes a float32 bias gradient.
+// warps add in float32 registers (64 or 128 a thread); so does act'(), where it makes a float32 bias gradient. Measured
+// error / time of 163,848 x 2,048 x 512 with a float32 residual: chunks of 512 4.7e-7 / 321 us, 768 6.8e-7 / 303, 1,024
+// 1.0e-6 / 301.
+//
+// Bound, at 163,848 rows (times among other passes are up to 20 % longer: sw_power_cap at 1.2-1.5 GHz): k = 2,048 plain
+// 254-262 us = 1.31-1.35 PFLOP/s (cuBLAS 253-275 on the same boxes), the MMAs; 512 x 2,048 plain 294 (cuBLAS 316-355);
+// GELU 307, its arithmetic: 47 % of issue slots and 1.25 special-function calls a value; e4m3 GELU 203, the same, with
+// the stores; residual in float32 303, the MMAs and 8 bytes a value of HBM traffic; act'() with column sums at 81,924
+// rows 238, shared memory (x in, sums, result) and arithmetic. One product recomputed in the backward instead of keeping
+// the pre-activation: 102 us of MMAs under that epilogue, against 8 bytes a value (0.2 ms) in float32.
 template <int TILE, bool X32, bool O32, bool PRE, bool SUM>
 struct LinearCfg {
   static constexpr int CG = linear_pair(TILE) ? 2 : 1;
@@ -695,7 +675,7 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
         const int kb1 = w.kb1(p);
         for (int kb = w.kb0(p); kb < kb1; kb += p.chunk, ++acc_i) {
           buf = acc_i & 1;
-          if (!(ok = idle_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) goto done;
+          if (!(ok = warp_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) goto done;
           tc_fence_after();
 #pragma unroll
           for (int j = 0; j < C::HC; j += 16) {
@@ -709,7 +689,7 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
           release(buf);
         }
       } else {
-        if (!(ok = idle_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) goto done;
+        if (!(ok = warp_wait(acc_full(buf), (acc_i >> 1) & 1, abort_flag))) goto done;
         tc_fence_after();
         ++acc_i;
       }
@@ -717,7 +697,7 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
       for (int ch = 0; ch < C::NCH; ++ch, ++q) {
         const int col = col0 + CC * ch;
         if (x_tma) {
-          if (!(ok = idle_wait(x_bar(ew), q & 1, abort_flag))) goto done;
+          if (!(ok = warp_wait(x_bar(ew), q & 1, abort_flag))) goto done;
         } else if (ch > 0 || !has_x) {
           free_slot();
           if (has_x) gather_x(row0, col);
@@ -1017,12 +997,22 @@ cudaError_t rows_by_type(const void* a, int64_t lda, const void* b, int64_t ldb,
 
 // ---- packing and the gradient without an activation ----------------------------------------------------------------
 
+// Rows of any stride and base to rows of whole 16 bytes: a warp per row, a lane gathers 16 bytes and stores them at once
+// (the last piece filled up with zeros).
 template <class T>
 __global__ void __launch_bounds__(256) pack_rows_kernel(const T* __restrict__ src, int64_t lds, T* __restrict__ dst,
                                                         int64_t ldd, int64_t rows, int64_t cols) {
-  const int64_t per = (cols + 255) / 256;
-  const int64_t row = blockIdx.x / per, col = (blockIdx.x % per) * 256 + threadIdx.x;
-  if (row < rows && col < cols) dst[row * ldd + col] = src[row * lds + col];
+  constexpr int V = 16 / sizeof(T);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const T* from = src + row * lds;
+#pragma unroll 2
+  for (int64_t j = (threadIdx.x & 31) * V; j < cols; j += 32 * V) {
+    __align__(16) T v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = j + e < cols ? from[j + e] : T(0);
+    *reinterpret_cast<uint4*>(dst + row * ldd + j) = *reinterpret_cast<const uint4*>(v);
+  }
 }
 
 // A block takes 32 V columns (lane = V columns) and every gridDim.y-th group of eight rows; partial sums per block in
@@ -1117,7 +1107,7 @@ cudaError_t launch_linear_rows(const void* a, int64_t lda, const void* b, int64_
 
 cudaError_t launch_pack_rows(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, int es,
                              cudaStream_t st) {
-  const int64_t blocks = rows * ((cols + 255) / 256);
+  const int64_t blocks = (rows + 7) / 8;
   if (blocks == 0) return cudaSuccess;
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
   if (es == 1)

@@ -18,7 +18,7 @@ __host__ __device__ constexpr int linear_tile_n(int t) { return linear_pair(t) ?
 __host__ __device__ constexpr int linear_chunk_cols(int t, bool f32) { return f32 || t == kTile64 ? 32 : 64; }
 // Rows of B that one CTA loads (and the box rows of its tensor map).
 __host__ __device__ constexpr int linear_box_n(int t) { return linear_tile_n(t) / (linear_pair(t) ? 2 : 1); }
-// Stages of k (128 bytes each) that a float32 result accumulates in the tensor core at a time; see linear.cu.
+// Stages of k (128 bytes each: 64 bf16) that a float32 result accumulates in the tensor core at a time (linear.cu).
 constexpr int kLinearChunk = 12;
 
 struct LinearParams {
@@ -53,7 +53,8 @@ constexpr int kLinearRowsMax = 8;
 cudaError_t launch_linear_rows(const void* a, int64_t lda, const void* b, int64_t ldb, bool wide, const LinearParams& p,
                                cudaStream_t stream);
 
-// dst[r, 0..cols) = src[r, 0..cols) for elements of `es` (1 or 2) bytes; dst rows padded to ldd.
+// dst[r, 0..cols) = src[r, 0..cols) for elements of `es` (1 or 2) bytes; dst 16-byte aligned, its rows ldd apart, a multiple
+// of 16 bytes.
 cudaError_t launch_pack_rows(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols, int es,
                              cudaStream_t stream);
 

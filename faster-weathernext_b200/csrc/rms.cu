@@ -17,6 +17,9 @@
 //            share of the weight's gradient) from row to row, and the next row's loads are issued before the work on
 //            one. 10,242 x 1,001 bf16 with a bf16 residual, forward / backward: kScalar 41 / 165 us, kShift 19 / 36;
 //   kScalar  one value per thread and access: other strides and addresses.
+// Measured (of the measured copy rate, 6,468 GB/s): 163,848 x 512, float32 stream + bf16 residual -> bf16 147 us (1.05),
+// -> e4m3 135 us (1.05), gradient 224 us (0.93: five arrays of a thread's values keep it to two blocks per SM); 60M
+// values of bf16 without a residual 41-47 us at widths of 512 to 4,096 (0.8-0.9: few bytes per row), odd widths 57-97.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

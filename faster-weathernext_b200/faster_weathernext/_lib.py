@@ -44,7 +44,8 @@ SYMBOLS = ("fwn_version", "fwn_last_error_string", "fwn_device_error", "fwn_lse_
            "fwn_cond_layernorm_add", "fwn_cond_layernorm_bwd_workspace", "fwn_cond_layernorm_bwd",
            "fwn_gemm_bf16", "fwn_gemm_bf16_aux", "fwn_gemm_bf16_gather", "fwn_gnn_gather_add_act", "fwn_gnn_ln_segment_sum",
            "fwn_rms_norm", "fwn_rms_norm_bwd_workspace_size", "fwn_rms_norm_bwd", "fwn_linear_workspace_size", "fwn_linear",
-           "fwn_linear_bwd_workspace_size", "fwn_linear_bwd", "fwn_test_attn_fwd_timeout")
+           "fwn_linear_pack", "fwn_linear_bwd_workspace_size",
+           "fwn_linear_bwd", "fwn_test_attn_fwd_timeout")
 
 
 class AttnDesc(ctypes.Structure):
@@ -125,6 +126,7 @@ def _declare(lib):
       "fwn_rms_norm_bwd": [ctypes.POINTER(RmsDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
       "fwn_linear_workspace_size": [ctypes.POINTER(LinearDesc), _P, _P, ctypes.POINTER(_SZ)],
       "fwn_linear": [ctypes.POINTER(LinearDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+      "fwn_linear_pack": [_P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _I, _P],
       "fwn_linear_bwd_workspace_size": [ctypes.POINTER(LinearDesc), _P, _P, _P, ctypes.POINTER(_SZ)],
       "fwn_linear_bwd": [ctypes.POINTER(LinearDesc), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
       "fwn_bitset_csr_count": [_P, _I, _I, _P, _P, _SZ, _P],

@@ -216,13 +216,17 @@ def _padded(t):
   """t, or a copy of t [r, c] in its own order with rows of whole 16 bytes, which TMA can address: an operand of three
   products (odd widths) is laid out once instead of by each."""
   src, ld, turned = _orient(t)
-  if (ld % 8 == 0 and src.data_ptr() % 16 == 0) or src.shape[0] <= 8:
+  rows, cols = (src.shape[1], src.shape[0]) if turned else src.shape
+  if (ld % 8 == 0 and src.data_ptr() % 16 == 0) or rows <= 8:
     return t
-  if turned:
-    src = src.t()
-  out = src.new_empty((src.shape[0], -(-src.shape[1] // 8) * 8))[:, :src.shape[1]]
-  out.copy_(src)
+  out = src.new_empty((rows, -(-cols // 8) * 8))
+  _lib.check(_on_device(src, _pack_launch, src, ld, out, rows, cols))
+  out = out[:, :cols]
   return out.t() if turned else out
+
+
+def _pack_launch(stream, src, ld, out, rows, cols):
+  return _lib.lib().fwn_linear_pack(src.data_ptr(), ld, out.data_ptr(), out.shape[1], rows, cols, _lib.DTYPE_BF16, stream)
 
 
 # Workspace bytes by a call's shape, types, strides and the alignment of its operands (asked once for each).

@@ -352,6 +352,11 @@ FWN_API fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const 
                               const float* b_scale, const void* bias, const void* x, void* out, void* d_bias,
                               void* workspace, size_t workspace_bytes, void* stream);
 
+/* An operand of several products in rows that TMA can address: dst[r, 0..cols) = src[r, 0..cols), bf16 (or e4m3) rows lds
+ * (any) and ldd apart; dst 16-byte aligned, ldd >= cols a multiple of 16 bytes (filled with zeros up to the next 16 bytes). */
+FWN_API fwn_status fwn_linear_pack(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t rows, int64_t cols,
+                                   int32_t dtype, void* stream);
+
 /* The whole backward: desc as the forward's (bf16 operands, flags without FWN_LINEAR_PRE_GRAD), with x_dtype and ldx of dy
  * [m, n], the gradient of the output. d_pre = dy act'(a b^T + bias) (dy itself without an activation) in bf16, then
  * d_a [m, k] = d_pre b, d_b = d_pre^T a in b's own orientation (both bf16, contiguous) and d_bias [n] in bias_dtype; each

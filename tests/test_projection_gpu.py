@@ -3,8 +3,8 @@
 Bounds, in relative 2-norm. A result rounded once to bf16 is off by at most half a step of each value, 2^-9 to 2^-8 of it,
 in the mean square over many values below 2^-9; fewer than 64 values are held to half a step each. A gradient through the
 bf16 pre-activation gradient has a second rounding of that size, whose errors are independent over the sum: twice the
-bound. float32 norms: about ten roundings of 2^-24. float32 products: every 512 of k accumulate in the tensor core, 16
-(bf16) or 32 (e4m3) at a step, each step truncating at most 2^-23 of the running sum, 32 * 2^-23 = 3.8e-6. Column sums
+bound. float32 norms: about ten roundings of 2^-24. float32 products: every 768 of k accumulate in the tensor core, 16
+(bf16) or 32 (e4m3) at a step, each step truncating 2^-24 of the running sum on average, 48 * 2^-24 = 2.9e-6. Column sums
 over rows in float32: 2^-24 times the square root of the terms, with a margin of ten. e4m3: half a step is 2^-4 of a
 normal value, 2^-10 below 2^-6."""
 import math
@@ -352,6 +352,19 @@ def test_linear_gradient_against_differences(cuda):
   f = lambda bb: (pr.linear(a, w, bb, activation="gelu", out_dtype=F32).double() * c.double()).sum()  # noqa: E731
   diff = float(f(b + t * db) - f(b - t * db)) / (2 * t)
   assert abs(diff - float((gb.double() * db.double()).sum())) <= 1e-3 * float(c.norm()) * float(db.norm())
+
+
+@pytest.mark.parametrize("m,k,n", [(9001, 520, 1000), (9001, 64, 1000), (20000, 2048, 512), (9001, 1040, 333)])
+@pytest.mark.parametrize("out", [BF, F32])
+def test_linear_many_tiles_again_and_again(cuda, m, k, n, out):
+  """Tiles that follow one another in a block reuse its slots, accumulators and biases: thirty calls, the same bits."""
+  pr = _pr()
+  a, w, b, r = _problem(m, k, n, m + k)
+  r = r.to(out)
+  y = pr.linear(a, w, b, r, activation="swish", out_dtype=out)
+  assert _rel(y, _linear64(a, w, b, r, "swish")) <= TOL_PRODUCT[out]
+  for _ in range(30):
+    assert torch.equal(y, pr.linear(a, w, b, r, activation="swish", out_dtype=out))
 
 
 @pytest.mark.parametrize("act", ["gelu", "swish"])
