@@ -8,8 +8,8 @@
 namespace fwn {
 
 // Device error word (FWN_ERR_DEVICE_TIMEOUT when a bounded wait expired). Read by fwn_device_error().
-// One word per translation unit (fwn_attn.cu, linear.cu); fwn_device_error reads all of them.
-static __device__ unsigned int g_device_error = 0;
+// One word per translation unit (fwn_attn.cu's, and linear.cu's under a name of its own); fwn_device_error reads both.
+__device__ unsigned int g_device_error = 0;
 
 // A wait gives up after this many nanoseconds of %globaltimer (well above any legitimate wait).
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;

@@ -13,6 +13,8 @@
 #include <cstdint>
 #include <type_traits>
 
+// This translation unit's device error word.
+#define g_device_error g_linear_device_error
 #include "common.cuh"
 #include "linear.cuh"
 
