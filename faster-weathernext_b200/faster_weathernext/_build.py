@@ -14,7 +14,7 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(ROOT, "csrc")
 INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 LIB = os.path.join(PKG, "libfwn_attn.so")
-SOURCES = ["fwn_attn.cu", "tiles.cu", "khop.cu", "norm.cu", "gnn.cu", "rms.cu", "linear.cu"]
+SOURCES = ["fwn_attn.cu", "tiles.cu", "khop.cu", "norm.cu", "gnn.cu", "rms.cu", "rms_bwd.cu", "linear.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr"]
