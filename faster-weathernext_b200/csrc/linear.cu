@@ -189,10 +189,13 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 __device__ __forceinline__ float2 pair(float a) { return make_float2(a, a); }
 // Four values for a bf16 result. The special-function unit, not the FP32 pipe, bounds an epilogue of two calls a value
 // (4,096 cycles for a 128 x 256 tile, as long as its MMAs at k = 512): the four denominators 1 + 2^z' (each at most 2^31,
-// so that their product stays in float32) share one reciprocal, 1.25 calls a value, and the rest runs in pairs.
+// so that their product stays in float32) share one reciprocal, 1.25 calls a value, and the rest runs in pairs. A NaN must
+// not reach that product, or three other columns would be NaN with it: the denominators take a minimum that drops it, and
+// x (in the slope 2^z' too) carries it into its own result.
 template <int ACT, bool SLOPE>
 __device__ __forceinline__ void activate4(float* v) {
   using L = Logistic<ACT>;
+  constexpr float kDenomMax = 2147483648.f;
   float2 x[2], d[2], e[2], xx[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -206,7 +209,7 @@ __device__ __forceinline__ void activate4(float* v) {
       z = fmul2(x[i], pair(L::p0));
     }
     e[i] = make_float2(ex2(z.x), ex2(z.y));
-    d[i] = fadd2(e[i], pair(1.f));
+    d[i] = fadd2(make_float2(fminf(e[i].x, kDenomMax), fminf(e[i].y, kDenomMax)), pair(1.f));
   }
   const float2 m = fmul2(d[0], d[1]);
   const float r = rcp(m.x * m.y);
