@@ -164,9 +164,9 @@ struct Logistic {
   static constexpr float p1 = ACT == 1 ? p0 * kGeluC1 : 0.f;
   // dz/dx = q0 + q1 x^2
   static constexpr float q0 = ACT == 1 ? 2.f * kGeluC0 : 1.f, q1 = ACT == 1 ? 3.f * kGeluC1 * q0 : 0.f;
-  // Below `low` 2^z' passes 2^30: there the value is taken as that at `low` (-5e-9, for swish -2e-8) and so is the slope
-  // (-5e-8, for swish -2e-8); above `high` the slope is 1 to float32's last bit.
-  static constexpr float low = ACT == 1 ? -5.5f : -20.5f, high = ACT == 1 ? 10.f : 40.f;
+  // Below `low`, where 2^z' is about 2^30, bf16 results are taken as those at `low` (-5.9e-9, for swish -1.6e-8), and so is
+  // the slope (-4.7e-8, for swish -1.5e-8); above `high` the slope is 1 to float32's last bit.
+  static constexpr float low = ACT == 1 ? -5.5f : -21.f, high = ACT == 1 ? 10.f : 40.f;
 };
 // One value, to float32 precision over the whole range.
 template <int ACT>

@@ -1,14 +1,18 @@
-"""GPU: the pre-norm projections where one value is not a number. Every case runs on each way a product takes: few rows
-(m <= 8), one tile, split k, many tiles on pairs of SMs.
+"""GPU: the pre-norm projections where one value is not a number and where an activation's tail counts. Every case runs on
+each way a product takes: few rows (m <= 8), one tile, split k, many tiles on pairs of SMs.
 
-Bounds. Columns beside a NaN: those of the same products without one (test_projection_gpu.py)."""
+Bounds. Columns beside a NaN: those of the same products without one (test_projection_gpu.py). An activation's value,
+each by itself, as a bf16 result: half a bf16 step, at most 2^-8 of the value; 1e-5 of it for the arithmetic (the
+exponential's argument reaches 80 log2(e), times 2^-24 and a few roundings); and absolutely 6e-9 (GELU) or 2.1e-8
+(swish): the value at -5.5 or -21, below which it is held there, is within that."""
 import pytest
 import torch
 
-from test_projection_gpu import BF, F32, TOL_GRAD, TOL_PRODUCT, _gen, _linear64, _pr, _problem, _rel
+from test_projection_gpu import BF, F32, TOL_GRAD, TOL_PRODUCT, _act64, _gen, _linear64, _no_device_error, _pr, _problem, _rel
 
 pytestmark = pytest.mark.gpu
 
+TAIL = {"gelu": 6e-9, "swish": 2.1e-8}
 # m, k, n: few rows; one tile; split k; few tiles; pairs of SMs, short k and long.
 PATHS = [(5, 256, 130), (42, 256, 130), (42, 2048, 512), (300, 256, 130), (9001, 520, 1000), (9001, 1040, 333)]
 
@@ -58,3 +62,22 @@ def test_a_nan_in_a_bias_or_weight_row_stays_in_its_gradients(cuda, m, k, n, act
   assert bool(torch.isnan(d_a.float()).all()) and bool(torch.isnan(d_w[[17, 66]].float()).all())
   assert bool(torch.isnan(d_b[[17, 66]]).all())
   assert _rel(d_w[keep], want_w[keep]) <= TOL_GRAD[BF] and _rel(d_b[keep], want_b[keep]) <= TOL_GRAD[F32]
+
+
+# ---- activations over their range -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m,k,n", [(1, 64, 4003), (16, 64, 4003), (300, 64, 4003), (3000, 64, 4003), (40, 2048, 515),
+                                   (9001, 1536, 515)])
+@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("act", ["gelu", "swish"])
+def test_bf16_results_of_an_activation_over_its_range(cuda, m, k, n, kind, act):
+  """Pre-activations from -40 to 40 and beyond (the bias, with a zero product), each value by itself, for bf16 and 8-bit
+  operands and on every way a product takes: a row's values do not depend on the rows it came with."""
+  b = torch.cat([torch.linspace(-40, 40, n - 6, device=cuda),
+                 torch.tensor([-1e4, 1e4, 0.0, -3.0, -4.0, -8.0], device=cuda)])
+  a = torch.zeros(m, k, device=cuda, dtype=BF)
+  w = torch.randn(n, k, device=cuda, generator=_gen(k)).to(BF)
+  want = _act64(b.double(), act)
+  y = _operands(kind, a, w)[0](b, activation=act).double()
+  assert bool(((y - want).abs() <= (2.0 ** -8 + 1e-5) * want.abs() + TAIL[act]).all())
+  _no_device_error()
