@@ -230,25 +230,6 @@ __device__ __forceinline__ void activate4(float* v) {
   }
 }
 
-// Four values through the hardware's tanh, one special-function call each: off by at most 2^-12 of |x| absolutely, so that
-// the tail (x < -2) keeps few digits of its own. For 8-bit operands, whose own rounding is 2^-4: the e4m3 GELU
-// up-projection (163,848 x 512 x 2,048) went from 309 to 234 us, the bf16 one, which stays exact, would from 317 to 302.
-template <int ACT>
-__device__ __forceinline__ void activate4_short(float* v) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float2 x = make_float2(v[2 * i], v[2 * i + 1]);
-    const float2 h = fmul2(x, pair(0.5f));
-    const float2 z = ACT == 1 ? fmul2(x, ffma2(fmul2(x, x), pair(kGeluC0 * kGeluC1), pair(kGeluC0))) : h;
-    float2 t;
-    asm("tanh.approx.f32 %0, %1;" : "=f"(t.x) : "f"(z.x));
-    asm("tanh.approx.f32 %0, %1;" : "=f"(t.y) : "f"(z.y));
-    const float2 y = ffma2(h, t, h);
-    v[2 * i] = y.x;
-    v[2 * i + 1] = y.y;
-  }
-}
-
 // ---- tensor-core kernel --------------------------------------------------------------------------------------------
 
 // Persistent; a CTA (CG = 1) or a pair of CTAs on two SMs (CG = 2) takes output tiles of 128 CG x BN, walked with n
@@ -275,8 +256,8 @@ __device__ __forceinline__ void activate4_short(float* v) {
 //
 // Bound, at 163,848 rows (times among other passes are up to 20 % longer: sw_power_cap at 1.2-1.5 GHz): k = 2,048 plain
 // 254-262 us = 1.31-1.35 PFLOP/s (cuBLAS 253-275 on the same boxes), the MMAs; 512 x 2,048 plain 294 (cuBLAS 316-355);
-// GELU 307, its arithmetic: 47 % of issue slots and 1.25 special-function calls a value; e4m3 GELU 203, the same, with
-// the stores; residual in float32 303, the MMAs and 8 bytes a value of HBM traffic; act'() with column sums at 81,924
+// GELU 293-308 and e4m3 GELU 228, the way of an epilogue chunk (TMEM, arithmetic, shared memory, store), with no unit full:
+// 47 % of issue slots, 1.25 special-function calls a value; residual in float32 303, the MMAs and 8 bytes a value of HBM traffic; act'() with column sums at 81,924
 // rows 238, shared memory (x in, sums, result) and arithmetic. One product recomputed in the backward instead of keeping
 // the pre-activation: 102 us of MMAs under that epilogue, against 8 bytes a value (0.2 ms) in float32.
 template <int TILE, bool X32, bool O32, bool PRE, bool SUM>
@@ -578,9 +559,6 @@ __global__ void __launch_bounds__(LinearCfg<TILE, X32, O32, PRE, SUM>::THREADS, 
         if constexpr (O32) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = activate<ACT>(v[i]);
-        } else if (!PRE && p.b_scale != nullptr) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) activate4_short<ACT>(v + 4 * i);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) activate4<ACT, PRE>(v + 4 * i);

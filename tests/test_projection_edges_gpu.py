@@ -68,7 +68,7 @@ def test_a_nan_in_a_bias_or_weight_row_stays_in_its_gradients(cuda, m, k, n, act
 
 @pytest.mark.parametrize("m,k,n", [(1, 64, 4003), (16, 64, 4003), (300, 64, 4003), (3000, 64, 4003), (40, 2048, 515),
                                    (9001, 1536, 515)])
-@pytest.mark.parametrize("kind", ["bf16"])
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
 @pytest.mark.parametrize("act", ["gelu", "swish"])
 def test_bf16_results_of_an_activation_over_its_range(cuda, m, k, n, kind, act):
   """Pre-activations from -40 to 40 and beyond (the bias, with a zero product), each value by itself, for bf16 and 8-bit
