@@ -168,14 +168,6 @@ struct Logistic {
   // the slope (-4.7e-8, for swish -1.5e-8); above `high` the slope is 1 to float32's last bit.
   static constexpr float low = ACT == 1 ? -5.5f : -21.f, high = ACT == 1 ? 10.f : 40.f;
 };
-// One value, to float32 precision over the whole range.
-template <int ACT>
-__device__ __forceinline__ float activate(float x) {
-  if constexpr (ACT == 0) return x;
-  using L = Logistic<ACT>;
-  const float z = ACT == 1 ? x * fmaf(L::p1 * x, x, L::p0) : x * L::p0;
-  return x * rcp(1.f + ex2(z));
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -185,6 +177,16 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   float r;
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
+}
+// One value, to float32 precision over the whole range. -infinity counts as the lowest finite value, whose result is -0, the
+// functions' limit, and what the clamp at `low` comes to in bf16 (x sigma would be infinity times 0).
+template <int ACT>
+__device__ __forceinline__ float activate(float x) {
+  if constexpr (ACT == 0) return x;
+  using L = Logistic<ACT>;
+  x = max_nan(x, -3.402823466e38f);
+  const float z = ACT == 1 ? x * fmaf(L::p1 * x, x, L::p0) : x * L::p0;
+  return x * rcp(1.f + ex2(z));
 }
 __device__ __forceinline__ float2 pair(float a) { return make_float2(a, a); }
 // Four values for a bf16 result. The special-function unit, not the FP32 pipe, bounds an epilogue of two calls a value

@@ -320,7 +320,8 @@ FWN_API fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, con
  * be given with its other dimension contiguous (bf16). x, the residual, has the output's type. Rows whose stride or base
  * is not a multiple of 16 bytes are allowed everywhere (such operands are copied into the workspace first). out
  * overlaps no input. FWN_ACT_NONE, FWN_ACT_GELU_TANH or FWN_ACT_SWISH, to the result's precision; a bf16 result may hold
- * what is below -5.5 (GELU) or -21 (swish) at the value there, -5.9e-9 or -1.6e-8.
+ * what is below -5.5 (GELU) or -21 (swish) at the value there, -5.9e-9 or -1.6e-8. At -infinity it is their limit, 0 to
+ * that bound (-0 in float32).
  *
  * FWN_LINEAR_PRE_GRAD: the backward's first step, out = x act'(a b^T + bias) in bf16 with x = the gradient of the
  * forward's output ([m, n], bf16 or float32): the gradient of the pre-activation, which is computed again here rather

@@ -1,5 +1,5 @@
-"""GPU: the pre-norm projections where one value is not a number and where an activation's tail counts. Every case runs on
-each way a product takes: few rows (m <= 8), one tile, split k, many tiles on pairs of SMs.
+"""GPU: the pre-norm projections where one value is not a number or infinite and where an activation's
+tail counts. Every case runs on each way a product takes: few rows (m <= 8), one tile, split k, many tiles on pairs of SMs.
 
 Bounds. Columns beside a NaN: those of the same products without one (test_projection_gpu.py). An activation's value,
 each by itself, as a bf16 result: half a bf16 step, at most 2^-8 of the value; 1e-5 of it for the arithmetic (the
@@ -81,3 +81,35 @@ def test_bf16_results_of_an_activation_over_its_range(cuda, m, k, n, kind, act):
   y = _operands(kind, a, w)[0](b, activation=act).double()
   assert bool(((y - want).abs() <= (2.0 ** -8 + 1e-5) * want.abs() + TAIL[act]).all())
   _no_device_error()
+
+
+@pytest.mark.parametrize("m,k,n", PATHS)
+@pytest.mark.parametrize("kind,out", [("bf16", BF), ("bf16", F32), ("fp8", BF), ("fp8", F32)])
+@pytest.mark.parametrize("act", ["gelu", "swish"])
+def test_infinite_pre_activations_give_the_limits(cuda, m, k, n, kind, out, act):
+  """A bias of infinity gives infinity, one of -infinity (a unit that is switched off) 0, on every way a product takes."""
+  a, w, b, _ = _problem(m, k, n, m + n)
+  b[17], b[66] = float("inf"), float("-inf")
+  call, a64, w64 = _operands(kind, a, w)
+  y = call(b, activation=act, out_dtype=out)
+  keep = [i for i in range(n) if i not in (17, 66)]
+  assert bool((y[:, 17].float() == float("inf")).all()) and bool((y[:, 66].float().abs() <= TAIL[act]).all())
+  assert _rel(y[:, keep], _linear64(a64, w64, b, None, act)[:, keep]) <= TOL_PRODUCT[out]
+
+
+@pytest.mark.parametrize("m,k,n", PATHS)
+@pytest.mark.parametrize("act", ["gelu", "swish"])
+def test_infinite_pre_activations_give_the_slopes_limits(cuda, m, k, n, act):
+  """Slope 1 at infinity, 0 at -infinity (held at that of -5.5 or -21: below 5e-8), the other columns' as without them."""
+  pr = _pr()
+  a, w, b, _ = _problem(m, k, n, m + k)
+  b[17], b[66] = float("inf"), float("-inf")
+  dy = torch.randn(m, n, device=cuda, generator=_gen(n)).to(BF)
+  ins = [t.requires_grad_() for t in (a, w, b)]
+  _, d_w, d_b = torch.autograd.grad(pr.linear(*ins, activation=act), ins, dy)
+  ref = [t.detach().double().requires_grad_() for t in ins]
+  _, want_w, want_b = torch.autograd.grad(_linear64(*ref, None, act), ref, dy.double())
+  keep = [i for i in range(n) if i not in (17, 66)]
+  assert _rel(d_w[keep], want_w[keep]) <= TOL_GRAD[BF] and _rel(d_b[keep], want_b[keep]) <= TOL_GRAD[F32]
+  assert abs(float(d_b[17]) - float(dy[:, 17].double().sum())) <= 1e-5 * float(dy[:, 17].double().norm())
+  assert abs(float(d_b[66])) <= 5e-8 * float(dy[:, 66].double().abs().sum())
