@@ -40,6 +40,14 @@ def _check(name, t, like, dtypes):
     raise ValueError(f"{name} is on {t.device}, expected the CUDA device of the first argument ({like.device})")
 
 
+def _constant(name, *tensors):
+  """Refuses inputs of a function without gradients that ask for one: its result would be cut off from them unnoticed."""
+  if torch.is_grad_enabled():
+    for t in tensors:
+      if t is not None and t.requires_grad:
+        raise NotImplementedError(f"{name} has no gradient (forecasts): call it under torch.no_grad() or on detached tensors")
+
+
 def _rows(t):
   """t as [rows, d] with d contiguous and rows that do not overlap: a view where the strides allow it, else a copy."""
   if t.is_contiguous():
@@ -185,15 +193,16 @@ def rms_norm(x, weight=None, residual=None, *, eps=1e-6, out_dtype=_BF16):
 def rms_norm_fp8(x, weight=None, residual=None, *, eps=1e-6):
   """rms_norm with h in 8 bits, the left operand of linear_fp8: returns (values e4m3 [..., d], scale float32 [...]), or,
   with a residual, (values, scale, s). scale = max |h| / 448 over the row, h = scale * values. Rows whose max |h| is
-  below 2^-100 get scale 0 and values 0. Not differentiable (forecasts)."""
+  below 2^-100 get scale 0 and values 0. No gradient (forecasts): inputs that require one raise NotImplementedError."""
   _rms_check(x, weight, residual, eps)
+  _constant("rms_norm_fp8", x, weight, residual)
   h, scale, x_new = _rms_forward(x, weight, residual, eps, _E4M3)
   return (h, scale) if residual is None else (h, scale, x_new)
 
 
 def quantize_fp8(t):
   """Rows of t [..., k] (float32 or bf16) in 8 bits: (values e4m3 [..., k], scale float32 [...]) as rms_norm_fp8's. The
-  form linear_fp8 takes a weight [n, k] in; computed once and kept."""
+  form linear_fp8 takes a weight [n, k] in; computed once and kept, a constant whatever t requires."""
   _rms_check(t, None, None, 0.0)
   return _rms_forward(t, None, None, 0.0, _E4M3, _lib.RMS_SCALE_ONLY)[:2]
 
@@ -374,8 +383,8 @@ def linear(a, weight, bias=None, residual=None, *, activation=None, out_dtype=_B
 
 def linear_fp8(a, a_scale, weight, weight_scale, bias=None, residual=None, *, activation=None, out_dtype=_BF16):
   """linear on 8-bit operands: act((a weight^T) a_scale weight_scale + bias) + residual, a [..., k] and weight [n, k]
-  e4m3 with float32 scales per row (a_scale [...], weight_scale [n]), as rms_norm_fp8 and quantize_fp8 give them. Not
-  differentiable (forecasts)."""
+  e4m3 with float32 scales per row (a_scale [...], weight_scale [n]), as rms_norm_fp8 and quantize_fp8 give them. No
+  gradient (forecasts): inputs that require one raise NotImplementedError."""
   _linear_check(a, weight, bias, residual, activation, out_dtype, _E4M3)
   _check("a_scale", a_scale, a, (_F32,))
   _check("weight_scale", weight_scale, a, (_F32,))
@@ -383,5 +392,6 @@ def linear_fp8(a, a_scale, weight, weight_scale, bias=None, residual=None, *, ac
     raise ValueError(f"a_scale has shape {tuple(a_scale.shape)}, expected {tuple(a.shape[:-1])}")
   if weight_scale.shape != weight.shape[:1]:
     raise ValueError(f"weight_scale has shape {tuple(weight_scale.shape)}, expected ({weight.shape[0]},)")
+  _constant("linear_fp8", a, a_scale, weight, weight_scale, bias, residual)
   return _linear_forward(a, weight, bias, residual, _ACT[activation], out_dtype, a_scale.contiguous(),
                          weight_scale.contiguous())

@@ -113,3 +113,26 @@ def test_infinite_pre_activations_give_the_slopes_limits(cuda, m, k, n, act):
   assert _rel(d_w[keep], want_w[keep]) <= TOL_GRAD[BF] and _rel(d_b[keep], want_b[keep]) <= TOL_GRAD[F32]
   assert abs(float(d_b[17]) - float(dy[:, 17].double().sum())) <= 1e-5 * float(dy[:, 17].double().norm())
   assert abs(float(d_b[66])) <= 5e-8 * float(dy[:, 66].double().abs().sum())
+
+
+# ---- derivatives that cannot be given are refused -------------------------------------------------------------------
+
+def test_8_bit_calls_refuse_inputs_that_require_a_gradient(cuda):
+  """Their results would be cut off from the input; under no_grad, and for a weight laid out once, they are constants."""
+  pr = _pr()
+  a, w, b, r = _problem(40, 64, 48, 1)
+  x, wn = torch.randn(40, 64, device=cuda), torch.ones(64, device=cuda)
+  a8, sa = pr.quantize_fp8(a)
+  w8, sw = pr.quantize_fp8(w.clone().requires_grad_())
+  assert not w8.requires_grad and not sw.requires_grad
+  r = r.to(BF)
+  leaf = lambda t: t.clone().requires_grad_()  # noqa: E731
+  calls = (lambda: pr.rms_norm_fp8(leaf(x), wn), lambda: pr.rms_norm_fp8(x, leaf(wn)),
+           lambda: pr.rms_norm_fp8(x, None, leaf(x)), lambda: pr.linear_fp8(a8, leaf(sa), w8, sw),
+           lambda: pr.linear_fp8(a8, sa, w8, leaf(sw)), lambda: pr.linear_fp8(a8, sa, w8, sw, leaf(b)),
+           lambda: pr.linear_fp8(a8, sa, w8, sw, None, leaf(r)))
+  for call in calls:
+    with pytest.raises(NotImplementedError):
+      call()
+    with torch.no_grad():
+      call()
