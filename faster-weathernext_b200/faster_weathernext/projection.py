@@ -17,6 +17,7 @@ its tensors' device and takes its workspace from torch's allocator.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from faster_weathernext import _lib
 
@@ -46,6 +47,16 @@ def _constant(name, *tensors):
     for t in tensors:
       if t is not None and t.requires_grad:
         raise NotImplementedError(f"{name} has no gradient (forecasts): call it under torch.no_grad() or on detached tensors")
+  _no_tangent(name, *tensors)
+
+
+def _no_tangent(name, *tensors):
+  """Refuses inputs with a forward-mode tangent, which the kernels would lose (they have backward gradients only)."""
+  if forward_ad._current_level < 0:  # outside every dual_level, as unpack_dual looks it up, without its call for each
+    return
+  for t in tensors:
+    if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+      raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _rows(t):
@@ -141,6 +152,7 @@ class _RmsNorm(torch.autograd.Function):
   @staticmethod
   def backward(ctx, dh, ds=None):
     x, w, r = ctx.saved_tensors
+    _no_tangent("rms_norm's gradient", x, w, r, dh, ds)
     need_x, need_w, need_r = ctx.needs_input_grad[:3]
     if dh is None:
       # Only the stored sum was used: its gradient passes through.
@@ -179,8 +191,10 @@ def rms_norm(x, weight=None, residual=None, *, eps=1e-6, out_dtype=_BF16):
 
   x [..., d] float32 or bf16 (d <= 16,384), residual of x's shape, weight [d], each float32 or bf16; any strides. Sums
   are float32. Returns h in out_dtype (bf16 or float32), or, with a residual, (h, s) with s in x's dtype: the residual
-  stream after the addition. Differentiable in x, weight and residual (gradients in their dtypes)."""
+  stream after the addition. Differentiable in x, weight and residual (backward, gradients in their dtypes; forward mode
+  raises NotImplementedError)."""
   _rms_check(x, weight, residual, eps)
+  _no_tangent("rms_norm", x, weight, residual)
   if out_dtype is not _BF16 and out_dtype is not _F32:
     raise ValueError(f"out_dtype {out_dtype}: expected torch.bfloat16 or torch.float32")
   if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
@@ -302,6 +316,7 @@ class _Linear(torch.autograd.Function):
   @staticmethod
   def backward(ctx, dy):
     a, weight, bias = ctx.saved_tensors
+    _no_tangent("linear's gradient", a, weight, bias, dy)
     need_a, need_w, need_b, need_r = ctx.needs_input_grad[:4]
     d_a = d_w = d_b = None
     if a.shape[0] == 0:
@@ -371,8 +386,10 @@ def linear(a, weight, bias=None, residual=None, *, activation=None, out_dtype=_B
   """act(a weight^T + bias) + residual in one kernel: a [..., k] and weight [n, k] bf16, bias [n] bf16 or float32,
   residual [..., n] in out_dtype (bf16 or float32), activation None, "gelu" (tanh form) or "swish"; float32
   accumulation, rounded once. weight may be the transposed view of a [k, n] tensor (either orientation is read in
-  place); rows of any stride. Differentiable in a, weight, bias and residual (gradients in their dtypes)."""
+  place); rows of any stride. Differentiable in a, weight, bias and residual (backward, gradients in their dtypes;
+  forward mode raises NotImplementedError)."""
   _linear_check(a, weight, bias, residual, activation, out_dtype, _BF16)
+  _no_tangent("linear", a, weight, bias, residual)
   act = _ACT[activation]
   if torch.is_grad_enabled() and (a.requires_grad or weight.requires_grad or
                                   (bias is not None and bias.requires_grad) or

@@ -136,3 +136,31 @@ def test_8_bit_calls_refuse_inputs_that_require_a_gradient(cuda):
       call()
     with torch.no_grad():
       call()
+
+
+def test_forward_mode_is_refused(cuda):
+  """A tangent of any input, in forward calls and in gradients, under no_grad too; calls without one pass at a dual level."""
+  from torch.autograd import forward_ad as fw
+  pr = _pr()
+  a, w, b, r = _problem(40, 64, 48, 1)
+  x, wn = torch.randn(40, 64, device=cuda), torch.ones(64, device=cuda)
+  a8, sa = pr.quantize_fp8(a)
+  w8, sw = pr.quantize_fp8(w)
+  r = r.to(BF)
+  ag, xg = a.clone().requires_grad_(), x.clone().requires_grad_()
+  y, h = pr.linear(ag, w, b, activation="gelu"), pr.rms_norm(xg, wn)
+  with fw.dual_level():
+    dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+    calls = (lambda f: pr.linear(f(a), w), lambda f: pr.linear(a, f(w)), lambda f: pr.linear(a, w, f(b)),
+             lambda f: pr.linear(a, w, None, f(r)), lambda f: pr.rms_norm(f(x)), lambda f: pr.rms_norm(x, f(wn)),
+             lambda f: pr.rms_norm(x, wn, f(x)), lambda f: pr.rms_norm_fp8(f(x)),
+             lambda f: pr.linear_fp8(a8, sa, w8, sw, f(b)), lambda f: pr.linear_fp8(a8, sa, w8, sw, None, f(r)),
+             lambda f: torch.autograd.grad(y, ag, f(torch.ones_like(y)), retain_graph=True),
+             lambda f: torch.autograd.grad(h, xg, f(torch.ones_like(h)), retain_graph=True))
+    for call in calls:
+      with pytest.raises(NotImplementedError):
+        call(dual)
+      call(lambda t: t)
+    for call in calls[:10]:
+      with torch.no_grad(), pytest.raises(NotImplementedError):
+        call(dual)
