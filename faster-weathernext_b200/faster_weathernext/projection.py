@@ -59,6 +59,14 @@ def _no_tangent(name, *tensors):
       raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
+def _first_order(name):
+  """Refuses a backward that keeps a graph (create_graph=True): the kernels' gradients would be constants in it, and second
+  derivatives would lack their terms unnoticed. (A node that raises when it is differentiated would not do: autograd.grad
+  skips nodes that lead to none of its inputs.)"""
+  if torch.is_grad_enabled():
+    raise NotImplementedError(f"{name} has no second derivative: take its gradient without create_graph=True")
+
+
 def _rows(t):
   """t as [rows, d] with d contiguous and rows that do not overlap: a view where the strides allow it, else a copy."""
   if t.is_contiguous():
@@ -160,6 +168,7 @@ class _RmsNorm(torch.autograd.Function):
         return None, None, None, None, None
       return (ds if need_x else None, torch.zeros_like(w) if need_w else None,
               ds.to(ctx.residual_dtype) if need_r else None, None, None)
+    _first_order("rms_norm")
     dx, dw, dr = _on_device(x, _RmsNorm._launch, ctx, x, w, r, dh, ds, need_x, need_w, need_r)
     return dx, dw, dr, None, None
 
@@ -192,7 +201,7 @@ def rms_norm(x, weight=None, residual=None, *, eps=1e-6, out_dtype=_BF16):
   x [..., d] float32 or bf16 (d <= 16,384), residual of x's shape, weight [d], each float32 or bf16; any strides. Sums
   are float32. Returns h in out_dtype (bf16 or float32), or, with a residual, (h, s) with s in x's dtype: the residual
   stream after the addition. Differentiable in x, weight and residual (backward, gradients in their dtypes; forward mode
-  raises NotImplementedError)."""
+  and second derivatives raise NotImplementedError)."""
   _rms_check(x, weight, residual, eps)
   _no_tangent("rms_norm", x, weight, residual)
   if out_dtype is not _BF16 and out_dtype is not _F32:
@@ -324,6 +333,7 @@ class _Linear(torch.autograd.Function):
       d_w = torch.zeros_like(weight) if need_w else None
       d_b = torch.zeros_like(bias) if need_b else None
     elif need_a or need_w or need_b:
+      _first_order("linear")
       d_a, d_w, d_b = _on_device(a, _Linear._launch, a, weight, bias, ctx.act,
                                  _rows(dy if dy.dim() == 2 else dy.reshape(a.shape[0], -1)), need_a, need_w, need_b)
       if need_a and len(ctx.shape) != 2:
@@ -387,7 +397,7 @@ def linear(a, weight, bias=None, residual=None, *, activation=None, out_dtype=_B
   residual [..., n] in out_dtype (bf16 or float32), activation None, "gelu" (tanh form) or "swish"; float32
   accumulation, rounded once. weight may be the transposed view of a [k, n] tensor (either orientation is read in
   place); rows of any stride. Differentiable in a, weight, bias and residual (backward, gradients in their dtypes;
-  forward mode raises NotImplementedError)."""
+  forward mode and second derivatives raise NotImplementedError)."""
   _linear_check(a, weight, bias, residual, activation, out_dtype, _BF16)
   _no_tangent("linear", a, weight, bias, residual)
   act = _ACT[activation]

@@ -164,3 +164,28 @@ def test_forward_mode_is_refused(cuda):
     for call in calls[:10]:
       with torch.no_grad(), pytest.raises(NotImplementedError):
         call(dual)
+
+
+def test_second_derivatives_are_refused(cuda):
+  """A gradient that keeps a graph through a product or norm is refused, whether or not what comes in has a graph; what a
+  residual or the stored sum passes through alone has its own, right, graph."""
+  pr = _pr()
+  a, w, b, r = _problem(40, 64, 48, 1)
+  ins = [t.requires_grad_() for t in (a, w, b, r)]
+  for f in (lambda y: y.sum(), lambda y: y.square().sum()):
+    y = pr.linear(a, w, b, r, activation="gelu", out_dtype=F32)
+    with pytest.raises(NotImplementedError):
+      torch.autograd.grad(f(y), ins, retain_graph=True, create_graph=True)
+    torch.autograd.grad(f(y), ins)
+  y = pr.linear(a.detach(), w.detach(), b.detach(), r, out_dtype=F32)
+  g, = torch.autograd.grad(y.pow(3).sum(), r, create_graph=True)
+  assert torch.allclose(torch.autograd.grad(g.sum(), r)[0], 6 * y)
+  x, s, wn = torch.randn(40, 64, device=cuda), torch.randn(40, 64, device=cuda), torch.ones(64, device=cuda)
+  ins = [t.requires_grad_() for t in (x, s, wn)]
+  for f in (lambda h: h.sum(), lambda h: h.square().sum()):
+    h, total = pr.rms_norm(x, wn, s, out_dtype=F32)
+    with pytest.raises(NotImplementedError):
+      torch.autograd.grad(f(h), ins, retain_graph=True, create_graph=True)
+    torch.autograd.grad(f(h), ins, retain_graph=True)
+  g, = torch.autograd.grad(total.pow(3).sum(), x, create_graph=True)
+  assert torch.allclose(torch.autograd.grad(g.sum(), x)[0], 6 * total)
