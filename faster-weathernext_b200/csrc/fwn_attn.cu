@@ -7,6 +7,7 @@
 #include <cstddef>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -977,6 +978,16 @@ namespace {
 bool is_float_dtype(int32_t t) { return t == FWN_DTYPE_BF16 || t == FWN_DTYPE_F32; }
 int64_t dtype_size(int32_t t) { return t == FWN_DTYPE_F32 ? 4 : t == FWN_DTYPE_BF16 ? 2 : 1; }
 bool aligned_to(const void* p, int64_t a) { return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(a) == 0; }
+// Tensors that start off their elements' size would fault in the kernels (NULL, an absent one, passes).
+struct Elements {
+  const void* p;
+  int64_t size;
+};
+fwn_status check_elements(std::initializer_list<Elements> tensors) {
+  for (const Elements& t : tensors)
+    if (!aligned_to(t.p, t.size)) return fail(FWN_ERR_INVALID_ARGUMENT, "a tensor starts off a multiple of its elements' %lld bytes", static_cast<long long>(t.size));
+  return FWN_OK;
+}
 
 fwn_status check_rms(const fwn_rms_desc* d, bool residual, bool weight, bool bwd) {
   if (!d) return fail(FWN_ERR_INVALID_ARGUMENT, "desc is null");
@@ -1019,6 +1030,9 @@ fwn_status fwn_rms_norm(const fwn_rms_desc* desc, const void* x, const void* res
   if ((residual != nullptr) != (x_out != nullptr)) return fail(FWN_ERR_INVALID_ARGUMENT, "residual and x_out come together");
   if ((d.out_dtype == FWN_DTYPE_E4M3) != (scale != nullptr))
     return fail(FWN_ERR_INVALID_ARGUMENT, "scale goes with an E4M3 output, and with that alone");
+  s = check_elements({{x, dtype_size(d.x_dtype)}, {x_out, dtype_size(d.x_dtype)}, {out, dtype_size(d.out_dtype)}, {scale, 4},
+                      {residual, dtype_size(d.residual_dtype)}, {weight, dtype_size(d.weight_dtype)}});
+  if (s != FWN_OK) return s;
   fwn::RmsParams p{};
   p.x = x;
   p.residual = residual;
@@ -1068,6 +1082,11 @@ fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, const void*
   const fwn_rms_desc& d = *desc;
   if (d.rows > 0 && (!x || !dh)) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
   if (d_weight && !weight) return fail(FWN_ERR_INVALID_ARGUMENT, "d_weight needs weight");
+  s = check_elements({{x, dtype_size(d.x_dtype)}, {ds, dtype_size(d.x_dtype)}, {dx, dtype_size(d.x_dtype)},
+                      {dh, dtype_size(d.out_dtype)}, {residual, dtype_size(d.residual_dtype)},
+                      {d_residual, dtype_size(d.residual_dtype)}, {weight, dtype_size(d.weight_dtype)},
+                      {d_weight, dtype_size(d.weight_dtype)}});
+  if (s != FWN_OK) return s;
   if (d_weight) {
     size_t need = 0;
     if ((s = fwn_rms_norm_bwd_workspace_size(desc, &need)) != FWN_OK) return s;
@@ -1260,6 +1279,10 @@ fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const float* a
   const bool pre = d.flags & FWN_LINEAR_PRE_GRAD, fp8 = d.dtype == FWN_DTYPE_E4M3;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (d_bias && (!pre || !bias)) return fail(FWN_ERR_INVALID_ARGUMENT, "d_bias goes with FWN_LINEAR_PRE_GRAD and a bias");
+  s = check_elements({{a, dtype_size(d.dtype)}, {b, dtype_size(d.dtype)}, {a_scale, 4}, {b_scale, 4},
+                      {bias, dtype_size(d.bias_dtype)}, {d_bias, dtype_size(d.bias_dtype)}, {x, dtype_size(d.x_dtype)},
+                      {out, dtype_size(d.out_dtype)}});
+  if (s != FWN_OK) return s;
   if (d.m == 0) {
     if (d_bias) {
       cudaError_t e = cudaMemsetAsync(d_bias, 0, static_cast<size_t>(d.n) * dtype_size(d.bias_dtype), st);
@@ -1432,6 +1455,7 @@ fwn_status fwn_linear_pack(const void* src, int64_t lds, void* dst, int64_t ldd,
     return fail(FWN_ERR_INVALID_ARGUMENT, "bad shape or stride");
   if (rows == 0) return ok();
   if (!src || !dst || !aligned16(dst)) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer or dst off 16 bytes");
+  if (fwn_status s = check_elements({{src, dtype_size(dtype)}}); s != FWN_OK) return s;
   cudaError_t e = fwn::launch_pack_rows(src, lds, dst, ldd, rows, cols, static_cast<int>(dtype_size(dtype)),
                                         static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "pack");
@@ -1454,6 +1478,9 @@ fwn_status fwn_linear_bwd(const fwn_linear_desc* desc, const void* a, const void
   const fwn_linear_desc& d = *desc;
   if (!a || !b || !dy) return fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
   if (d_bias && !bias) return fail(FWN_ERR_INVALID_ARGUMENT, "d_bias needs the bias");
+  s = check_elements({{a, 2}, {b, 2}, {d_a, 2}, {d_b, 2}, {dy, dtype_size(d.x_dtype)}, {bias, dtype_size(d.bias_dtype)},
+                      {d_bias, dtype_size(d.bias_dtype)}});
+  if (s != FWN_OK) return s;
   const LinearBwdPlan pl = plan_linear_bwd(d, a, b, dy, num_sms());
   if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned_to(workspace, 256)))
     return fail(FWN_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) needed", pl.bytes);

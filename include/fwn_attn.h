@@ -278,8 +278,8 @@ FWN_API fwn_status fwn_gemm_bf16_gather(const void* a, const void* bt, const voi
  *
  * Root-mean-square norm: s = x + residual (or x), h = s / sqrt(mean(s^2) + eps) * weight over rows of d values.
  * Every tensor has its last dimension contiguous; x and residual have a row stride in elements, the outputs are
- * contiguous and do not overlap the inputs. d up to 16,384; any alignment of whole elements (rows whose addresses and
- * width allow it, 32 bytes and multiples of 8, move in wide accesses). */
+ * contiguous and do not overlap the inputs. d up to 16,384; any alignment of whole elements, others refused (rows
+ * whose addresses and width allow it, 32 bytes and multiples of 8, move in wide accesses). */
 typedef struct fwn_rms_desc {
   int64_t rows;
   int32_t d;
@@ -318,8 +318,8 @@ FWN_API fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, con
  * m, n, k >= 1 (m = 0 does nothing); float32 accumulation on the tensor cores. Operands bf16, or e4m3 with one float32
  * scale per row of a and of b (the product's element (i, j) is multiplied by a_scale[i] b_scale[j]). Either operand may
  * be given with its other dimension contiguous (bf16). x, the residual, has the output's type. Rows whose stride or base
- * is not a multiple of 16 bytes are allowed everywhere (such operands are copied into the workspace first). out
- * overlaps no input. FWN_ACT_NONE, FWN_ACT_GELU_TANH or FWN_ACT_SWISH, to the result's precision; a bf16 result may hold
+ * is not a multiple of 16 bytes (but one of whole elements) are allowed everywhere (such operands are copied into the
+ * workspace first). out overlaps no input. FWN_ACT_NONE, FWN_ACT_GELU_TANH or FWN_ACT_SWISH, to the result's precision; a bf16 result may hold
  * what is below -5.5 (GELU) or -21 (swish) at the value there, -5.9e-9 or -1.6e-8. At -infinity it is their limit, 0 to
  * that bound (-0 in float32).
  *

@@ -33,3 +33,30 @@ def test_workspace_sizes_are_kept_by_device(monkeypatch):
     ws, size = projection._workspace(_OnDevice(device), desc, size_of(device), 256, 512)
     assert size == 256 * (device + 1) and ws == (device, (size,))
   assert asked == [0, 1]
+
+
+def test_tensors_off_their_elements_are_refused():
+  """A float32 tensor at an address off 4 bytes, a bf16 one off 2: refused by every entry point before any CUDA call."""
+  from faster_weathernext import _lib
+  lib, bad = _lib.lib(), _lib.FWN_ERR_INVALID_ARGUMENT
+  rms = _lib.RmsDesc(4, 64, 1, 0, 1, 0, 0, 1e-6, 0, 64, 64)  # float32 x and weight, bf16 residual and out
+  good = [256, 256, 256, 256, 256, None]                     # x, residual, weight, x_out, out, scale
+  for i, off in enumerate((258, 257, 258, 258, 257)):
+    assert lib.fwn_rms_norm(rms, *good[:i], off, *good[i + 1:], 0) == bad
+  fp8 = _lib.RmsDesc(4, 64, 1, 0, 1, 2, 0, 1e-6, 0, 64, 64)
+  assert lib.fwn_rms_norm(fp8, 256, None, None, None, 257, 258, 0) == bad  # the scale; e4m3 values start anywhere
+  good = [256] * 8                                           # x, residual, weight, dh, ds, dx, d_residual, d_weight
+  for i, off in enumerate((258, 257, 258, 257, 258, 258, 257, 258)):
+    assert lib.fwn_rms_norm_bwd(rms, *good[:i], off, *good[i + 1:], 256, 1 << 30, 0) == bad
+  lin = _lib.LinearDesc(4, 32, 48, 0, 1, 1, 1, 0, 0, 48, 48, 32, 32)       # float32 bias, residual and out
+  good = [256, None, 256, None, 256, 256, 256, None]         # a, a_scale, b, b_scale, bias, x, out, d_bias
+  for i, off in ((0, 257), (2, 257), (4, 258), (5, 258), (6, 258)):
+    assert lib.fwn_linear(lin, *good[:i], off, *good[i + 1:], None, 0, 0) == bad
+  lin8 = _lib.LinearDesc(4, 32, 48, 2, 1, 1, 1, 0, 0, 48, 48, 32, 32)
+  for scales in ((258, 256), (256, 258)):
+    assert lib.fwn_linear(lin8, 257, scales[0], 257, scales[1], None, None, 256, None, None, 0, 0) == bad
+  assert lib.fwn_linear_pack(257, 48, 256, 48, 4, 48, 0, 0) == bad
+  good = [256, 256, 256, 256, 256, 256, 256]                 # a, b, bias, dy, d_a, d_b, d_bias
+  for i, off in enumerate((257, 257, 258, 258, 257, 257, 258)):
+    assert lib.fwn_linear_bwd(lin, *good[:i], off, *good[i + 1:], 256, 1 << 30, 0) == bad
+  assert b"elements" in lib.fwn_last_error_string()
