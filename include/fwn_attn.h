@@ -319,9 +319,10 @@ FWN_API fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, con
  * scale per row of a and of b (the product's element (i, j) is multiplied by a_scale[i] b_scale[j]). Either operand may
  * be given with its other dimension contiguous (bf16). x, the residual, has the output's type. Rows whose stride or base
  * is not a multiple of 16 bytes (but one of whole elements) are allowed everywhere (such operands are copied into the
- * workspace first). out overlaps no input. FWN_ACT_NONE, FWN_ACT_GELU_TANH or FWN_ACT_SWISH, to the result's precision; a bf16 result may hold
- * what is below -5.5 (GELU) or -21 (swish) at the value there, -5.9e-9 or -1.6e-8. At -infinity it is their limit, 0 to
- * that bound (-0 in float32).
+ * workspace first). out overlaps no input. FWN_ACT_NONE, FWN_ACT_GELU_TANH or FWN_ACT_SWISH, to the result's precision; a
+ * bf16 result may hold what is below -5.5 (GELU) or -21 (swish) at the value there, -5.9e-9 or -1.6e-8. At -infinity it is
+ * their limit, 0 to that bound (-0 in float32). A float32 result is the sum of products over chunks of k of at most 768
+ * (1,536 of e4m3), within which the tensor core truncates its running sum: 7e-7 of the result in the 2-norm.
  *
  * FWN_LINEAR_PRE_GRAD: the backward's first step, out = x act'(a b^T + bias) in bf16 with x = the gradient of the
  * forward's output ([m, n], bf16 or float32): the gradient of the pre-activation, which is computed again here rather
@@ -360,7 +361,8 @@ FWN_API fwn_status fwn_linear_pack(const void* src, int64_t lds, void* dst, int6
                                    int32_t dtype, void* stream);
 
 /* The whole backward: desc as the forward's (bf16 operands, flags without FWN_LINEAR_PRE_GRAD), with x_dtype and ldx of dy
- * [m, n], the gradient of the output. d_pre = dy act'(a b^T + bias) (dy itself without an activation) in bf16, then
+ * [m, n], the gradient of the output. d_pre = dy act'(a b^T + bias) (dy itself without an activation), rounded to bf16 (the
+ * products' operand, whatever dy's type: 2.3e-3 of d_a and d_b in the 2-norm, 1.7e-3 of it their own rounding), then
  * d_a [m, k] = d_pre b, d_b = d_pre^T a in b's own orientation (both bf16, contiguous) and d_bias [n] in bias_dtype; each
  * may be NULL (d_bias: must be without a bias). The residual's gradient is dy. Deterministic. m >= 1. */
 FWN_API fwn_status fwn_linear_bwd_workspace_size(const fwn_linear_desc* desc, const void* a, const void* b, const void* dy,

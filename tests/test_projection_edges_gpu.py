@@ -13,8 +13,9 @@ from test_projection_gpu import BF, F32, TOL_GRAD, TOL_PRODUCT, _act64, _gen, _l
 pytestmark = pytest.mark.gpu
 
 TAIL = {"gelu": 6e-9, "swish": 2.1e-8}
-# m, k, n: few rows; one tile; split k; few tiles; pairs of SMs, short k and long.
-PATHS = [(5, 256, 130), (42, 256, 130), (42, 2048, 512), (300, 256, 130), (9001, 520, 1000), (9001, 1040, 333)]
+# m, k, n: few rows; one tile; split k, of bf16 and of e4m3; few tiles; pairs of SMs, short k, odd rows and long k.
+PATHS = [(5, 256, 130), (42, 256, 130), (42, 2048, 512), (42, 4096, 512), (300, 256, 130), (9001, 520, 1000),
+         (9001, 1040, 333), (9001, 1536, 1000)]
 
 
 def _operands(kind, a, w):
@@ -67,7 +68,7 @@ def test_a_nan_in_a_bias_or_weight_row_stays_in_its_gradients(cuda, m, k, n, act
 # ---- activations over their range -----------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("m,k,n", [(1, 64, 4003), (16, 64, 4003), (300, 64, 4003), (3000, 64, 4003), (40, 2048, 515),
-                                   (9001, 1536, 515)])
+                                   (40, 4096, 515), (9001, 1536, 515), (9001, 1536, 1000)])
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
 @pytest.mark.parametrize("act", ["gelu", "swish"])
 def test_bf16_results_of_an_activation_over_its_range(cuda, m, k, n, kind, act):
