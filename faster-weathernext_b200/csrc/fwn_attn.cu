@@ -1187,8 +1187,17 @@ struct LinearPlan {
   bool pack_a, pack_b;       // operand rows that TMA cannot address are copied once
   int64_t lda, ldb;          // as the kernel reads them
   int tile, splits;
+  int64_t stages;            // of k in a tile's longest run
   size_t off_b, off_part, off_sum, bytes;
 };
+// A tile's epilogue waits for its run of k, 0.3-0.6 us a stage: this many stay well below the limit of the waits
+// (kWaitLimitNs), after which the kernel would give up with its result unwritten.
+constexpr int64_t kMaxStages = 1 << 20;
+fwn_status check_plan(const LinearPlan& pl) {
+  if (pl.stages > kMaxStages) return fail(FWN_ERR_UNSUPPORTED, "%lld x 128 bytes of k in one run: at most %lld are supported",
+                                          static_cast<long long>(pl.stages), static_cast<long long>(kMaxStages));
+  return FWN_OK;
+}
 
 // Whether a 256 x 256 tile takes its form with eight epilogue warps and five stages (kTile256Long) or sixteen and four
 // (kTile256): the first feeds the MMAs better, the second hides an epilogue that takes longer than a short k's MMAs.
@@ -1251,6 +1260,7 @@ LinearPlan plan_linear(const fwn_linear_desc& d, const void* a, const void* b, i
       }
     }
   }
+  pl.stages = (kb + pl.splits - 1) / pl.splits;
   pl.off_part = at;
   if (pl.splits > 1)
     at += static_cast<size_t>(pl.splits) * round_up(d.m, fwn::linear_tile_m(pl.tile)) * round_up(d.n, 4) * sizeof(float);
@@ -1266,7 +1276,11 @@ fwn_status fwn_linear_workspace_size(const fwn_linear_desc* desc, const void* a,
   if (!bytes) return fail(FWN_ERR_INVALID_ARGUMENT, "bytes is null");
   fwn_status s = check_linear(desc);
   if (s != FWN_OK) return s;
-  *bytes = desc->m == 0 ? 0 : plan_linear(*desc, a, b, num_sms()).bytes;
+  *bytes = 0;
+  if (desc->m == 0) return ok();
+  const LinearPlan pl = plan_linear(*desc, a, b, num_sms());
+  if ((s = check_plan(pl)) != FWN_OK) return s;
+  *bytes = pl.bytes;
   return ok();
 }
 
@@ -1298,6 +1312,7 @@ fwn_status fwn_linear(const fwn_linear_desc* desc, const void* a, const float* a
   if (x && d.m > 1 && d.ldx < d.n) return fail(FWN_ERR_INVALID_ARGUMENT, "ldx is below n");
   const int sms = num_sms();
   const LinearPlan pl = plan_linear(d, a, b, sms);
+  if ((s = check_plan(pl)) != FWN_OK) return s;
   if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned_to(workspace, 256)))
     return fail(FWN_ERR_WORKSPACE, "workspace of %zu bytes (256-byte aligned) needed", pl.bytes);
   uint8_t* ws = static_cast<uint8_t*>(workspace);

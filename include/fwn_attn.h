@@ -315,7 +315,8 @@ FWN_API fwn_status fwn_rms_norm_bwd(const fwn_rms_desc* desc, const void* x, con
                                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* Projection with bias, activation and residual in its epilogue: out[m, n] = act(a[m, k] b[n, k]^T + bias) + x, any
- * m, n, k >= 1 (m = 0 does nothing); float32 accumulation on the tensor cores. Operands bf16, or e4m3 with one float32
+ * m, n, k >= 1 (m = 0 does nothing; FWN_ERR_UNSUPPORTED where a tile would run over more than 2^20 x 128 bytes of k at
+ * once); float32 accumulation on the tensor cores. Operands bf16, or e4m3 with one float32
  * scale per row of a and of b (the product's element (i, j) is multiplied by a_scale[i] b_scale[j]). Either operand may
  * be given with its other dimension contiguous (bf16). x, the residual, has the output's type. Rows whose stride or base
  * is not a multiple of 16 bytes (but one of whole elements) are allowed everywhere (such operands are copied into the

@@ -60,3 +60,18 @@ def test_tensors_off_their_elements_are_refused():
   for i, off in enumerate((257, 257, 258, 258, 257, 257, 258)):
     assert lib.fwn_linear_bwd(lin, *good[:i], off, *good[i + 1:], 256, 1 << 30, 0) == bad
   assert b"elements" in lib.fwn_last_error_string()
+
+
+def test_a_run_of_k_beyond_the_waits_limit_is_refused():
+  """An output tile's run of k that takes seconds would end in a wait that gives up; few rows have none."""
+  import ctypes
+  from faster_weathernext import _lib
+  lib, k = _lib.lib(), 2 ** 30
+  size = ctypes.c_size_t(7)
+  lin = lambda m, k, flags=0, act=0: _lib.LinearDesc(m, 32, k, 0, 0, 1, 0, act, flags, k, k, 32, 32)  # noqa: E731
+  grad = lin(64, k, _lib.LINEAR_PRE_GRAD, _lib.ACT_GELU_TANH)     # the gradient of the pre-activation: k is not split
+  assert lib.fwn_linear_workspace_size(grad, 256, 256, size) == _lib.FWN_ERR_UNSUPPORTED
+  assert lib.fwn_linear(grad, 256, None, 256, None, 256, 256, 256, None, 256, 1 << 40, 0) == _lib.FWN_ERR_UNSUPPORTED
+  assert lib.fwn_linear_workspace_size(lin(64, 2 ** 31 - 2048), 256, 256, size) == _lib.FWN_ERR_UNSUPPORTED
+  assert lib.fwn_linear_workspace_size(lin(64, 2 ** 26), 256, 256, size) == _lib.FWN_OK and size.value > 0
+  assert lib.fwn_linear_workspace_size(lin(8, k), 256, 256, size) == _lib.FWN_OK and size.value == 0
