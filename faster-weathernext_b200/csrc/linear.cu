@@ -256,12 +256,14 @@ __device__ __forceinline__ void activate4(float* v) {
 // error / time of 163,848 x 2,048 x 512 with a float32 residual: chunks of 512 4.7e-7 / 321 us, 768 6.8e-7 / 303, 1,024
 // 1.0e-6 / 301.
 //
-// Bound, at 163,848 rows (times among other passes are up to 20 % longer: sw_power_cap at 1.2-1.5 GHz): k = 2,048 plain
+// Bound, at 163,848 rows (times among other passes are up to 30 % longer: sw_power_cap at 1.2-1.5 GHz): k = 2,048 plain
 // 254-262 us = 1.31-1.35 PFLOP/s (cuBLAS 253-275 on the same boxes), the MMAs; 512 x 2,048 plain 294 (cuBLAS 316-355);
-// GELU 293-308 and e4m3 GELU 228, the way of an epilogue chunk (TMEM, arithmetic, shared memory, store), with no unit full:
-// 47 % of issue slots, 1.25 special-function calls a value; residual in float32 303, the MMAs and 8 bytes a value of HBM traffic; act'() with column sums at 81,924
-// rows 238, shared memory (x in, sums, result) and arithmetic. One product recomputed in the backward instead of keeping
-// the pre-activation: 102 us of MMAs under that epilogue, against 8 bytes a value (0.2 ms) in float32.
+// GELU 293-308 and e4m3 GELU 226, the latency of an epilogue chunk's steps (TMEM, arithmetic, shared memory, store), with no
+// unit full (tensor pipe 57 and 35 %, issue slots 50 and 64 %); residual in float32 285-303, the MMAs and 8 bytes a value of
+// HBM traffic; act'() with column sums at 81,924 rows 242, shared memory (x in, sums, result) and arithmetic. One product
+// recomputed in the backward instead of keeping the pre-activation: 102 us of MMAs under that epilogue, against 8 bytes a
+// value (0.2 ms) in float32. d_pre leaves in bf16, the operand of the two products that read it: 2.3e-3 of their results
+// against 1.7e-3 for their own rounding alone; two bf16 parts of it would double both (81,924 rows: 2 x 120 us).
 template <int TILE, bool X32, bool O32, bool PRE, bool SUM>
 struct LinearCfg {
   static constexpr int CG = linear_pair(TILE) ? 2 : 1;
@@ -279,9 +281,11 @@ struct LinearCfg {
   static constexpr int NS = TILE == kTile256 ? (PRE ? 3 : 4) : TILE == kTile64 ? 6 : 5;
   static constexpr int TMEM_COLS = 2 * BN;
   static constexpr int THREADS = 128 + 32 * EW;
-  // Registers at launch (65,536 over the threads, in steps of 8) and after the warpgroups have traded: 128 x 32 + 512 x
-  // 112 = 640 x 96, 128 x 56 + 256 x 224 = 384 x 168.
+  // Registers at launch (65,536 over the threads, in steps of 8: 96 or 168) and after the warpgroups have traded: 128 x 40 +
+  // 512 x 104 of 640 x 96, 128 x 56 + 256 x 224 = 384 x 168. Spilled: 104 to 224 bytes where k is added in chunks on
+  // kTile256 (float32 results of odd widths, act'() with a float32 dy), at most 28 elsewhere.
   static constexpr int REGS_LOW = TILE == kTile256 ? 40 : 56, REGS_HIGH = TILE == kTile256 ? 104 : 224;
+  static_assert(128 * REGS_LOW + 32 * EW * REGS_HIGH <= THREADS * (65536 / THREADS / 8 * 8), "more than the launch has");
   static constexpr int N_BAR = 2 * NS + 4 + 1 + EW;
   static constexpr int OFF_SLOT = NS * STAGE;            // per epilogue warp
   static constexpr int OFF_RED = OFF_SLOT + EW * SLOT;

@@ -396,7 +396,8 @@ def _linear_check(a, weight, bias, residual, activation, out_dtype, dtype):
 def linear(a, weight, bias=None, residual=None, *, activation=None, out_dtype=_BF16):
   """act(a weight^T + bias) + residual in one kernel: a [..., k] and weight [n, k] bf16, bias [n] bf16 or float32,
   residual [..., n] in out_dtype (bf16 or float32), activation None, "gelu" (tanh form) or "swish"; float32
-  accumulation, rounded once. weight may be the transposed view of a [k, n] tensor (either orientation is read in
+  accumulation, rounded once (in the backward so is the gradient of the pre-activation, to bf16: the operand of the
+  products for a's and weight's). weight may be the transposed view of a [k, n] tensor (either orientation is read in
   place); rows of any stride. Differentiable in a, weight, bias and residual (backward, gradients in their dtypes;
   forward mode and second derivatives raise NotImplementedError)."""
   _linear_check(a, weight, bias, residual, activation, out_dtype, _BF16)
