@@ -1203,7 +1203,8 @@ fwn_status check_plan(const LinearPlan& pl) {
 // (kTile256): the first feeds the MMAs better, the second hides an epilogue that takes longer than a short k's MMAs.
 // Measured at 163,848 x k x 1,024, long / short in us: plain k 256 90 / 97, k 1,024 255 / 280; GELU k 512 175 / 170,
 // k 640 191 / 202; e4m3 plain k 512 127 / 105, k 768 122 / 140; e4m3 GELU k 1,024 186 / 173, k 1,280 201 / 205,
-// k 1,536 (n 512) 124 / 144; act'() k 1,024 432 / 452, k 1,280 442 / 492, k 1,536 (n 512) 270 / 317.
+// k 1,536 (n 512) 124 / 144; act'() with a bf16 dy k 768 348 / 332, k 1,024 410 / 417, k 1,152 431 / 446, k 1,280 495 / 499,
+// with a float32 one k 1,024 507 / 476, k 1,152 562 / 505, k 1,280 560 / 548 (bf16 dy, k 1,536, n 512 270 / 317).
 bool long_form(const fwn_linear_desc& d, int64_t kb) {
   if (d.flags & FWN_LINEAR_PRE_GRAD) return kb >= 20;
   if (d.ldo * dtype_size(d.out_dtype) % 16 != 0) return kb >= 20;  // an epilogue of plain stores (odd widths)

@@ -6,10 +6,11 @@
 // where it is stored.
 //
 // Bound: HBM. A row is read once, kept in registers (at most 32 values per thread) through the sum of squares (and the
-// row maximum of the 8-bit output) and written once. 8 to 512 threads take a row (the gradient, kShift and kScalar: to 1,024,
-// where 64 registers a thread spill 36 to 368 bytes forward and 460 to 664 in the gradient; its other forms up to 204), the
-// smallest group that holds it in registers: it needs the fewest exchanges and has the most bytes on their way per thread; where
-// those are few (bf16 rows), a group takes up to four rows at once. Three ways to lay a row over its threads:
+// row maximum of the 8-bit output) and written once. 8 to 512 threads take a row (the gradient, kShift and kScalar: to
+// 1,024, whose 64 registers a thread spill 36 to 368 bytes forward and 460 to 664 in the gradient; its other forms spill
+// up to 204), the smallest group that holds it in registers: it needs the fewest exchanges and has the most bytes on their
+// way per thread; where those are few (bf16 rows), a group takes up to four rows at once. Three ways to lay a row over its
+// threads:
 //   kWide    8 values per thread and access (16 bytes of bf16, 32 of float32, the widest accesses of sm_100): widths
 //            and strides that are multiples of 8;
 //   kShift   the same accesses for rows of any width that follow one another without gaps: groups of 8 start at the
@@ -20,8 +21,8 @@
 //   kScalar  one value per thread and access: other strides and addresses.
 // Measured (of the measured copy rate, 6,468 GB/s): 163,848 x 512, float32 stream + bf16 residual -> bf16 147 us (1.05),
 // -> e4m3 136 us (1.05), gradient 225 us (0.93: five arrays of a thread's values keep it to two blocks per SM); 60M
-// values of bf16 without a residual 41-47 us at widths of 512 to 4,096 (0.8-0.9: few bytes per row), odd widths 57-97. Rows brought to
-// 8 bits alone: 163,848 x 512 of float32 66 us (0.98), of bf16 50 (0.78).
+// values of bf16 without a residual 41-47 us at widths of 512 to 4,096 (0.8-0.9: few bytes per row), odd widths 57-97.
+// Rows brought to 8 bits alone: 163,848 x 512 of float32 66 us (0.98), of bf16 50 (0.78).
 #include "rms_rows.cuh"
 
 namespace fwn {
