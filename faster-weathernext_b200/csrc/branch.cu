@@ -1,0 +1,244 @@
+// A residual branch in one pass: the norm after a block, its gate, dropout, the addition to the scaled residual stream and
+// the norm before the next block,
+//   z = y rstd(y) post_weight,  s = alpha x + gate z m,  h = s rstd(s) weight,  rstd(v) = 1 / sqrt(mean(v^2) + eps),
+// with m dropout's mask (philox.cuh), and dropout alone. x, s float32 or bf16, y, gate and weights float32 or bf16, h bf16,
+// float32, or e4m3 with one float32 scale per row (max |h| / 448). Sums are float32, s is normalised unrounded.
+//
+// Bound: HBM. The two norms need two sums over a row, the second of values that depend on the first: a row stays in
+// registers through both, read once and written once. The threads of a row, their accesses (kWide: 8 values an access;
+// kShift: the same for contiguous rows of any width, from the aligned address before the row) and their exchanges are the
+// RMS norm's (rms_rows.cuh).
+#include "branch.cuh"
+#include "rms_rows.cuh"
+
+namespace fwn {
+
+namespace {
+
+template <class F>
+cudaError_t branch_width(int room, F f) {
+  using std::integral_constant;
+#define FWN_ROW(TPR, NV) \
+  if (room <= TPR * NV * 8) return f(integral_constant<int, TPR>(), integral_constant<int, NV>())
+  FWN_ROW(8, 1);
+  FWN_ROW(16, 1);
+  FWN_ROW(32, 1);
+  FWN_ROW(32, 2);
+  FWN_ROW(64, 2);
+  FWN_ROW(128, 2);
+  FWN_ROW(256, 2);
+  FWN_ROW(512, 2);
+#undef FWN_ROW
+  return cudaErrorInvalidValue;
+}
+
+// kShift: a row of the gate from the columns of the row's groups. A gate of every row's own starts off as the row does.
+template <int MODE, int V>
+__device__ __forceinline__ void gate_group(const void* gate, bool gate_bf16, int64_t row, int j, int d, bool values, bool more,
+                                           float (&v)[V]) {
+  const int64_t at = row * d;
+  if (MODE == kShift && values) {
+    if (gate_bf16) {
+      Raw<bf16, V> r;
+      load_group<MODE>(static_cast<const bf16*>(gate) + at, j, d, more, r);
+      expand<MODE>(r, j, d, v);
+    } else {
+      Raw<float, V> r;
+      load_group<MODE>(static_cast<const float*>(gate) + at, j, d, more, r);
+      expand<MODE>(r, j, d, v);
+    }
+  } else {
+    const void* from = gate_bf16 ? static_cast<const void*>(static_cast<const bf16*>(gate) + at)
+                                 : static_cast<const void*>(static_cast<const float*>(gate) + at);
+    weight_group<MODE>(from, gate_bf16, j, d, v);
+  }
+}
+
+template <class X, class Y, int TPR, int MODE, int NV>
+__global__ void __launch_bounds__(block_of(TPR), 512 / block_of(TPR)) branch_norm_kernel(const BranchParams p) {
+  constexpr int V = 8;
+  __shared__ float red[3][1][32];
+  Rows<TPR> at;
+  const int off = MODE == kShift ? static_cast<int>(at.row * p.d & 7) : 0;  // of all this group's rows
+  const int d = p.d;
+  const float over = 1.f / static_cast<float>(d);
+  const bool one_gate = p.gate_span >= p.rows, values = p.gate_span == 1 && !one_gate;
+  const bool drops = p.drop.threshold > 0;
+  const uint64_t seed = drops ? drop_seed(p.drop) : 0;
+  for (; at.base < p.rows; at.base += at.step, at.row += at.step) {
+    const int64_t row = at.row;
+    const int n = row < p.rows ? d : 0;
+    const bool more = (p.rows - 1 - row) * d >= V - 1;
+    Raw<X, V> xr[NV];
+    Raw<Y, V> yr[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = group_at<TPR, V>(i, off);
+      load_group<MODE>(static_cast<const Y*>(p.y) + row * p.y_stride, j, n, more, yr[i]);
+      load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, more, xr[i]);
+    }
+    float s[NV][V], sum[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      expand<MODE>(yr[i], group_at<TPR, V>(i, off), n, s[i]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0] = fmaf(s[i][e], s[i][e], sum[0]);
+    }
+    row_reduce<TPR, false>(sum, red[0]);
+    const float r1 = rsqrtf(sum[0] * over + p.eps);
+    sum[0] = 0.f;
+    const int64_t grow = one_gate || n == 0 ? 0 : values ? row : static_cast<uint32_t>(row) / static_cast<uint32_t>(p.gate_span);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = group_at<TPR, V>(i, off);
+      float w[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[i][e] *= r1;
+      if (p.post_weight != nullptr) {
+        weight_group<MODE>(p.post_weight, p.post_bf16, j, n, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[i][e] *= w[e];
+      }
+      if (p.gate != nullptr) {
+        gate_group<MODE>(p.gate, p.gate_bf16, grow, j, n, values, more, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[i][e] *= w[e];
+      }
+      if (drops) drop8(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3, s[i]);
+      expand<MODE>(xr[i], j, n, w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[i][e] = fmaf(p.alpha, w[e], s[i][e]);
+      store_group<MODE>(static_cast<X*>(p.s) + row * d, j, n, s[i]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum[0] = fmaf(s[i][e], s[i][e], sum[0]);
+    }
+    row_reduce<TPR, false>(sum, red[1]);
+    const float r2 = rsqrtf(sum[0] * over + p.eps);
+    if (p.rstd != nullptr && (threadIdx.x & (TPR - 1)) == 0 && n > 0)
+      reinterpret_cast<float2*>(p.rstd)[row] = make_float2(r1, r2);
+    float most[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[i][e] *= r2;
+      if (p.weight != nullptr) {
+        float w[V];
+        weight_group<MODE>(p.weight, p.weight_bf16, group_at<TPR, V>(i, off), n, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[i][e] *= w[e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) most[0] = max_nan(most[0], fabsf(s[i][e]));
+    }
+    if (p.out_type == kRmsE4m3) {
+      row_reduce<TPR, true>(most, red[2]);
+      const bool tiny = most[0] < kTinyRow;  // false for NaN, which the scale and the values keep
+      const float inv = tiny ? 0.f : kE4m3Max / most[0];
+      if ((threadIdx.x & (TPR - 1)) == 0 && n > 0) p.scale[row] = tiny ? 0.f : most[0] / kE4m3Max;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[i][e] *= inv;
+        store_group<MODE>(static_cast<e4m3_t*>(p.h) + row * d, group_at<TPR, V>(i, off), n, s[i]);
+      }
+    } else if (p.out_type == kRmsBf16) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store_group<MODE>(static_cast<bf16*>(p.h) + row * d, group_at<TPR, V>(i, off), n, s[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store_group<MODE>(static_cast<float*>(p.h) + row * d, group_at<TPR, V>(i, off), n, s[i]);
+    }
+  }
+}
+
+template <class X, class Y, int MODE>
+cudaError_t go(const BranchParams& p, cudaStream_t st) {
+  return branch_width(room_of(MODE, p.d), [&](auto tpr, auto nv) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, GROUPS = block_of(TPR) / TPR;
+    // kWide: the grid covers the rows. kShift: resident blocks walk them, a multiple of eight rows at a step.
+    int64_t blocks = (p.rows + GROUPS - 1) / GROUPS;
+    if (MODE == kShift) {
+      blocks = std::min<int64_t>(blocks, static_cast<int64_t>(p.sms) * (2048 / block_of(TPR)));
+      if (GROUPS < 8) blocks = (blocks + 7) / 8 * 8;
+    }
+    branch_norm_kernel<X, Y, TPR, MODE, NV><<<static_cast<unsigned>(blocks), block_of(TPR), 0, st>>>(p);
+    return cudaGetLastError();
+  });
+}
+template <class X, class Y>
+cudaError_t by_mode(const BranchParams& p, cudaStream_t st) {
+  return p.wide ? go<X, Y, kWide>(p, st) : go<X, Y, kShift>(p, st);
+}
+
+// ---- dropout alone -------------------------------------------------------------------------------------------------
+
+// Two groups of eight values a thread, so that both loads are on their way.
+template <class T, bool WIDE>
+__global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T* __restrict__ out, int64_t n, const DropParams drop) {
+  constexpr int U = 2;
+  const uint64_t seed = drop_seed(drop);
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 * U + threadIdx.x;
+  Raw<T, 8> r[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t at = (i0 + u * 256) * 8;
+    if (WIDE && at + 8 <= n) {
+      load_raw(x + at, r[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        Raw<T, 1> one;
+        one.u[0] = 0;
+        if (at + e < n) load_raw(x + at + e, one);
+        if constexpr (sizeof(T) == 4)
+          r[u].u[e] = one.u[0];
+        else
+          r[u].u[e / 2] = e & 1 ? r[u].u[e / 2] | one.u[0] << 16 : one.u[0];
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t at = (i0 + u * 256) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = raw_at(r[u], e);
+    drop8(drop, seed, static_cast<uint64_t>(at) >> 3, v);
+    if (WIDE && at + 8 <= n) {
+      store_vals(out + at, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float one[1] = {v[e]};
+        if (at + e < n) store_vals(out + at + e, one);
+      }
+    }
+  }
+}
+
+template <class T>
+cudaError_t dropout_by(const void* x, void* out, int64_t n, bool wide, const DropParams& drop, cudaStream_t st) {
+  const int64_t blocks = (n + 4095) / 4096;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  if (wide)
+    dropout_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<const T*>(x), static_cast<T*>(out), n, drop);
+  else
+    dropout_kernel<T, false><<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<const T*>(x), static_cast<T*>(out), n, drop);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_branch(const BranchParams& p, cudaStream_t st) {
+  if (p.rows == 0) return cudaSuccess;
+  if (p.x_bf16) return p.y_bf16 ? by_mode<bf16, bf16>(p, st) : by_mode<bf16, float>(p, st);
+  return p.y_bf16 ? by_mode<float, bf16>(p, st) : by_mode<float, float>(p, st);
+}
+
+cudaError_t launch_dropout(const void* x, void* out, int64_t n, bool bf16_values, bool wide, int sms, const DropParams& drop,
+                           cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  return bf16_values ? dropout_by<bf16>(x, out, n, wide, drop, st) : dropout_by<float>(x, out, n, wide, drop, st);
+}
+
+}  // namespace fwn

@@ -14,6 +14,7 @@
 #include "../../include/fwn_attn.h"
 #include "common.cuh"
 
+#include "abi.cuh"
 #include "attn_bwd.cuh"
 #include "attn_fwd.cuh"
 #include "attn_fwd_wide.cuh"
@@ -609,6 +610,43 @@ fwn_status bwd_dispatch(const fwn_attn_desc* desc, const void* q, const void* k,
                         void* dq, void* dk, void* dv, const void* ws, size_t ws_bytes, int parts, void* stream);
 
 }  // namespace
+
+// What the ABI's other translation units take from this one (abi.cuh).
+namespace fwn {
+
+fwn_status abi_fail(fwn_status s, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_last_error = buf;
+  return s;
+}
+fwn_status abi_ok() { return ok(); }
+int abi_sms() { return num_sms(); }
+
+fwn_status abi_map(CUtensorMap* map, const void* base, int32_t dtype, int rank, const int64_t* dims, const int64_t* strides,
+                   int box_bytes, int box_rows) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return fail(FWN_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
+  const int64_t es = abi_size(dtype);
+  cuuint64_t n[3] = {}, ld[2] = {};
+  for (int i = 0; i < rank; ++i) n[i] = static_cast<cuuint64_t>(dims[i]);
+  for (int i = 0; i + 1 < rank; ++i) ld[i] = static_cast<cuuint64_t>(strides[i] * es);
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_bytes / es), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, dtype == FWN_DTYPE_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                        : dtype == FWN_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT8,
+                   static_cast<cuuint32_t>(rank), const_cast<void*>(base), n, ld, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FWN_ERR_INVALID_ARGUMENT, "cuTensorMapEncodeTiled (rank %d) failed (%d)", rank, static_cast<int>(r));
+  return FWN_OK;
+}
+
+}  // namespace fwn
 
 extern "C" {
 

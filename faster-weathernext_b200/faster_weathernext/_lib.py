@@ -45,7 +45,8 @@ SYMBOLS = ("fwn_version", "fwn_last_error_string", "fwn_device_error", "fwn_lse_
            "fwn_gemm_bf16", "fwn_gemm_bf16_aux", "fwn_gemm_bf16_gather", "fwn_gnn_gather_add_act", "fwn_gnn_ln_segment_sum",
            "fwn_rms_norm", "fwn_rms_norm_bwd_workspace_size", "fwn_rms_norm_bwd", "fwn_linear_workspace_size", "fwn_linear",
            "fwn_linear_pack", "fwn_linear_bwd_workspace_size",
-           "fwn_linear_bwd", "fwn_test_attn_fwd_timeout")
+           "fwn_linear_bwd", "fwn_dropout", "fwn_branch_norm", "fwn_branch_norm_bwd_workspace_size", "fwn_branch_norm_bwd",
+           "fwn_test_attn_fwd_timeout")
 
 
 class AttnDesc(ctypes.Structure):
@@ -75,6 +76,19 @@ class LinearDesc(ctypes.Structure):
               ("out_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
               ("act", ctypes.c_int32), ("flags", ctypes.c_int32), ("lda", ctypes.c_int64), ("ldb", ctypes.c_int64),
               ("ldx", ctypes.c_int64), ("ldo", ctypes.c_int64)]
+
+
+class DropoutDesc(ctypes.Structure):
+  _fields_ = [("seed", ctypes.c_uint64), ("seed_at", ctypes.c_void_p), ("site", ctypes.c_uint32),
+              ("threshold", ctypes.c_uint32)]
+
+
+class BranchDesc(ctypes.Structure):
+  _fields_ = [("rows", ctypes.c_int64), ("x_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64),
+              ("gate_span", ctypes.c_int64), ("d", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+              ("y_dtype", ctypes.c_int32), ("post_dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
+              ("gate_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+              ("residual_scale", ctypes.c_float), ("reserved", ctypes.c_int32), ("drop", DropoutDesc)]
 
 
 class FwnError(RuntimeError):
@@ -129,6 +143,10 @@ def _declare(lib):
       "fwn_linear_pack": [_P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _I, _P],
       "fwn_linear_bwd_workspace_size": [ctypes.POINTER(LinearDesc), _P, _P, _P, ctypes.POINTER(_SZ)],
       "fwn_linear_bwd": [ctypes.POINTER(LinearDesc), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+      "fwn_dropout": [ctypes.POINTER(DropoutDesc), _P, _P, ctypes.c_int64, _I, _P],
+      "fwn_branch_norm": [ctypes.POINTER(BranchDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+      "fwn_branch_norm_bwd_workspace_size": [ctypes.POINTER(BranchDesc), ctypes.POINTER(_SZ)],
+      "fwn_branch_norm_bwd": [ctypes.POINTER(BranchDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
       "fwn_bitset_csr_count": [_P, _I, _I, _P, _P, _SZ, _P],
       "fwn_bitset_csr_fill": [_P, _I, _I, _P, _P, _P],
       "fwn_attn_fwd": [ctypes.POINTER(AttnDesc), _P, _P, _P, ctypes.POINTER(TileList), _P, _P, _P],

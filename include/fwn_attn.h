@@ -372,6 +372,67 @@ FWN_API fwn_status fwn_linear_bwd(const fwn_linear_desc* desc, const void* a, co
                                   const void* dy, void* d_a, void* d_b, void* d_bias, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
+/* ---- residual branches -----------------------------------------------------------------------------------------
+ * No counterpart in the reference. Dropout from a counter-based generator, whose mask is computed again wherever it is
+ * needed and never stored, and the norms after and before a block in one pass with its gate, dropout and residual scale.
+ *
+ * The mask of a tensor of values i = 0, 1, ... (row by row): Philox4x32-10 on the counter (i / 8, site, 0) under the key
+ * seed; value i takes the 16-bit number i % 8 of its words (low halves first) and becomes 0, whatever it was, where the
+ * number is below threshold (0 to 65,536, the probability times 65,536); the others are multiplied by 65536 / (65536 -
+ * threshold). seed_at (device memory, 8-byte aligned; NULL: seed) holds the seed: read when the kernels run, so that a
+ * captured graph takes a new mask where it was changed between replays. `site` tells apart the masks of one step. */
+typedef struct fwn_dropout_desc {
+  uint64_t seed;
+  const void* seed_at;
+  uint32_t site;
+  uint32_t threshold;
+} fwn_dropout_desc;
+
+/* out[i] = x[i] under the mask, n values of dtype (bf16 or float32; dropout's gradient is the same call on the output's
+ * gradient). out may be x. */
+FWN_API fwn_status fwn_dropout(const fwn_dropout_desc* drop, const void* x, void* out, int64_t n, int32_t dtype, void* stream);
+
+/* With rstd(v) = 1 / sqrt(mean(v^2) + eps) over rows of d values:
+ *   z = y rstd(y) post_weight,  s = residual_scale x + (gate z under the mask),  h = s rstd(s) weight.
+ * x and y have row strides in elements; everything else is contiguous; outputs do not overlap inputs. The gate has a row for
+ * every gate_span rows of x (gate_span = rows: one for all, 1: one for each; rows is a multiple of it). post_weight, weight
+ * [d], gate NULL: ones. d up to 8,192; rows whose addresses, strides and width allow it (32 bytes of float32, 16 of bf16;
+ * multiples of 8 values) move in wide accesses; others must be contiguous, from such an address, and at most 8,185 wide
+ * (FWN_ERR_UNSUPPORTED otherwise). */
+typedef struct fwn_branch_desc {
+  int64_t rows;
+  int64_t x_stride;
+  int64_t y_stride;
+  int64_t gate_span;
+  int32_t d;
+  int32_t x_dtype;       /* BF16 or F32: x, s, ds, dx */
+  int32_t y_dtype;       /* BF16 or F32: y, dy */
+  int32_t post_dtype;    /* BF16 or F32: post_weight, d_post_weight */
+  int32_t weight_dtype;  /* BF16 or F32: weight, d_weight */
+  int32_t gate_dtype;    /* BF16 or F32: gate, d_gate */
+  int32_t out_dtype;     /* h: BF16, F32 or E4M3; dh (BF16 or F32) */
+  float eps;
+  float residual_scale;
+  int32_t reserved;      /* 0 */
+  fwn_dropout_desc drop;
+} fwn_branch_desc;
+
+/* Forward. s [rows, d] receives the stream (rounded to x_dtype; h is computed from the unrounded), h [rows, d] the norm;
+ * with an E4M3 h, scale [rows] receives max |h| / 448 (a row whose max |h| is below 2^-100: scale 0 and values 0).
+ * rstd (NULL, or float32 [rows, 2]) receives rstd(y) and rstd(s), which the backward needs. */
+FWN_API fwn_status fwn_branch_norm(const fwn_branch_desc* desc, const void* x, const void* y, const void* post_weight,
+                                   const void* weight, const void* gate, void* s, void* h, float* scale, float* rstd,
+                                   void* stream);
+
+/* Backward: the forward's inputs and rstd, dh [rows, d] (out_dtype) and ds [rows, d] (x_dtype), the gradients of h and s,
+ * either NULL (none). dx, dy, d_post_weight, d_weight, d_gate as the tensors they belong to, each NULL (not computed).
+ * Deterministic. workspace: fwn_branch_norm_bwd_workspace_size bytes, 16-byte aligned (0 bytes: may be NULL). */
+FWN_API fwn_status fwn_branch_norm_bwd_workspace_size(const fwn_branch_desc* desc, size_t* bytes);
+FWN_API fwn_status fwn_branch_norm_bwd(const fwn_branch_desc* desc, const void* x, const void* y, const void* post_weight,
+                                       const void* weight, const void* gate, const float* rstd, const void* dh,
+                                       const void* ds, void* dx, void* dy, void* d_post_weight, void* d_weight, void* d_gate,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- grid <-> mesh interaction networks -------------------------------------------------------------------
  * The blocked GNNs of the encoder / decoder (src/faster_weathernext/patch.py:347-509, ChunkedDeepGNN: edge MLP on
  * (edge, sender, receiver) features with the first layer's matmul applied per node before the gather, a sorted
