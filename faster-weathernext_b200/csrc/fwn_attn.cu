@@ -20,6 +20,7 @@
 #include "attn_fwd_wide.cuh"
 #include "attn_bwd_wide.cuh"
 #include "gemm.cuh"
+#include "grouped.cuh"
 #include "linear.cuh"
 #include "rms.cuh"
 #include "tiles.cuh"
@@ -669,6 +670,10 @@ fwn_status fwn_device_error(void* stream, int32_t* code) {
   e = fwn::take_linear_error(&linear_word);
   if (e != cudaSuccess) return cuda_fail(e, "device error word (projections)");
   word |= linear_word;
+  for (auto take : {fwn::take_grouped_error, fwn::take_grouped_fwd_error, fwn::take_grouped_bwd_error}) {
+    if ((e = take(&linear_word)) != cudaSuccess) return cuda_fail(e, "device error word (experts)");
+    word |= linear_word;
+  }
   *code = !word ? 0 : (word & 0x400u) ? FWN_ERR_INVALID_ARGUMENT : FWN_ERR_DEVICE_TIMEOUT;
   return ok();
 }

@@ -43,6 +43,20 @@ struct LinearParams {
   int64_t split_rows;    // rows of one split's partial sums in the output (splits > 1)
 };
 
+// Products grouped by expert (grouped.cu) on the same kernel: none; an expert's rows by its weight; an expert's rows summed over.
+enum LinearGroup { kGroupNone = 0, kGroupRows = 1, kGroupK = 2 };
+struct GroupParams {
+  const int32_t* offsets;     // [groups + 1]: the experts' first rows, in order and within the tensor
+  const int32_t* first;       // [groups + 1]: tiles of rows (runs of k) before an expert's
+  const CUtensorMap* map_a;   // [groups] each, written on the device: a, b (kGroupK), x and out (kGroupRows)
+  const CUtensorMap* map_b;
+  const CUtensorMap* map_x;
+  const CUtensorMap* map_o;
+  int groups;
+  int run;                    // kGroupK: stages of k in a run
+  bool by_run;                // kGroupK: out has a matrix for every run (else for every expert)
+};
+
 cudaError_t launch_linear_tiles(int tile, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx,
                                 const CUtensorMap& to, const LinearParams& p, int sms, cudaStream_t stream);
 // out = epilogue(sum over splits of part); p as of the whole product, part [splits, split_rows, ldp].

@@ -46,6 +46,8 @@ SYMBOLS = ("fwn_version", "fwn_last_error_string", "fwn_device_error", "fwn_lse_
            "fwn_rms_norm", "fwn_rms_norm_bwd_workspace_size", "fwn_rms_norm_bwd", "fwn_linear_workspace_size", "fwn_linear",
            "fwn_linear_pack", "fwn_linear_bwd_workspace_size",
            "fwn_linear_bwd", "fwn_dropout", "fwn_branch_norm", "fwn_branch_norm_bwd_workspace_size", "fwn_branch_norm_bwd",
+           "fwn_linear_grouped_workspace_size", "fwn_linear_grouped", "fwn_linear_grouped_bwd_workspace_size",
+           "fwn_linear_grouped_bwd",
            "fwn_test_attn_fwd_timeout")
 
 
@@ -89,6 +91,13 @@ class BranchDesc(ctypes.Structure):
               ("y_dtype", ctypes.c_int32), ("post_dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32),
               ("gate_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("eps", ctypes.c_float),
               ("residual_scale", ctypes.c_float), ("reserved", ctypes.c_int32), ("drop", DropoutDesc)]
+
+
+class GroupedDesc(ctypes.Structure):
+  _fields_ = [("m", ctypes.c_int64), ("groups", ctypes.c_int32), ("n", ctypes.c_int32), ("k", ctypes.c_int32),
+              ("out_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+              ("act", ctypes.c_int32), ("flags", ctypes.c_int32), ("lda", ctypes.c_int64), ("ldb", ctypes.c_int64),
+              ("b_stride", ctypes.c_int64), ("ldx", ctypes.c_int64)]
 
 
 class FwnError(RuntimeError):
@@ -147,6 +156,10 @@ def _declare(lib):
       "fwn_branch_norm": [ctypes.POINTER(BranchDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
       "fwn_branch_norm_bwd_workspace_size": [ctypes.POINTER(BranchDesc), ctypes.POINTER(_SZ)],
       "fwn_branch_norm_bwd": [ctypes.POINTER(BranchDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+      "fwn_linear_grouped_workspace_size": [ctypes.POINTER(GroupedDesc), ctypes.POINTER(_SZ)],
+      "fwn_linear_grouped": [ctypes.POINTER(GroupedDesc), _P, _P, _P, _P, _P, _P, _SZ, _P],
+      "fwn_linear_grouped_bwd_workspace_size": [ctypes.POINTER(GroupedDesc), _P, ctypes.POINTER(_SZ)],
+      "fwn_linear_grouped_bwd": [ctypes.POINTER(GroupedDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
       "fwn_bitset_csr_count": [_P, _I, _I, _P, _P, _SZ, _P],
       "fwn_bitset_csr_fill": [_P, _I, _I, _P, _P, _P],
       "fwn_attn_fwd": [ctypes.POINTER(AttnDesc), _P, _P, _P, ctypes.POINTER(TileList), _P, _P, _P],

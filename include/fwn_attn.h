@@ -433,6 +433,45 @@ FWN_API fwn_status fwn_branch_norm_bwd(const fwn_branch_desc* desc, const void* 
                                        const void* ds, void* dx, void* dy, void* d_post_weight, void* d_weight, void* d_gate,
                                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- mixtures of experts ---------------------------------------------------------------------------------------
+ * No counterpart in the reference (its MLPs are dense, src/faster_weathernext/patch.py:250-252). Products grouped by expert:
+ * rows offsets[e] <= i < offsets[e + 1] of a [m, k] are expert e's,
+ *   out[i, :] = act(a[i, :] b[e]^T + bias[e]),  b [groups, n, k] (or [groups, k, n]), bias [groups, n] or NULL,
+ * and rows of no expert (before offsets[0], from offsets[groups] on) are 0 in out. offsets, int32 [groups + 1] in device
+ * memory, are read there alone: no call waits for them. They are not decreasing and within [0, m]; others are raised to the
+ * one before, brought into the range, and reported by fwn_device_error as FWN_ERR_INVALID_ARGUMENT. bf16 operands, float32
+ * accumulation; out bf16 or float32, contiguous, overlapping no input. Precision as fwn_linear's.
+ * groups up to 1,023, n and k up to 2^20. a and b start at, and have row and expert strides that are, multiples of 16 bytes
+ * (FWN_ERR_UNSUPPORTED otherwise; fwn_linear_pack lays out others), except for m <= 8 with b [groups, n, k]. */
+typedef struct fwn_grouped_desc {
+  int64_t m;
+  int32_t groups;
+  int32_t n;
+  int32_t k;
+  int32_t out_dtype;   /* BF16 or F32 */
+  int32_t bias_dtype;  /* BF16 or F32 */
+  int32_t x_dtype;     /* dy: BF16 or F32 */
+  int32_t act;         /* fwn_act */
+  int32_t flags;       /* 0 or FWN_LINEAR_B_N_CONTIGUOUS: b is [groups, k, n] */
+  int64_t lda;         /* row strides in elements */
+  int64_t ldb;
+  int64_t b_stride;    /* between experts */
+  int64_t ldx;         /* of dy */
+} fwn_grouped_desc;
+
+/* Workspaces: 256-byte aligned; a call's own, not shared by calls that may overlap. */
+FWN_API fwn_status fwn_linear_grouped_workspace_size(const fwn_grouped_desc* desc, size_t* bytes);
+FWN_API fwn_status fwn_linear_grouped(const fwn_grouped_desc* desc, const void* a, const void* b, const void* bias,
+                                      const int32_t* offsets, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Backward, as fwn_linear_bwd's for each expert: dy [m, n], the gradient of out; d_a [m, k] (0 in rows of no expert), d_b in
+ * b's own orientation (0 for an expert without rows), both bf16 and contiguous, d_bias [groups, n] in bias_dtype; each may
+ * be NULL (d_bias: must be without a bias). Deterministic. */
+FWN_API fwn_status fwn_linear_grouped_bwd_workspace_size(const fwn_grouped_desc* desc, const void* dy, size_t* bytes);
+FWN_API fwn_status fwn_linear_grouped_bwd(const fwn_grouped_desc* desc, const void* a, const void* b, const void* bias,
+                                          const int32_t* offsets, const void* dy, void* d_a, void* d_b, void* d_bias,
+                                          void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- grid <-> mesh interaction networks -------------------------------------------------------------------
  * The blocked GNNs of the encoder / decoder (src/faster_weathernext/patch.py:347-509, ChunkedDeepGNN: edge MLP on
  * (edge, sender, receiver) features with the first layer's matmul applied per node before the gather, a sorted
