@@ -23,6 +23,7 @@
 #include "grouped.cuh"
 #include "linear.cuh"
 #include "rms.cuh"
+#include "routing.cuh"
 #include "tiles.cuh"
 
 namespace {
@@ -670,7 +671,8 @@ fwn_status fwn_device_error(void* stream, int32_t* code) {
   e = fwn::take_linear_error(&linear_word);
   if (e != cudaSuccess) return cuda_fail(e, "device error word (projections)");
   word |= linear_word;
-  for (auto take : {fwn::take_grouped_error, fwn::take_grouped_fwd_error, fwn::take_grouped_bwd_error}) {
+  for (auto take : {fwn::take_grouped_error, fwn::take_grouped_fwd_error, fwn::take_grouped_bwd_error,
+                    fwn::take_routing_error}) {
     if ((e = take(&linear_word)) != cudaSuccess) return cuda_fail(e, "device error word (experts)");
     word |= linear_word;
   }

@@ -1,0 +1,442 @@
+// Routing of rows to experts: the largest logits of each row and their softmax, the rows in the experts' order (a stable
+// counting sort), and the ways there and back with their gradients.
+//
+// Bound: HBM for the rows' ways (a row is read once and written to its `top` places, or the other way round; going by the
+// sorted rows instead would read a row `top` times), launches for the sort: one for few rows, else three (choice and counts
+// per block, prefixes over the blocks, places). No atomics decide an order: the same bits every time.
+#include <algorithm>
+
+#include "rms_rows.cuh"
+#include "routing.cuh"
+
+namespace fwn {
+
+__device__ unsigned int g_routing_device_error = 0;
+
+namespace {
+
+// A logit and its place as one number that orders as the choice does: larger logits first (NaN largest, -0 as 0), then
+// the lower expert. 0 is below every logit's.
+__device__ __forceinline__ unsigned long long rank_of(float v, int e) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  const uint32_t key = v != v ? 0xFFFFFFFFu : u & 0x80000000u ? ~u : u | 0x80000000u;
+  return static_cast<unsigned long long>(key) << 32 | (0xFFFFFFFFu - static_cast<uint32_t>(e));
+}
+__device__ __forceinline__ int expert_of(unsigned long long r) { return static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(r)); }
+__device__ __forceinline__ float logit_of(unsigned long long r) {
+  const uint32_t key = static_cast<uint32_t>(r >> 32);
+  return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);  // NaN's key gives a NaN
+}
+
+// The block's rows: LPR lanes a row, NV logits a lane; `hist` [experts] counts their choices.
+template <class T, int LPR, int NV>
+__device__ void choose(const RouteParams& p, int64_t first, int* hist) {
+  const int lane = threadIdx.x & (LPR - 1), per = blockDim.x / LPR;
+  const T* logits = static_cast<const T*>(p.logits);
+  for (int r = threadIdx.x / LPR; r < kRouteRows; r += per) {
+    const int64_t row = first + r;
+    const bool in = row < p.rows;
+    unsigned long long keys[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = i * LPR + lane;
+      keys[i] = in && e < p.experts ? rank_of(static_cast<float>(logits[row * p.stride + e]), e) : 0ull;
+    }
+    float top = 0.f, sum = 0.f, mine[kRouteTopMax / LPR + 1];  // choice j is lane j % LPR's
+    int who[kRouteTopMax / LPR + 1];
+#pragma unroll
+    for (int j0 = 0; j0 < kRouteTopMax / LPR + 1; ++j0) {
+      mine[j0] = 0.f;
+      who[j0] = 0;
+    }
+#pragma unroll 1
+    for (int j = 0; j < p.top; ++j) {
+      unsigned long long best = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) best = max(best, keys[i]);
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) keys[i] = keys[i] == best ? 0ull : keys[i];
+      const float v = logit_of(best);
+      if (j == 0) top = v;
+      // A row whose logits are all -infinity: weights 0.
+      const float w = top == -INFINITY ? 0.f : expf(v - top);
+      sum += w;
+#pragma unroll
+      for (int j0 = 0; j0 < kRouteTopMax / LPR + 1; ++j0) {
+        if (j == j0 * LPR + lane) {
+          mine[j0] = w;
+          who[j0] = expert_of(best);
+        }
+      }
+    }
+#pragma unroll
+    for (int j0 = 0; j0 < kRouteTopMax / LPR + 1; ++j0) {
+      const int j = j0 * LPR + lane;
+      if (in && j < p.top) {
+        p.chosen[row * p.top + j] = who[j0];
+        p.weights[row * p.top + j] = top == -INFINITY ? 0.f : mine[j0] / sum;
+        atomicAdd(hist + who[j0], 1);
+      }
+    }
+  }
+}
+
+// The places of the block's pairs (row, choice) in their order: `base` [experts] is where the block's first of each expert
+// goes; `count` [8, experts] is the warps' workspace. A warp takes adjacent pairs.
+__device__ void place(const RouteParams& p, int64_t first, const int* base, int* count) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pairs = static_cast<int>(min(static_cast<int64_t>(kRouteRows), p.rows - first)) * p.top;
+  const int each = (pairs + 255) / 256 * 32;
+  const int begin = warp * each, end = min(pairs, begin + each);
+  int* mine = count + warp * p.experts;
+  for (int i = threadIdx.x; i < 8 * p.experts; i += blockDim.x) count[i] = 0;
+  __syncthreads();
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int i = begin; i < end; i += 32) {
+      const bool in = i + lane < end;
+      const int64_t pair = first * p.top + i + lane;
+      const int e = in ? p.chosen[pair] : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, e);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      const int at = in ? mine[e] : 0;
+      __syncwarp();
+      if (in && rank == 0) mine[e] = at + __popc(same);
+      __syncwarp();
+      if (pass == 1 && in) {
+        p.position[pair] = at + rank;
+        p.order[at + rank] = static_cast<int32_t>(pair);
+      }
+    }
+    __syncthreads();
+    if (pass == 0) {
+      for (int e = threadIdx.x; e < p.experts; e += blockDim.x) {
+        int at = base[e];
+        for (int w = 0; w < 8; ++w) {
+          const int n = count[w * p.experts + e];
+          count[w * p.experts + e] = at;
+          at += n;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Exclusive prefixes of total [n] (n <= 1,023) by a block of 256 threads, with the sum behind them: out [n + 1].
+__device__ void prefixes(const int* total, int n, int* out) {
+  __shared__ int sums[256];
+  const int t = threadIdx.x;
+  int v[4], s = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = 4 * t + i < n ? total[4 * t + i] : 0;
+    s += v[i];
+  }
+  sums[t] = s;
+  __syncthreads();
+  for (int o = 1; o < 256; o <<= 1) {
+    const int u = t >= o ? sums[t - o] : 0;
+    __syncthreads();
+    sums[t] += u;
+    __syncthreads();
+  }
+  int at = sums[t] - s;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (4 * t + i <= n) out[4 * t + i] = at;
+    at += v[i];
+  }
+  __syncthreads();
+}
+
+// ONE: all rows are one block's: choice, prefixes and places in this launch.
+template <class T, int LPR, int NV, bool ONE>
+__global__ void __launch_bounds__(256) route_choose_kernel(const RouteParams p) {
+  extern __shared__ int route_smem[];  // hist [experts]; ONE: prefixes [experts + 1], counts [8, experts] too
+  int* hist = route_smem;
+  for (int e = threadIdx.x; e < p.experts; e += 256) hist[e] = 0;
+  __syncthreads();
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kRouteRows;
+  choose<T, LPR, NV>(p, first, hist);
+  __syncthreads();
+  if constexpr (ONE) {
+    int* at = hist + p.experts;
+    prefixes(hist, p.experts, at);
+    for (int e = threadIdx.x; e <= p.experts; e += 256) p.offsets[e] = at[e];
+    place(p, 0, at, at + p.experts + 1);
+  } else {
+    for (int e = threadIdx.x; e < p.experts; e += 256) p.counts[static_cast<int64_t>(e) * gridDim.x + blockIdx.x] = hist[e];
+  }
+}
+
+// A warp per expert: its blocks' counts become prefixes, and its total.
+__global__ void __launch_bounds__(256) route_scan_kernel(const RouteParams p, int64_t blocks) {
+  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (e >= p.experts) return;
+  int32_t* c = p.counts + e * blocks;
+  int total = 0;
+  for (int64_t b0 = 0; b0 < blocks; b0 += 128) {
+    int v[4], s = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = b0 + 4 * lane + i < blocks ? c[b0 + 4 * lane + i] : 0;
+      s += v[i];
+    }
+    int upto = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    int at = total + upto - s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (b0 + 4 * lane + i < blocks) c[b0 + 4 * lane + i] = at;
+      at += v[i];
+    }
+    total += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  if (lane == 0) p.totals[e] = total;
+}
+
+__global__ void __launch_bounds__(256) route_place_kernel(const RouteParams p) {
+  extern __shared__ int route_smem[];  // prefixes [experts + 1], counts [8, experts]
+  int* at = route_smem;
+  prefixes(p.totals, p.experts, at);
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= p.experts; e += 256) p.offsets[e] = at[e];
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.experts; e += 256) at[e] += p.counts[static_cast<int64_t>(e) * gridDim.x + blockIdx.x];
+  __syncthreads();
+  place(p, static_cast<int64_t>(blockIdx.x) * kRouteRows, at, at + p.experts + 1);
+}
+
+template <class T, int LPR, int NV>
+cudaError_t route_go(const RouteParams& p, cudaStream_t st) {
+  const int64_t blocks = route_blocks(p.rows);
+  const size_t e = static_cast<size_t>(p.experts) * sizeof(int);
+  if (blocks == 1) {
+    route_choose_kernel<T, LPR, NV, true><<<1, 256, 10 * e + sizeof(int), st>>>(p);
+    return cudaGetLastError();
+  }
+  route_choose_kernel<T, LPR, NV, false><<<static_cast<unsigned>(blocks), 256, e, st>>>(p);
+  route_scan_kernel<<<(p.experts + 7) / 8, 256, 0, st>>>(p, blocks);
+  route_place_kernel<<<static_cast<unsigned>(blocks), 256, 9 * e + sizeof(int), st>>>(p);
+  return cudaGetLastError();
+}
+template <class T>
+cudaError_t route_by(const RouteParams& p, cudaStream_t st) {
+  if (p.experts <= 8) return route_go<T, 8, 1>(p, st);
+  if (p.experts <= 16) return route_go<T, 16, 1>(p, st);
+  if (p.experts <= 32) return route_go<T, 32, 1>(p, st);
+  if (p.experts <= 64) return route_go<T, 32, 2>(p, st);
+  if (p.experts <= 128) return route_go<T, 32, 4>(p, st);
+  if (p.experts <= 256) return route_go<T, 32, 8>(p, st);
+  return route_go<T, 32, 32>(p, st);
+}
+
+// d logit[chosen j] = w_j (d w_j - sum over i of w_i d w_i), 0 elsewhere; a thread per logit.
+template <class T>
+__global__ void __launch_bounds__(256) route_bwd_kernel(const float* __restrict__ weights, const int32_t* __restrict__ chosen,
+                                                        const float* __restrict__ d_weights, int64_t rows, int experts, int top,
+                                                        T* __restrict__ d_logits) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= rows * experts) return;
+  const int64_t row = i / experts;
+  const int e = static_cast<int>(i - row * experts);
+  float sum = 0.f, w = 0.f, dw = 0.f;
+  for (int j = 0; j < top; ++j) {
+    const float a = __ldg(weights + row * top + j), b = __ldg(d_weights + row * top + j);
+    sum = fmaf(a, b, sum);
+    if (__ldg(chosen + row * top + j) == e) {
+      w = a;
+      dw = b;
+    }
+  }
+  const float v = w == 0.f ? 0.f : w * (dw - sum);
+  if constexpr (sizeof(T) == 2)
+    d_logits[i] = __float2bfloat16_rn(v);
+  else
+    d_logits[i] = v;
+}
+
+// ---- the rows' ways -------------------------------------------------------------------------------------------------
+
+// The place of a pair, or -1 (reported) where it would lie outside.
+__device__ __forceinline__ int64_t place_of(const RowMoveParams& p, int64_t row, int j) {
+  const int32_t at = __ldg(p.position + row * p.top + j);
+  if (at >= 0 && at < p.rows * p.top) return at;
+  atomicOr(&g_routing_device_error, 0x400u);
+  return -1;
+}
+
+// A warp per row. DOTS: the products x . y of the row's places too. V values an access; U accesses of a row on their way.
+template <class T, int V, int K, bool DOTS>
+__global__ void __launch_bounds__(256) spread_kernel(const RowMoveParams p) {
+  constexpr int U = DOTS ? (K >= 8 ? 1 : 2) : V == 8 ? 4 / (sizeof(T) / 2) : 8;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const int lane = threadIdx.x & 31;
+  int64_t at[K];
+  float w[K], dot[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    at[j] = j < p.top ? place_of(p, row, j) : -1;
+    w[j] = p.weights != nullptr && j < p.top ? __ldg(p.weights + row * p.top + j) : 1.f;
+    dot[j] = 0.f;
+  }
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  for (int c0 = lane * V; c0 < p.d; c0 += 32 * V * U) {
+    Raw<T, V> r[U], q[DOTS ? K : 1][DOTS ? U : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 32 * V;
+      if (c < p.d) load_raw(x + c, r[u]);
+    }
+    if constexpr (DOTS) {
+#pragma unroll
+      for (int j = 0; j < K; ++j)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = c0 + u * 32 * V;
+          if (at[j] >= 0 && c < p.d) load_raw(static_cast<const T*>(p.y) + at[j] * p.d + c, q[j][u]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 32 * V;
+      if (c >= p.d) break;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if (at[j] < 0) continue;
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = raw_at(r[u], e);
+        if constexpr (DOTS) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) dot[j] = fmaf(v[e], raw_at(q[j][u], e), dot[j]);
+        }
+        if (p.weights != nullptr) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[e] *= w[j];
+        }
+        if (p.to != nullptr) store_vals(static_cast<T*>(p.to) + at[j] * p.d + c, v);
+      }
+    }
+  }
+  if constexpr (DOTS) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+      if (lane == j && j < p.top) p.dots[row * p.top + j] = dot[j];
+    }
+  }
+}
+
+template <class T, int V, int K>
+__global__ void __launch_bounds__(256) gather_kernel(const RowMoveParams p) {
+  constexpr int U = K * V * static_cast<int>(sizeof(T)) >= 64 ? 1 : 64 / (K * V * static_cast<int>(sizeof(T))) > 8 ? 8 : 64 / (K * V * static_cast<int>(sizeof(T)));
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= p.rows) return;
+  const int lane = threadIdx.x & 31;
+  int64_t at[K];
+  float w[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    at[j] = j < p.top ? place_of(p, row, j) : -1;
+    w[j] = p.weights != nullptr && j < p.top ? __ldg(p.weights + row * p.top + j) : 1.f;
+  }
+  for (int c0 = lane * V; c0 < p.d; c0 += 32 * V * U) {
+    Raw<T, V> q[K][U];
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = c0 + u * 32 * V;
+        if (at[j] >= 0 && c < p.d) load_raw(static_cast<const T*>(p.y) + at[j] * p.d + c, q[j][u]);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int c = c0 + u * 32 * V;
+      if (c >= p.d) break;
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = 0.f;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if (at[j] < 0) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = fmaf(w[j], raw_at(q[j][u], e), v[e]);
+      }
+      store_vals(static_cast<T*>(p.to) + row * p.d + c, v);
+    }
+  }
+}
+
+template <class F>
+cudaError_t by_top(int top, F f) {
+  using std::integral_constant;
+  if (top <= 1) return f(integral_constant<int, 1>());
+  if (top <= 2) return f(integral_constant<int, 2>());
+  if (top <= 4) return f(integral_constant<int, 4>());
+  if (top <= 8) return f(integral_constant<int, 8>());
+  return f(integral_constant<int, kRouteTopMax>());
+}
+unsigned row_blocks(int64_t rows) { return static_cast<unsigned>((rows + 7) / 8); }
+
+template <class T, int V>
+cudaError_t spread_go(const RowMoveParams& p, cudaStream_t st) {
+  return by_top(p.top, [&](auto k) {
+    constexpr int K = decltype(k)::value;
+    if (p.dots != nullptr)
+      spread_kernel<T, V, K, true><<<row_blocks(p.rows), 256, 0, st>>>(p);
+    else
+      spread_kernel<T, V, K, false><<<row_blocks(p.rows), 256, 0, st>>>(p);
+    return cudaGetLastError();
+  });
+}
+template <class T, int V>
+cudaError_t gather_go(const RowMoveParams& p, cudaStream_t st) {
+  return by_top(p.top, [&](auto k) {
+    gather_kernel<T, V, decltype(k)::value><<<row_blocks(p.rows), 256, 0, st>>>(p);
+    return cudaGetLastError();
+  });
+}
+
+}  // namespace
+
+cudaError_t launch_route(const RouteParams& p, cudaStream_t st) {
+  return p.bf16_logits ? route_by<bf16>(p, st) : route_by<float>(p, st);
+}
+
+cudaError_t launch_route_bwd(const float* weights, const int32_t* chosen, const float* d_weights, int64_t rows, int experts,
+                             int top, void* d_logits, bool bf16_logits, cudaStream_t st) {
+  const int64_t blocks = (rows * experts + 255) / 256;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  if (bf16_logits)
+    route_bwd_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(weights, chosen, d_weights, rows, experts, top, static_cast<bf16*>(d_logits));
+  else
+    route_bwd_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(weights, chosen, d_weights, rows, experts, top, static_cast<float*>(d_logits));
+  return cudaGetLastError();
+}
+
+cudaError_t launch_spread(const RowMoveParams& p, cudaStream_t st) {
+  if (p.bf16_rows) return p.wide ? spread_go<bf16, 8>(p, st) : spread_go<bf16, 1>(p, st);
+  return p.wide ? spread_go<float, 8>(p, st) : spread_go<float, 1>(p, st);
+}
+cudaError_t launch_gather(const RowMoveParams& p, cudaStream_t st) {
+  if (p.bf16_rows) return p.wide ? gather_go<bf16, 8>(p, st) : gather_go<bf16, 1>(p, st);
+  return p.wide ? gather_go<float, 8>(p, st) : gather_go<float, 1>(p, st);
+}
+
+cudaError_t take_routing_error(unsigned int* word) {
+  cudaError_t e = cudaMemcpyFromSymbol(word, g_routing_device_error, sizeof(*word));
+  if (e != cudaSuccess) return e;
+  const unsigned int zero = 0;
+  return cudaMemcpyToSymbol(g_routing_device_error, &zero, sizeof(zero));
+}
+
+}  // namespace fwn

@@ -16,7 +16,7 @@ INCLUDE = os.path.join(os.path.dirname(ROOT), "include")
 LIB = os.path.join(PKG, "libfwn_attn.so")
 SOURCES = ["fwn_attn.cu", "tiles.cu", "khop.cu", "norm.cu", "gnn.cu", "rms.cu", "rms_bwd.cu", "linear.cu",
            "branch.cu", "branch_bwd_f32.cu", "branch_bwd_bf16.cu", "branch_abi.cu",
-           "grouped.cu", "grouped_fwd.cu", "grouped_bwd.cu", "grouped_abi.cu"]
+           "grouped.cu", "grouped_fwd.cu", "grouped_bwd.cu", "grouped_abi.cu", "routing.cu", "routing_abi.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr"]

@@ -47,7 +47,8 @@ SYMBOLS = ("fwn_version", "fwn_last_error_string", "fwn_device_error", "fwn_lse_
            "fwn_linear_pack", "fwn_linear_bwd_workspace_size",
            "fwn_linear_bwd", "fwn_dropout", "fwn_branch_norm", "fwn_branch_norm_bwd_workspace_size", "fwn_branch_norm_bwd",
            "fwn_linear_grouped_workspace_size", "fwn_linear_grouped", "fwn_linear_grouped_bwd_workspace_size",
-           "fwn_linear_grouped_bwd",
+           "fwn_linear_grouped_bwd", "fwn_route_workspace_size", "fwn_route", "fwn_route_bwd", "fwn_route_spread",
+           "fwn_route_gather",
            "fwn_test_attn_fwd_timeout")
 
 
@@ -98,6 +99,11 @@ class GroupedDesc(ctypes.Structure):
               ("out_dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
               ("act", ctypes.c_int32), ("flags", ctypes.c_int32), ("lda", ctypes.c_int64), ("ldb", ctypes.c_int64),
               ("b_stride", ctypes.c_int64), ("ldx", ctypes.c_int64)]
+
+
+class RouteDesc(ctypes.Structure):
+  _fields_ = [("rows", ctypes.c_int64), ("experts", ctypes.c_int32), ("top", ctypes.c_int32), ("dtype", ctypes.c_int32),
+              ("reserved", ctypes.c_int32)]
 
 
 class FwnError(RuntimeError):
@@ -160,6 +166,11 @@ def _declare(lib):
       "fwn_linear_grouped": [ctypes.POINTER(GroupedDesc), _P, _P, _P, _P, _P, _P, _SZ, _P],
       "fwn_linear_grouped_bwd_workspace_size": [ctypes.POINTER(GroupedDesc), _P, ctypes.POINTER(_SZ)],
       "fwn_linear_grouped_bwd": [ctypes.POINTER(GroupedDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P],
+      "fwn_route_workspace_size": [ctypes.POINTER(RouteDesc), ctypes.POINTER(_SZ)],
+      "fwn_route": [ctypes.POINTER(RouteDesc), _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P, _SZ, _P],
+      "fwn_route_bwd": [ctypes.POINTER(RouteDesc), _P, _P, _P, _P, _P],
+      "fwn_route_spread": [ctypes.POINTER(RouteDesc), _I, _P, ctypes.c_int64, _P, _P, _P, _P, _P, _P],
+      "fwn_route_gather": [ctypes.POINTER(RouteDesc), _I, _P, _P, _P, _P, _P],
       "fwn_bitset_csr_count": [_P, _I, _I, _P, _P, _SZ, _P],
       "fwn_bitset_csr_fill": [_P, _I, _I, _P, _P, _P],
       "fwn_attn_fwd": [ctypes.POINTER(AttnDesc), _P, _P, _P, ctypes.POINTER(TileList), _P, _P, _P],

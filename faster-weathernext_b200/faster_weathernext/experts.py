@@ -8,10 +8,12 @@
 
 Everything is differentiable, and nothing waits for the device: the experts' sizes stay there. No counterpart in the
 reference, whose MLPs are dense (src/faster_weathernext/patch.py:250-252); beside projection.linear, whose kernel
-linear_grouped walks over the experts. The kernels are csrc/grouped*.cu and csrc/linear_tile.cuh (C ABI in
-include/fwn_attn.h, fwn_linear_grouped*). Every call runs on the current stream of its tensors' device and takes its
-workspace from torch's allocator.
+linear_grouped walks over the experts. The kernels are csrc/grouped*.cu, csrc/linear_tile.cuh and csrc/routing.cu (C ABI in
+include/fwn_attn.h, fwn_linear_grouped* and fwn_route*). Every call runs on the current stream of its tensors' device and
+takes its workspace from torch's allocator.
 """
+
+import dataclasses
 
 import torch
 
@@ -173,3 +175,172 @@ def linear_grouped(a, weight, offsets, bias=None, *, activation=None, out_dtype=
   else:
     weight = _orient3(weight)[0]
   return _on_device(a, _grouped_launch, a, weight, offsets, bias, act, out_dtype)
+
+
+# ---- routing ---------------------------------------------------------------------------------------------------------
+
+@dataclasses.dataclass(frozen=True)
+class Routing:
+  """Where rows go: experts [rows, top_k] int32 (largest logit first) and weights [rows, top_k] float32 (differentiable);
+  position [rows, top_k] int32, the place of each pair (row, choice) in the experts' order; order [rows * top_k] int32, the
+  pair (row * top_k + choice) in each place; offsets [experts + 1] int32, the first place of each expert."""
+  experts: torch.Tensor
+  weights: torch.Tensor
+  position: torch.Tensor
+  order: torch.Tensor
+  offsets: torch.Tensor
+
+
+def _route_launch(stream, logits, top_k):
+  rows, e = logits.shape
+  new = lambda shape, dtype=torch.int32: logits.new_empty(shape, dtype=dtype)  # noqa: E731
+  chosen, weights, position = new((rows, top_k)), new((rows, top_k), _F32), new((rows, top_k))
+  order, offsets = new((rows * top_k,)), new((e + 1,))
+  desc = _lib.RouteDesc(rows, e, top_k, _CODE[logits.dtype], 0)
+  lib = _lib.lib()
+  ws, size = _workspace(logits, desc, lib.fwn_route_workspace_size)
+  status = lib.fwn_route(desc, logits.data_ptr(), max(logits.stride(0), e), chosen.data_ptr(), weights.data_ptr(),
+                         order.data_ptr(), position.data_ptr(), offsets.data_ptr(), _ptr(ws), size, stream)
+  if status:
+    _lib.check(status)
+  return chosen, weights, position, order, offsets
+
+
+class _Route(torch.autograd.Function):
+  """route with the weights' gradient; the choice itself has none."""
+
+  @staticmethod
+  def forward(ctx, logits, top_k):
+    chosen, weights, position, order, offsets = _on_device(logits, _route_launch, _rows(logits), top_k)
+    ctx.mark_non_differentiable(chosen, position, order, offsets)
+    ctx.shape, ctx.dtype = logits.shape, logits.dtype
+    ctx.save_for_backward(chosen, weights)
+    return chosen, weights, position, order, offsets
+
+  @staticmethod
+  def backward(ctx, _chosen, d_weights, *_rest):
+    chosen, weights = ctx.saved_tensors
+    _no_tangent("route's gradient", weights, d_weights)
+    _first_order("route")
+    return _on_device(weights, _Route._launch, ctx, chosen, weights, d_weights.contiguous()), None
+
+  @staticmethod
+  def _launch(stream, ctx, chosen, weights, d_weights):
+    d_logits = weights.new_empty(ctx.shape, dtype=ctx.dtype)
+    desc = _lib.RouteDesc(chosen.shape[0], ctx.shape[1], chosen.shape[1], _CODE[ctx.dtype], 0)
+    status = _lib.lib().fwn_route_bwd(desc, weights.data_ptr(), chosen.data_ptr(), d_weights.data_ptr(), d_logits.data_ptr(),
+                                      stream)
+    if status:
+      _lib.check(status)
+    return d_logits
+
+
+def route(logits, top_k):
+  """The top_k largest of each row's logits [rows, e] (float32 or bf16, any strides; e <= 1,023, top_k <= 16) and their
+  softmax, and the rows in the experts' order: a Routing. Equal logits go to the lower expert, a NaN counts as the largest
+  (and gives its row NaN weights), -infinity has weight 0 (a row of nothing else: every weight 0). The sort is stable and
+  deterministic. Differentiable in the logits through the weights (backward; forward mode and second derivatives raise
+  NotImplementedError)."""
+  if logits.dim() != 2 or logits.shape[1] < 1:
+    raise ValueError(f"logits has shape {tuple(logits.shape)}, expected [rows, e] with e >= 1")
+  _check("logits", logits, logits, (_BF16, _F32))
+  if not isinstance(top_k, int) or not 1 <= top_k <= logits.shape[1]:
+    raise ValueError(f"top_k is {top_k!r}, expected a whole number of 1 to {logits.shape[1]}")
+  _no_tangent("route", logits)
+  if torch.is_grad_enabled() and logits.requires_grad:
+    return Routing(*_Route.apply(logits, top_k))
+  return Routing(*_on_device(logits, _route_launch, _rows(logits), top_k))
+
+
+def _move_desc(t, position):
+  rows, top_k = position.shape
+  return _lib.RouteDesc(rows, top_k, top_k, _CODE[t.dtype], 0)  # the number of experts does not matter here
+
+
+def _spread_launch(stream, x, position, weights, y, wanted):
+  """(weights[r, j] x[r] in the experts' order or None, dots with y or None)."""
+  rows, top_k = position.shape
+  d = x.shape[1]
+  out = x.new_empty((rows * top_k, d)) if wanted else None
+  dots = x.new_empty((rows, top_k), dtype=_F32) if y is not None else None
+  status = _lib.lib().fwn_route_spread(_move_desc(x, position), d, x.data_ptr(), max(x.stride(0), d), position.data_ptr(),
+                                       _ptr(weights), _ptr(y), _ptr(out), _ptr(dots), stream)
+  if status:
+    _lib.check(status)
+  return out, dots
+
+
+def _gather_launch(stream, y, position, weights):
+  out = y.new_empty((position.shape[0], y.shape[1]))
+  status = _lib.lib().fwn_route_gather(_move_desc(y, position), y.shape[1], y.data_ptr(), position.data_ptr(), _ptr(weights),
+                                       out.data_ptr(), stream)
+  if status:
+    _lib.check(status)
+  return out
+
+
+class _Dispatch(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, x, position):
+    ctx.save_for_backward(position)
+    return _on_device(x, _spread_launch, _rows(x), position, None, None, True)[0]
+
+  @staticmethod
+  def backward(ctx, d_rows):
+    position, = ctx.saved_tensors
+    _no_tangent("dispatch's gradient", d_rows)
+    _first_order("dispatch")
+    return _on_device(d_rows, _gather_launch, d_rows.contiguous(), position, None), None
+
+
+class _Combine(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, y, weights, position):
+    y2 = y.contiguous()
+    ctx.save_for_backward(y2, weights, position)
+    return _on_device(y2, _gather_launch, y2, position, weights)
+
+  @staticmethod
+  def backward(ctx, d_out):
+    y, weights, position = ctx.saved_tensors
+    _no_tangent("combine's gradient", y, weights, d_out)
+    _first_order("combine")
+    d_y, d_weights = _on_device(d_out, _spread_launch, _rows(d_out), position, weights, y if ctx.needs_input_grad[1] else None,
+                                ctx.needs_input_grad[0])
+    return d_y, d_weights, None
+
+
+def _routed_check(name, t, routing, each):
+  """t [rows * each, d] belongs to a routing of `rows` rows."""
+  _check(name, t, t, (_BF16, _F32))
+  _check("routing.position", routing.position, t, (torch.int32,))
+  _check("routing.weights", routing.weights, t, (_F32,))
+  if (routing.position.dim() != 2 or routing.weights.shape != routing.position.shape or not routing.position.is_contiguous()
+      or not routing.weights.is_contiguous()):
+    raise ValueError("routing's position and weights are not contiguous [rows, top_k] as route returns them")
+  rows = routing.position.shape[0] * each
+  if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1:
+    raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({rows}, d) with d >= 1")
+  _no_tangent(name, t, routing.weights)
+
+
+def dispatch(x, routing):
+  """The rows of x [rows, d] (float32 or bf16, any strides) in the experts' order: [rows * top_k, d], linear_grouped's left
+  operand with routing.offsets. Differentiable in x: the gradient of a row is the sum of its places', in float32, rounded
+  once (backward; forward mode and second derivatives raise NotImplementedError)."""
+  _routed_check("x", x, routing, 1)
+  if torch.is_grad_enabled() and x.requires_grad:
+    return _Dispatch.apply(x, routing.position)
+  return _on_device(x, _spread_launch, _rows(x), routing.position, None, None, True)[0]
+
+
+def combine(y, routing):
+  """The experts' rows y [rows * top_k, d] (float32 or bf16), in the experts' order, added back: out[r] = sum over a row's
+  choices of weight * y's row, in float32, rounded once to y's type. Differentiable in y and in the routing's weights
+  (backward; forward mode and second derivatives raise NotImplementedError)."""
+  _routed_check("y", y, routing, routing.position.shape[-1])
+  if torch.is_grad_enabled() and (y.requires_grad or routing.weights.requires_grad):
+    return _Combine.apply(y, routing.weights, routing.position)
+  return _on_device(y, _gather_launch, y.contiguous(), routing.position, routing.weights)

@@ -472,6 +472,40 @@ FWN_API fwn_status fwn_linear_grouped_bwd(const fwn_grouped_desc* desc, const vo
                                           const int32_t* offsets, const void* dy, void* d_a, void* d_b, void* d_bias,
                                           void* workspace, size_t workspace_bytes, void* stream);
 
+/* Routing of rows to experts. fwn_route: the `top` largest logits of each row (logits [rows, experts], row stride `stride`;
+ * equal ones: the lower expert; a NaN is the largest, -0 equals 0), largest first, into experts [rows, top], and their
+ * softmax into weights (float32 [rows, top]; a row whose logits are all -infinity: 0); then the pairs (row, choice) sorted
+ * by expert, in their order: order [rows top] holds the pair row top + choice of each sorted place, position [rows, top]
+ * the place of each pair, offsets [experts + 1] the first place of each expert (int32 all; fwn_linear_grouped's offsets).
+ * experts up to 1,023, top up to 16, rows top below 2^31. workspace: fwn_route_workspace_size bytes. */
+typedef struct fwn_route_desc {
+  int64_t rows;
+  int32_t experts;
+  int32_t top;
+  int32_t dtype;     /* of the logits, or of the rows moved: BF16 or F32 */
+  int32_t reserved;  /* 0 */
+} fwn_route_desc;
+FWN_API fwn_status fwn_route_workspace_size(const fwn_route_desc* desc, size_t* bytes);
+FWN_API fwn_status fwn_route(const fwn_route_desc* desc, const void* logits, int64_t stride, int32_t* experts, float* weights,
+                             int32_t* order, int32_t* position, int32_t* offsets, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* d_logits [rows, experts] (contiguous, dtype) of the weights' gradient: w_j (d w_j - sum over i of w_i d w_i) for the
+ * chosen, 0 for the others. */
+FWN_API fwn_status fwn_route_bwd(const fwn_route_desc* desc, const float* weights, const int32_t* experts,
+                                 const float* d_weights, void* d_logits, void* stream);
+
+/* The rows' ways, of d (`width`) values of dtype. fwn_route_spread: out[position[r, j]] = weights[r, j] x[r] (weights NULL:
+ * ones), and, with y [rows top, d], dots[r, j] = x[r] . y[position[r, j]] (float32; out may then be NULL). fwn_route_gather:
+ * out[r] = sum over j of weights[r, j] y[position[r, j]], in float32 and in that order. x has a row stride, the others are
+ * contiguous; outputs overlap no input. They are each other's gradients. A position outside [0, rows top) moves nothing and
+ * is reported by fwn_device_error as FWN_ERR_INVALID_ARGUMENT. */
+FWN_API fwn_status fwn_route_spread(const fwn_route_desc* desc, int32_t width, const void* x, int64_t x_stride,
+                                    const int32_t* position, const float* weights, const void* y, void* out, float* dots,
+                                    void* stream);
+FWN_API fwn_status fwn_route_gather(const fwn_route_desc* desc, int32_t width, const void* y, const int32_t* position,
+                                    const float* weights, void* out, void* stream);
+
 /* ---- grid <-> mesh interaction networks -------------------------------------------------------------------
  * The blocked GNNs of the encoder / decoder (src/faster_weathernext/patch.py:347-509, ChunkedDeepGNN: edge MLP on
  * (edge, sender, receiver) features with the first layer's matmul applied per node before the gather, a sorted
