@@ -8,21 +8,21 @@
 // registers through both, read once and written once. The threads of a row, their accesses (kWide: 8 values an access;
 // kShift: the same for contiguous rows of any width, from the aligned address before the row) and their exchanges are the
 // RMS norm's (rms_rows.cuh).
-#include "branch.cuh"
-#include "rms_rows.cuh"
+#include "branch_rows.cuh"
 
 namespace fwn {
 
 namespace {
 
+// Threads of a row and groups of eight values a thread: sixteen values, so that a thread has some 100 bytes on their way.
 template <class F>
 cudaError_t branch_width(int room, F f) {
   using std::integral_constant;
 #define FWN_ROW(TPR, NV) \
   if (room <= TPR * NV * 8) return f(integral_constant<int, TPR>(), integral_constant<int, NV>())
   FWN_ROW(8, 1);
-  FWN_ROW(16, 1);
-  FWN_ROW(32, 1);
+  FWN_ROW(8, 2);
+  FWN_ROW(16, 2);
   FWN_ROW(32, 2);
   FWN_ROW(64, 2);
   FWN_ROW(128, 2);
@@ -31,122 +31,104 @@ cudaError_t branch_width(int room, F f) {
 #undef FWN_ROW
   return cudaErrorInvalidValue;
 }
-
-// kShift: a row of the gate from the columns of the row's groups. A gate of every row's own starts off as the row does.
-template <int MODE, int V>
-__device__ __forceinline__ void gate_group(const void* gate, bool gate_bf16, int64_t row, int j, int d, bool values, bool more,
-                                           float (&v)[V]) {
-  const int64_t at = row * d;
-  if (MODE == kShift && values) {
-    if (gate_bf16) {
-      Raw<bf16, V> r;
-      load_group<MODE>(static_cast<const bf16*>(gate) + at, j, d, more, r);
-      expand<MODE>(r, j, d, v);
-    } else {
-      Raw<float, V> r;
-      load_group<MODE>(static_cast<const float*>(gate) + at, j, d, more, r);
-      expand<MODE>(r, j, d, v);
-    }
-  } else {
-    const void* from = gate_bf16 ? static_cast<const void*>(static_cast<const bf16*>(gate) + at)
-                                 : static_cast<const void*>(static_cast<const float*>(gate) + at);
-    weight_group<MODE>(from, gate_bf16, j, d, v);
-  }
-}
+constexpr int branch_resident(int tpr) { return 512 / block_of(tpr); }
 
 template <class X, class Y, int TPR, int MODE, int NV>
-__global__ void __launch_bounds__(block_of(TPR), 512 / block_of(TPR)) branch_norm_kernel(const BranchParams p) {
-  constexpr int V = 8;
+__global__ void __launch_bounds__(block_of(TPR), branch_resident(TPR)) branch_norm_kernel(const BranchParams p) {
   __shared__ float red[3][1][32];
   Rows<TPR> at;
   const int off = MODE == kShift ? static_cast<int>(at.row * p.d & 7) : 0;  // of all this group's rows
   const int d = p.d;
   const float over = 1.f / static_cast<float>(d);
-  const bool one_gate = p.gate_span >= p.rows, values = p.gate_span == 1 && !one_gate;
+  const bool one_gate = p.gate == nullptr || p.gate_span >= p.rows, own_gate = p.gate_span == 1 && !one_gate;
   const bool drops = p.drop.threshold > 0;
+  const uint32_t least = drop_least(p.drop);
+  const float factor = drops ? p.drop.factor : 1.f;
+  // The next row is on its way while one is worked on; the columns' factors stay in registers.
+  Raw<X, 8> xr[NV];
+  Raw<Y, 8> yr[NV];
+  auto fetch = [&](int64_t row) {
+    const int n = row < p.rows ? d : 0;
+    const bool more = (p.rows - 1 - row) * d >= 7;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = group_at<TPR, 8>(i, off);
+      load_group<MODE>(static_cast<const Y*>(p.y) + row * p.y_stride, j, n, more, yr[i]);
+      load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, more, xr[i]);
+    }
+  };
+  fetch(at.row);
+  V8 g[NV], w[NV];  // post_weight gate factor, weight
+  auto columns_of = [&](int64_t gate) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = group_at<TPR, 8>(i, off);
+      g[i] = mul(columns<MODE>(p.post_weight, p.post_bf16, j, d), factor);
+      if (p.gate != nullptr && !own_gate) g[i] = mul(g[i], columns<MODE>(gate_row(p.gate, p.gate_bf16, gate, d), p.gate_bf16, j, d));
+    }
+  };
+  int gate = -1;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) w[i] = columns<MODE>(p.weight, p.weight_bf16, group_at<TPR, 8>(i, off), d);
+  if (one_gate || own_gate) columns_of(0);
   const uint64_t seed = drops ? drop_seed(p.drop) : 0;
   for (; at.base < p.rows; at.base += at.step, at.row += at.step) {
     const int64_t row = at.row;
     const int n = row < p.rows ? d : 0;
-    const bool more = (p.rows - 1 - row) * d >= V - 1;
-    Raw<X, V> xr[NV];
-    Raw<Y, V> yr[NV];
+    if (!one_gate && !own_gate && n > 0) {
+      const int mine = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(p.gate_span));
+      if (mine != gate) columns_of(gate = mine);
+    }
+    V8 s[NV], x[NV];
+    float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, V>(i, off);
-      load_group<MODE>(static_cast<const Y*>(p.y) + row * p.y_stride, j, n, more, yr[i]);
-      load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, more, xr[i]);
+      const int j = group_at<TPR, 8>(i, off);
+      s[i] = values<MODE>(yr[i], j, n);
+      x[i] = mul(values<MODE>(xr[i], j, n), p.alpha);
+      dot(acc, s[i], s[i]);
     }
-    float s[NV][V], sum[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      expand<MODE>(yr[i], group_at<TPR, V>(i, off), n, s[i]);
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum[0] = fmaf(s[i][e], s[i][e], sum[0]);
-    }
+    if (at.base + at.step < p.rows) fetch(row + at.step);
+    float sum[1] = {acc.x + acc.y};
     row_reduce<TPR, false>(sum, red[0]);
     const float r1 = rsqrtf(sum[0] * over + p.eps);
-    sum[0] = 0.f;
-    const int64_t grow = one_gate || n == 0 ? 0 : values ? row : static_cast<uint32_t>(row) / static_cast<uint32_t>(p.gate_span);
+    acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, V>(i, off);
-      float w[V];
+      const int j = group_at<TPR, 8>(i, off);
+      s[i] = mul(mul(s[i], r1), g[i]);
+      if (own_gate) s[i] = mul(s[i], gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, (p.rows - 1 - row) * d >= 7));
+      if (drops) s[i] = kept(s[i], drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3), least);
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[i][e] *= r1;
-      if (p.post_weight != nullptr) {
-        weight_group<MODE>(p.post_weight, p.post_bf16, j, n, w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] *= w[e];
-      }
-      if (p.gate != nullptr) {
-        gate_group<MODE>(p.gate, p.gate_bf16, grow, j, n, values, more, w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] *= w[e];
-      }
-      if (drops) drop8(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3, s[i]);
-      expand<MODE>(xr[i], j, n, w);
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[i][e] = fmaf(p.alpha, w[e], s[i][e]);
-      store_group<MODE>(static_cast<X*>(p.s) + row * d, j, n, s[i]);
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum[0] = fmaf(s[i][e], s[i][e], sum[0]);
+      for (int q = 0; q < 4; ++q) s[i].p[q] = fadd2(s[i].p[q], x[i].p[q]);
+      put<MODE>(static_cast<X*>(p.s) + row * d, j, n, s[i]);
+      dot(acc, s[i], s[i]);
     }
+    sum[0] = acc.x + acc.y;
     row_reduce<TPR, false>(sum, red[1]);
     const float r2 = rsqrtf(sum[0] * over + p.eps);
     if (p.rstd != nullptr && (threadIdx.x & (TPR - 1)) == 0 && n > 0)
       reinterpret_cast<float2*>(p.rstd)[row] = make_float2(r1, r2);
-    float most[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[i][e] *= r2;
-      if (p.weight != nullptr) {
-        float w[V];
-        weight_group<MODE>(p.weight, p.weight_bf16, group_at<TPR, V>(i, off), n, w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] *= w[e];
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) most[0] = max_nan(most[0], fabsf(s[i][e]));
-    }
+    for (int i = 0; i < NV; ++i) s[i] = mul(mul(s[i], r2), w[i]);
     if (p.out_type == kRmsE4m3) {
+      float most[1] = {0.f};
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most[0] = max_nan(most[0], fabsf(at8(s[i], e)));
       row_reduce<TPR, true>(most, red[2]);
       const bool tiny = most[0] < kTinyRow;  // false for NaN, which the scale and the values keep
       const float inv = tiny ? 0.f : kE4m3Max / most[0];
       if ((threadIdx.x & (TPR - 1)) == 0 && n > 0) p.scale[row] = tiny ? 0.f : most[0] / kE4m3Max;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[i][e] *= inv;
-        store_group<MODE>(static_cast<e4m3_t*>(p.h) + row * d, group_at<TPR, V>(i, off), n, s[i]);
-      }
+      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<e4m3_t*>(p.h) + row * d, group_at<TPR, 8>(i, off), n, mul(s[i], inv));
     } else if (p.out_type == kRmsBf16) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) store_group<MODE>(static_cast<bf16*>(p.h) + row * d, group_at<TPR, V>(i, off), n, s[i]);
+      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<bf16*>(p.h) + row * d, group_at<TPR, 8>(i, off), n, s[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) store_group<MODE>(static_cast<float*>(p.h) + row * d, group_at<TPR, V>(i, off), n, s[i]);
+      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<float*>(p.h) + row * d, group_at<TPR, 8>(i, off), n, s[i]);
     }
   }
 }
@@ -155,12 +137,9 @@ template <class X, class Y, int MODE>
 cudaError_t go(const BranchParams& p, cudaStream_t st) {
   return branch_width(room_of(MODE, p.d), [&](auto tpr, auto nv) {
     constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, GROUPS = block_of(TPR) / TPR;
-    // kWide: the grid covers the rows. kShift: resident blocks walk them, a multiple of eight rows at a step.
-    int64_t blocks = (p.rows + GROUPS - 1) / GROUPS;
-    if (MODE == kShift) {
-      blocks = std::min<int64_t>(blocks, static_cast<int64_t>(p.sms) * (2048 / block_of(TPR)));
-      if (GROUPS < 8) blocks = (blocks + 7) / 8 * 8;
-    }
+    // Resident blocks walk the rows (kShift: a multiple of eight rows at a step).
+    int64_t blocks = std::min<int64_t>((p.rows + GROUPS - 1) / GROUPS, static_cast<int64_t>(p.sms) * branch_resident(TPR));
+    if (MODE == kShift && GROUPS < 8) blocks = (blocks + 7) / 8 * 8;
     branch_norm_kernel<X, Y, TPR, MODE, NV><<<static_cast<unsigned>(blocks), block_of(TPR), 0, st>>>(p);
     return cudaGetLastError();
   });
@@ -172,11 +151,13 @@ cudaError_t by_mode(const BranchParams& p, cudaStream_t st) {
 
 // ---- dropout alone -------------------------------------------------------------------------------------------------
 
-// Two groups of eight values a thread, so that both loads are on their way.
+// U groups of eight values a thread: their loads are on their way together, and they share the generator's keys.
+constexpr int kDropGroups = 4;
 template <class T, bool WIDE>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T* __restrict__ out, int64_t n, const DropParams drop) {
-  constexpr int U = 2;
+  constexpr int U = kDropGroups;
   const uint64_t seed = drop_seed(drop);
+  const uint32_t least = drop_least(drop);
   const int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 * U + threadIdx.x;
   Raw<T, 8> r[U];
 #pragma unroll
@@ -200,10 +181,10 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int64_t at = (i0 + u * 256) * 8;
+    const uint4 words = drop_words(drop, seed, static_cast<uint64_t>(at) >> 3);
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = raw_at(r[u], e);
-    drop8(drop, seed, static_cast<uint64_t>(at) >> 3, v);
+    for (int e = 0; e < 8; ++e) v[e] = drop_keeps(words, least, e) ? raw_at(r[u], e) * drop.factor : 0.f;
     if (WIDE && at + 8 <= n) {
       store_vals(out + at, v);
     } else {
@@ -218,7 +199,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T
 
 template <class T>
 cudaError_t dropout_by(const void* x, void* out, int64_t n, bool wide, const DropParams& drop, cudaStream_t st) {
-  const int64_t blocks = (n + 4095) / 4096;
+  const int64_t blocks = (n + 256 * 8 * kDropGroups - 1) / (256 * 8 * kDropGroups);
   if (blocks > INT32_MAX) return cudaErrorInvalidValue;
   if (wide)
     dropout_kernel<T, true><<<static_cast<unsigned>(blocks), 256, 0, st>>>(static_cast<const T*>(x), static_cast<T*>(out), n, drop);

@@ -8,19 +8,20 @@ namespace {
 __device__ __forceinline__ float value_at(const void* p, bool is_bf16, int64_t i) {
   return is_bf16 ? __bfloat162float(static_cast<const bf16*>(p)[i]) : static_cast<const float*>(p)[i];
 }
-__device__ __forceinline__ void put(void* p, bool is_bf16, int64_t i, float v) {
+__device__ __forceinline__ void put_at(void* p, bool is_bf16, int64_t i, float v) {
   if (is_bf16)
     static_cast<bf16*>(p)[i] = __float2bfloat16_rn(v);
   else
     static_cast<float*>(p)[i] = v;
 }
 
-// A block takes 32 columns. blockIdx.y 0: the slices' partials of u, gate by gate (as many gates at once as leave each a
-// power of two of the 32 warps), to d_gate and, over the gates, to d_post_weight; 1: the blocks' partials of d_weight.
+// A block takes 8 columns, a warp four rows of partials at a time. blockIdx.y 0: the slices' partials of u, gate by gate (as
+// many gates at once as leave each a power of two of the 32 warps), to d_gate and, over the gates, to d_post_weight; 1: the
+// blocks' partials of d_weight.
 __global__ void __launch_bounds__(1024) branch_bwd_finish_kernel(const BranchBwdParams p) {
-  __shared__ float red[32][33];
+  __shared__ float red[32][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int j = blockIdx.x * 32 + lane, d = p.d;
+  const int j = blockIdx.x * 8 + (lane & 7), d = p.d;
   const bool in = j < d;
   const bool for_u = blockIdx.y == 0 && p.part_u != nullptr;
   const float* part = for_u ? p.part_u : p.part_w;
@@ -36,29 +37,31 @@ __global__ void __launch_bounds__(1024) branch_bwd_finish_kernel(const BranchBwd
     float t = 0.f;
     if (in && g < gates) {
 #pragma unroll 8
-      for (int r = sub; r < rows; r += per) t += part[(static_cast<int64_t>(g) * rows + r) * d + j];
+      for (int r = 4 * sub + (lane >> 3); r < rows; r += 4 * per) t += part[(static_cast<int64_t>(g) * rows + r) * d + j];
     }
+    t += __shfl_xor_sync(0xffffffffu, t, 8);
+    t += __shfl_xor_sync(0xffffffffu, t, 16);
     if (per > 1) {
-      red[warp][lane] = t;
+      if (lane < 8) red[warp][lane] = t;
       __syncthreads();
-      if (sub == 0)
+      if (sub == 0 && lane < 8)
         for (int q = 1; q < per; ++q) t += red[warp + q][lane];
       __syncthreads();
     }
-    if (sub == 0 && in && g < gates) {
+    if (sub == 0 && lane < 8 && in && g < gates) {
       const int64_t at = static_cast<int64_t>(g) * d + j;
-      if (gated && p.d_gate != nullptr) put(p.d_gate, p.gate_bf16, at, t * pw);
+      if (gated && p.d_gate != nullptr) put_at(p.d_gate, p.gate_bf16, at, t * pw);
       total += gated ? t * value_at(p.gate, p.gate_bf16, at) : t;
     }
   }
-  red[warp][lane] = total;  // 0 where sub > 0
+  if (lane < 8) red[warp][lane] = total;  // 0 where sub > 0
   __syncthreads();
-  if (warp == 0 && in) {
+  if (warp == 0 && lane < 8 && in) {
     for (int q = 1; q < 32; ++q) total += red[q][lane];
     if (for_u) {
-      if (p.d_post != nullptr) put(p.d_post, p.post_bf16, j, total);
+      if (p.d_post != nullptr) put_at(p.d_post, p.post_bf16, j, total);
     } else {
-      put(p.d_weight, p.weight_bf16, j, total);
+      put_at(p.d_weight, p.weight_bf16, j, total);
     }
   }
 }
@@ -67,9 +70,9 @@ __global__ void __launch_bounds__(1024) branch_bwd_finish_kernel(const BranchBwd
 
 void branch_bwd_shape(int64_t rows, int d, int gates, int sms, bool wide, int* slices, int* blocks) {
   const int mode = wide ? kWide : kShift;
-  branch_bwd_width(room_of(mode, d), [&](auto tpr) {
+  branch_bwd_width(room_of(mode, d), [&](auto tpr, auto nv) {
     constexpr int TPR = decltype(tpr)::value, GROUPS = block_of(TPR) / TPR;
-    const int resident = sms * branch_bwd_resident(TPR);
+    const int resident = sms * branch_bwd_resident(TPR, decltype(nv)::value);
     const int64_t most = (rows / gates + GROUPS - 1) / GROUPS;  // slices of a gate with a row each
     int64_t s = std::max<int64_t>(1, std::min<int64_t>(most, (resident + gates - 1) / gates));
     // kShift: the rows of a group start off alike, eight (or a multiple) apart, unless it has one row.
@@ -88,7 +91,7 @@ cudaError_t launch_branch_bwd_f32(const BranchBwdParams& p, cudaStream_t st) {
 cudaError_t launch_branch_bwd_finish(const BranchBwdParams& p, cudaStream_t st) {
   const int sums = (p.part_u != nullptr ? 1 : 0) + (p.part_w != nullptr ? 1 : 0);
   if (sums == 0) return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>((p.d + 31) / 32), static_cast<unsigned>(sums));
+  const dim3 grid(static_cast<unsigned>((p.d + 7) / 8), static_cast<unsigned>(sums));
   branch_bwd_finish_kernel<<<grid, 1024, 0, st>>>(p);
   return cudaGetLastError();
 }

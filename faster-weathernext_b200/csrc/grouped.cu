@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <cstdint>
 
 #define g_device_error g_grouped_device_error
@@ -115,33 +116,42 @@ __global__ void __launch_bounds__(128) grouped_rows_kernel(const bf16* __restric
                                                            int groups, const LinearParams p) {
   constexpr int V = WIDE ? 8 : 1;
   const int lane = threadIdx.x & 31, col = blockIdx.x * 4 + (threadIdx.x >> 5);
-  // The run's expert and rows: expert g takes the rows that offsets[g + 1] is the first to exceed.
-  int run = -1, before = -2, g = -1, r0 = 0, r1 = 0;
+  // The expert of each row: row r is expert g's where offsets[g + 1] is the first to exceed r (-1: a row of none).
   const int m = static_cast<int>(p.m);
-  for (int r = 0; r < m; ++r) {
-    int mine = -1;
-    for (int i0 = 0; i0 <= groups; i0 += 32) {
-      const unsigned over = __ballot_sync(0xffffffffu, i0 + lane <= groups && __ldg(given + min(i0 + lane, groups)) > r);
-      if (over) {
-        mine = i0 + __ffs(over) - 2;  // -1: a row before the first expert's
-        break;
+  int of[M];
+#pragma unroll
+  for (int r = 0; r < M; ++r) of[r] = -1;
+  unsigned found = 0;
+  bool wrong = false;
+  int last = 0;
+  for (int i0 = 0; i0 <= groups; i0 += 32) {
+    const bool in = i0 + lane <= groups;
+    const int v = in ? __ldg(given + i0 + lane) : INT_MAX;
+    const int before = __shfl_up_sync(0xffffffffu, v, 1);
+    wrong |= in && (v < 0 || v > m || v < (lane > 0 ? before : last));
+    last = __shfl_sync(0xffffffffu, v, 31);
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+      const unsigned over = __ballot_sync(0xffffffffu, in && v > r);
+      if (over != 0 && !(found >> r & 1)) {
+        found |= 1u << r;
+        of[r] = i0 + __ffs(over) - 2;
       }
     }
-    if (mine != before) ++run;
-    before = mine;
-    if (run == static_cast<int>(blockIdx.y)) {
-      if (r1 == 0) r0 = r;
-      r1 = r + 1;
-      g = mine;
-    }
   }
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 32) {
-    int high = 0;
-    for (int i = lane; i <= groups; i += 32) {
-      const int v = __ldg(given + i);
-      if (v < 0 || v > m || (i > 0 && v < __ldg(given + i - 1))) high = 1;
+  if (wrong && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 32) atomicOr(&g_device_error, 0x400u);
+  // The block's run of rows of one expert.
+  int run = -1, g = -1, r0 = 0, r1 = 0;
+#pragma unroll
+  for (int r = 0; r < M; ++r) {
+    if (r < m) {
+      if (r == 0 || of[r] != of[r > 0 ? r - 1 : 0]) ++run;
+      if (run == static_cast<int>(blockIdx.y)) {
+        if (r1 == 0) r0 = r;
+        r1 = r + 1;
+        g = of[r];
+      }
     }
-    if (high) atomicOr(&g_device_error, 0x400u);
   }
   if (r1 == 0 || col >= p.n) return;  // whole warps
   float acc[M];
@@ -149,7 +159,7 @@ __global__ void __launch_bounds__(128) grouped_rows_kernel(const bf16* __restric
   for (int r = 0; r < M; ++r) acc[r] = 0.f;
   if (g >= 0) {
     const bf16* brow = b + g * b_stride + col * ldb;
-#pragma unroll 4
+#pragma unroll 8
     for (int at = lane * V; at < p.k; at += 32 * V) {
       auto load = [](const bf16* src, float (&v)[V]) {
         if constexpr (WIDE) {
@@ -280,26 +290,26 @@ __global__ void __launch_bounds__(256) grouped_cast_kernel(const void* __restric
   }
 }
 
-// A block takes 32 columns of an expert, its 32 warps every 32nd row of partials; their sums are added in order.
-__global__ void __launch_bounds__(1024) grouped_column_sum_kernel(const float* __restrict__ part, const int32_t* __restrict__ first,
-                                                                  int per, int n, void* __restrict__ out, bool out_bf16) {
-  __shared__ float red[32][33];
+// A block takes 32 columns of an expert, its warps every W-th row of partials; their sums are added in order. Many experts
+// have few rows each: 8 warps a block (64 experts of 81,924 rows x 2,048: 33 us with 32).
+template <int W>
+__global__ void __launch_bounds__(32 * W) grouped_column_sum_kernel(const float* __restrict__ part, const int32_t* __restrict__ first,
+                                                                    int per, int n, void* __restrict__ out, bool out_bf16) {
+  __shared__ float red[W][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.y;
   const int j = blockIdx.x * 32 + lane;
   const int64_t r0 = static_cast<int64_t>(__ldg(first + g)) * per, r1 = static_cast<int64_t>(__ldg(first + g + 1)) * per;
   float t = 0.f;
   if (j < n) {
 #pragma unroll 8
-    for (int64_t r = r0 + warp; r < r1; r += 32) t += part[r * n + j];
+    for (int64_t r = r0 + warp; r < r1; r += W) t += part[r * n + j];
   }
   red[warp][lane] = t;
   __syncthreads();
-  t = red[lane][warp];  // column `warp` of the block, the sums of its warps across the lanes
+  if (warp == 0 && j < n) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-  const int c = blockIdx.x * 32 + warp;
-  if (lane == 0 && c < n) {
-    const int64_t at = static_cast<int64_t>(g) * n + c;
+    for (int w = 1; w < W; ++w) t += red[w][lane];
+    const int64_t at = static_cast<int64_t>(g) * n + j;
     if (out_bf16)
       static_cast<bf16*>(out)[at] = __float2bfloat16_rn(t);
     else
@@ -370,7 +380,10 @@ cudaError_t launch_grouped_cast(const void* x, bool x_f32, int64_t ldx, int n, v
 cudaError_t launch_grouped_column_sum(const float* part, const int32_t* first, int groups, int per, int n, void* out,
                                       bool out_bf16, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>((n + 31) / 32), static_cast<unsigned>(groups));
-  grouped_column_sum_kernel<<<grid, 1024, 0, st>>>(part, first, per, n, out, out_bf16);
+  if (groups >= 16)
+    grouped_column_sum_kernel<8><<<grid, 256, 0, st>>>(part, first, per, n, out, out_bf16);
+  else
+    grouped_column_sum_kernel<32><<<grid, 1024, 0, st>>>(part, first, per, n, out, out_bf16);
   return cudaGetLastError();
 }
 

@@ -82,7 +82,9 @@ __device__ __forceinline__ void tile_store3(const void* tmap, int c0, int c1, in
                ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(src)
                : "memory");
 }
-// A tensor map that an earlier kernel wrote: before this thread's first copy through it.
+// A tensor map that an earlier kernel wrote, before a block's first copy through it. Once for all, at the kernel's start: with
+// a fence by every warp that met the next expert's map, each change of expert took 3 to 12 us (163,848 x 512 x 2,048, 8 experts
+// act'() 334 us, 64 760; one expert 249).
 __device__ __forceinline__ void map_acquire(const void* tmap) {
   asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(reinterpret_cast<uint64_t>(tmap)) : "memory");
 }
@@ -484,6 +486,14 @@ __device__ __forceinline__ void linear_tile_body(const CUtensorMap& tm_a, const 
     if (GROUP != kGroupRows && !p.out_direct) tma_prefetch_desc(&tm_o);
     if (GROUP == kGroupNone && p.x != nullptr && !p.x_direct) tma_prefetch_desc(&tm_x);
   }
+  if constexpr (GROUP != kGroupNone) {
+    for (int g = threadIdx.x; g < gp.groups; g += C::THREADS) {
+      map_acquire(gp.map_a + g);
+      if (GROUP == kGroupK) map_acquire(gp.map_b + g);
+      if (GROUP == kGroupRows && !p.out_direct) map_acquire(gp.map_o + g);
+      if (GROUP == kGroupRows && p.x != nullptr && !p.x_direct) map_acquire(gp.map_x + g);
+    }
+  }
   if (warp == 1) tmem_alloc_cg<CG>(smem_u32(tmem_holder), C::TMEM_COLS);
   tc_fence_before();
   __syncwarp();
@@ -503,16 +513,11 @@ __device__ __forceinline__ void linear_tile_body(const CUtensorMap& tm_a, const 
     const int base = is_a ? rank * 128 : rank * C::BNC, boxes = is_a ? 2 : C::BNC / 64;
     uint32_t g = 0;
     bool ok = true;
-    int group = -1;
     for (Walk w(p, gp, first); w.in(p) && ok; w.next(p, gp, step)) {
       int at = (is_a ? w.mt * 128 * CG : w.nt * C::BN) + base;
       if constexpr (GROUP != kGroupNone) {
         if (GROUP == kGroupRows && is_a) at = w.row0 + base;
-        if ((GROUP == kGroupK || is_a) && w.g != group) {
-          group = w.g;
-          tm = (is_a ? gp.map_a : gp.map_b) + group;
-          map_acquire(tm);
-        }
+        if (GROUP == kGroupK || is_a) tm = (is_a ? gp.map_a : gp.map_b) + w.g;
       }
       const int kb1 = w.kb1(p);
       for (int kb = w.kb0(p); kb < kb1; ++kb, ++g) {
@@ -629,14 +634,9 @@ __device__ __forceinline__ void linear_tile_body(const CUtensorMap& tm_a, const 
       if constexpr (GROUP == kGroupRows) return w.end;
       return p.m;
     };
-    int x_group = -1, o_group = -1;  // experts whose maps this thread has acquired
     auto issue_x = [&](const Walk& w, int ch) {  // the residual (dy) of chunk ch of a tile into the slot
       const CUtensorMap* tm = &tm_x;
-      if constexpr (GROUP == kGroupRows) {
-        tm = gp.map_x + w.g;
-        if (w.g != x_group) map_acquire(tm);
-        x_group = w.g;
-      }
+      if constexpr (GROUP == kGroupRows) tm = gp.map_x + w.g;
       mbar_arrive_expect_tx(x_bar(ew), 32 * C::X_ROW);
       tile_load<1>(slot, tm, w.nt * C::BN + part * C::HC + ch * CC, static_cast<int>(row_of(w)), x_bar(ew));
     };
@@ -930,8 +930,6 @@ __device__ __forceinline__ void linear_tile_body(const CUtensorMap& tm_a, const 
             if constexpr (GROUP == kGroupNone) {
               if (row0 < p.m && col < p.n) tile_store(&tm_o, col, static_cast<int>(row0 + w.sp * p.split_rows), slot);
             } else if constexpr (GROUP == kGroupRows) {
-              if (w.g != o_group) map_acquire(gp.map_o + w.g);
-              o_group = w.g;
               if (row0 < end && col < p.n) tile_store(gp.map_o + w.g, col, static_cast<int>(row0), slot);
             } else {
               if (row0 < end && col < p.n) tile_store3(&tm_o, col, static_cast<int>(row0), gp.by_run ? w.at : w.g, slot);

@@ -44,15 +44,16 @@ __device__ __forceinline__ uint4 philox(uint64_t counter, uint32_t site, uint64_
 
 __device__ __forceinline__ uint64_t drop_seed(const DropParams& p) { return p.seed_at != nullptr ? __ldg(p.seed_at) : p.seed; }
 
-// Eight values, the first of which has an index of 8 i8 in its tensor: dropped ones become 0 whatever they were.
-__device__ __forceinline__ void drop8(const DropParams& p, uint64_t seed, uint64_t i8, float (&v)[8]) {
-  const uint4 q = philox(i8, p.site, seed);
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = (w[i] & 0xFFFFu) >= p.threshold ? v[2 * i] * p.factor : 0.f;
-    v[2 * i + 1] = (w[i] >> 16) >= p.threshold ? v[2 * i + 1] * p.factor : 0.f;
-  }
+// The words of the eight values from index 8 i8 of their tensor, and whether value E of them is kept: `least` is the
+// threshold in the upper half of a word. All are dropped at a threshold of 65,536, which `least` cannot hold: drop_words
+// then gives zeros, below a `least` of all ones.
+__device__ __forceinline__ uint32_t drop_least(const DropParams& p) { return p.threshold < 65536u ? p.threshold << 16 : 0xFFFFFFFFu; }
+__device__ __forceinline__ uint4 drop_words(const DropParams& p, uint64_t seed, uint64_t i8) {
+  return p.threshold < 65536u ? philox(i8, p.site, seed) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ bool drop_keeps(const uint4& q, uint32_t least, int e) {
+  const uint32_t w = e < 2 ? q.x : e < 4 ? q.y : e < 6 ? q.z : q.w;
+  return (e & 1 ? w : w << 16) >= least;  // the upper half decides: least's lower one is 0 (or both are all ones)
 }
 
 }  // namespace fwn

@@ -126,23 +126,24 @@ __device__ void place(const RouteParams& p, int64_t first, const int* base, int*
 
 // Exclusive prefixes of total [n] (n <= 1,023) by a block of 256 threads, with the sum behind them: out [n + 1].
 __device__ void prefixes(const int* total, int n, int* out) {
-  __shared__ int sums[256];
-  const int t = threadIdx.x;
+  __shared__ int sums[8];
+  const int t = threadIdx.x, lane = t & 31;
   int v[4], s = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[i] = 4 * t + i < n ? total[4 * t + i] : 0;
     s += v[i];
   }
-  sums[t] = s;
-  __syncthreads();
-  for (int o = 1; o < 256; o <<= 1) {
-    const int u = t >= o ? sums[t - o] : 0;
-    __syncthreads();
-    sums[t] += u;
-    __syncthreads();
+  int upto = s;  // of the warp's threads so far
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += u;
   }
-  int at = sums[t] - s;
+  if (lane == 31) sums[t >> 5] = upto;
+  __syncthreads();
+  int at = upto - s;
+  for (int w = 0; w < t >> 5; ++w) at += sums[w];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (4 * t + i <= n) out[4 * t + i] = at;

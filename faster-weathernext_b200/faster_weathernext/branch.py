@@ -94,15 +94,14 @@ def dropout(x, p, seed, *, site=0):
 
 def _gate_rows(gate, x):
   """(gate as rows [gates, d], rows of x for each): gate [d], of x's shape, or with one row for all of x's last rows."""
-  d, shape = x.shape[-1], tuple(gate.shape)
-  rows = x.numel() // d
-  if shape == (d,):
-    return gate, rows
-  if shape == tuple(x.shape):
+  shape, xs = gate.shape, x.shape
+  if shape == xs[-1:]:
+    return gate, x.numel() // xs[-1]
+  if shape == xs:
     return gate, 1
-  if x.dim() >= 2 and shape in (tuple(x.shape[:-2]) + (d,), tuple(x.shape[:-2]) + (1, d)):
-    return gate, x.shape[-2]
-  raise ValueError(f"gate has shape {shape}, expected ({d},), x's {tuple(x.shape)} or one row for each {tuple(x.shape[:-2])}")
+  if len(xs) >= 2 and (shape == xs[:-2] + xs[-1:] or shape == xs[:-2] + (1,) + xs[-1:]):
+    return gate, xs[-2]
+  raise ValueError(f"gate has shape {tuple(shape)}, expected ({xs[-1]},), x's {tuple(xs)} or one row for each {tuple(xs[:-2])}")
 
 
 def _starts(t):
@@ -117,32 +116,46 @@ def _plain(t):
   return t.clone(memory_format=torch.contiguous_format)
 
 
-def _wide_or_plain(d, *tensors):
-  """The tensors as rows [rows, d]: as they are where every row of each allows wide accesses, else contiguous."""
-  out = [_rows(t) for t in tensors]
-  if d % 8 == 0 and all(_starts(t) and (t.stride(0) % 8 == 0 or t.shape[0] == 1) for t in out):
-    return out
-  return [_plain(t) for t in out]
+def _wide_or_plain(d, x, y):
+  """(x, its row stride, y, its row stride): as they are where they are contiguous, or where every row of both allows wide
+  accesses; else contiguous copies."""
+  if x.is_contiguous() and y.is_contiguous() and _starts(x) and _starts(y):
+    return x, d, y, d
+  x2, y2 = _rows(x), _rows(y)
+  if d % 8 == 0 and all(_starts(t) and (t.stride(0) % 8 == 0 or t.shape[0] == 1) for t in (x2, y2)):
+    return x2, max(x2.stride(0), d), y2, max(y2.stride(0), d)
+  return _plain(x2), d, _plain(y2), d
 
 
-def _branch_desc(x, y, pw, w, gate, span, out_dtype, eps, scale, drop):
-  rows, d = x.shape
-  return _lib.BranchDesc(rows, x.stride(0), y.stride(0), span, d, _CODE[x.dtype], _CODE[y.dtype],
-                         0 if pw is None else _CODE[pw.dtype], 0 if w is None else _CODE[w.dtype],
-                         0 if gate is None else _CODE[gate.dtype], _CODE[out_dtype], eps, scale, 0, drop)
+# Descriptors by their fields, of calls without dropout: a call's own time counts for single rows, and filling one takes 4 us.
+_DESCS = {}
+
+
+def _branch_desc(x, xs, y, ys, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site):
+  d = x.shape[-1]
+  fields = (x.numel() // d, xs, ys, span, d, _CODE[x.dtype], _CODE[y.dtype], 0 if pw is None else _CODE[pw.dtype],
+            0 if w is None else _CODE[w.dtype], 0 if gate is None else _CODE[gate.dtype], _CODE[out_dtype], eps, scale, 0)
+  if threshold:
+    return _lib.BranchDesc(*fields, _drop_desc(threshold, seed, site))
+  desc = _DESCS.get(fields)
+  if desc is None:
+    if len(_DESCS) >= 4096:
+      _DESCS.clear()
+    desc = _DESCS[fields] = _lib.BranchDesc(*fields)
+  return desc
 
 
 def _ptr(t):
   return None if t is None else t.data_ptr()
 
 
-def _branch_launch(stream, x, y, pw, w, gate, span, out_dtype, eps, scale, drop, keep_rstd):
-  rows, d = x.shape
-  s = x.new_empty((rows, d))
-  h = x.new_empty((rows, d), dtype=out_dtype)
-  h_scale = x.new_empty((rows,), dtype=_F32) if out_dtype is _E4M3 else None
-  rstd = x.new_empty((rows, 2), dtype=_F32) if keep_rstd else None
-  desc = _branch_desc(x, y, pw, w, gate, span, out_dtype, eps, scale, drop)
+def _branch_launch(stream, x, xs, y, ys, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site, keep_rstd, shape):
+  """(h, its scales or None, s, both roots of each row or None), h and s of x's shape."""
+  s = x.new_empty(shape)
+  h = x.new_empty(shape, dtype=out_dtype)
+  h_scale = x.new_empty(shape[:-1], dtype=_F32) if out_dtype is _E4M3 else None
+  rstd = x.new_empty((*shape[:-1], 2), dtype=_F32) if keep_rstd else None
+  desc = _branch_desc(x, xs, y, ys, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site)
   status = _lib.lib().fwn_branch_norm(desc, x.data_ptr(), y.data_ptr(), _ptr(pw), _ptr(w), _ptr(gate), s.data_ptr(),
                                       h.data_ptr(), _ptr(h_scale), _ptr(rstd), stream)
   if status:
@@ -150,10 +163,9 @@ def _branch_launch(stream, x, y, pw, w, gate, span, out_dtype, eps, scale, drop,
   return h, h_scale, s, rstd
 
 
-def _branch_forward(x, y, pw, w, gate, span, out_dtype, eps, scale, drop, keep_rstd=False):
-  x2, y2 = _wide_or_plain(x.shape[-1], x, y)
-  return _on_device(x, _branch_launch, x2, y2, _plain(pw), _plain(w), _plain(gate), span, out_dtype, eps, scale, drop,
-                    keep_rstd)
+def _branch_forward(x, y, pw, w, gate, span, out_dtype, eps, scale, threshold=0, seed=None, site=0, keep_rstd=False):
+  return _on_device(x, _branch_launch, *_wide_or_plain(x.shape[-1], x, y), _plain(pw), _plain(w), _plain(gate), span, out_dtype,
+                    eps, scale, threshold, seed, site, keep_rstd, x.shape)
 
 
 class _BranchNorm(torch.autograd.Function):
@@ -164,10 +176,10 @@ class _BranchNorm(torch.autograd.Function):
   def forward(ctx, x, y, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site):
     ctx.args = span, out_dtype, eps, scale, threshold, site
     ctx.seed = None if isinstance(seed, torch.Tensor) else seed
-    h, _, s, rstd = _branch_forward(x, y, pw, w, gate, span, out_dtype, eps, scale, _drop_desc(threshold, seed, site), True)
+    h, _, s, rstd = _branch_forward(x, y, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site, True)
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(x, y, pw, w, gate, rstd, seed if isinstance(seed, torch.Tensor) else None)
-    return h.view(x.shape), s.view(x.shape)
+    return h, s
 
   @staticmethod
   def backward(ctx, dh, ds):
@@ -184,27 +196,21 @@ class _BranchNorm(torch.autograd.Function):
     span, out_dtype, eps, scale, threshold, site = ctx.args
     need = ctx.needs_input_grad
     d = x.shape[-1]
-    x2, y2 = _wide_or_plain(d, x, y)
+    x2, xs, y2, ys = _wide_or_plain(d, x, y)
     pw2, w2, gate2, dh, ds = _plain(pw), _plain(w), _plain(gate), _plain(dh), _plain(ds)
     new = lambda t, wanted: torch.empty_like(t, memory_format=torch.contiguous_format) if wanted else None  # noqa: E731
     dx, dy, dpw, dw = new(x, need[0]), new(y, need[1]), new(pw, need[2]), new(w, need[3])
     dgate = new(gate, need[4])
-    desc = _branch_desc(x2, y2, pw, w, gate, span, out_dtype, eps, scale, _drop_desc(threshold, seed, site))
+    desc = _branch_desc(x2, xs, y2, ys, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site)
     lib = _lib.lib()
-    ws, size = _branch_workspace(x, desc, lib)
+    ws, size = _workspace(x, _branch_desc(x2, xs, y2, ys, pw, w, gate, span, out_dtype, 0.0, 0.0, 0, None, 0),
+                          lib.fwn_branch_norm_bwd_workspace_size)  # it goes by the shape alone
     status = lib.fwn_branch_norm_bwd(desc, x2.data_ptr(), y2.data_ptr(), _ptr(pw2), _ptr(w2), _ptr(gate2), rstd.data_ptr(),
                                      _ptr(dh), _ptr(ds), _ptr(dx), _ptr(dy), _ptr(dpw), _ptr(dw), _ptr(dgate), _ptr(ws), size,
                                      stream)
     if status:
       _lib.check(status)
     return dx, dy, dpw, dw, dgate
-
-
-def _branch_workspace(x, desc, lib):
-  """The backward's workspace: its size goes by the shape alone, not by the call's seed or scales."""
-  shape = _lib.BranchDesc(desc.rows, desc.x_stride, desc.y_stride, desc.gate_span, desc.d, desc.x_dtype, desc.y_dtype,
-                          desc.post_dtype, desc.weight_dtype, desc.gate_dtype, desc.out_dtype)
-  return _workspace(x, shape, lib.fwn_branch_norm_bwd_workspace_size)
 
 
 def _branch_check(x, y, pw, w, gate, residual_scale, eps):
@@ -254,9 +260,8 @@ def branch_norm(x, y, post_weight=None, weight=None, *, gate=None, residual_scal
   _no_tangent("branch_norm", x, y, post_weight, weight, gate)
   if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, post_weight, weight, gate)):
     return _BranchNorm.apply(x, y, post_weight, weight, gate, span, out_dtype, eps, residual_scale, threshold, seed, site)
-  h, _, s, _ = _branch_forward(x, y, post_weight, weight, gate, span, out_dtype, eps, residual_scale,
-                               _drop_desc(threshold, seed, site))
-  return (h, s) if x.dim() == 2 else (h.view(x.shape), s.view(x.shape))
+  h, _, s, _ = _branch_forward(x, y, post_weight, weight, gate, span, out_dtype, eps, residual_scale, threshold, seed, site)
+  return h, s
 
 
 def branch_norm_fp8(x, y, post_weight=None, weight=None, *, gate=None, residual_scale=1.0, eps=1e-6):
@@ -265,5 +270,4 @@ def branch_norm_fp8(x, y, post_weight=None, weight=None, *, gate=None, residual_
   values 0. No dropout and no gradient (forecasts): inputs that require one raise NotImplementedError."""
   gate, span = _branch_check(x, y, post_weight, weight, gate, residual_scale, eps)
   _constant("branch_norm_fp8", x, y, post_weight, weight, gate)
-  h, scale, s, _ = _branch_forward(x, y, post_weight, weight, gate, span, _E4M3, eps, residual_scale, _drop_desc(0, None, 0))
-  return h.view(x.shape), scale.view(x.shape[:-1]), s.view(x.shape)
+  return _branch_forward(x, y, post_weight, weight, gate, span, _E4M3, eps, residual_scale)[:3]

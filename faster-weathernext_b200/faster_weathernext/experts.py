@@ -13,7 +13,7 @@ include/fwn_attn.h, fwn_linear_grouped* and fwn_route*). Every call runs on the 
 takes its workspace from torch's allocator.
 """
 
-import dataclasses
+import typing
 
 import torch
 
@@ -179,8 +179,7 @@ def linear_grouped(a, weight, offsets, bias=None, *, activation=None, out_dtype=
 
 # ---- routing ---------------------------------------------------------------------------------------------------------
 
-@dataclasses.dataclass(frozen=True)
-class Routing:
+class Routing(typing.NamedTuple):
   """Where rows go: experts [rows, top_k] int32 (largest logit first) and weights [rows, top_k] float32 (differentiable);
   position [rows, top_k] int32, the place of each pair (row, choice) in the experts' order; order [rows * top_k] int32, the
   pair (row * top_k + choice) in each place; offsets [experts + 1] int32, the first place of each expert."""
@@ -193,9 +192,9 @@ class Routing:
 
 def _route_launch(stream, logits, top_k):
   rows, e = logits.shape
-  new = lambda shape, dtype=torch.int32: logits.new_empty(shape, dtype=dtype)  # noqa: E731
-  chosen, weights, position = new((rows, top_k)), new((rows, top_k), _F32), new((rows, top_k))
-  order, offsets = new((rows * top_k,)), new((e + 1,))
+  chosen, position, order = logits.new_empty((3, rows, top_k), dtype=torch.int32).unbind()
+  order = order.view(rows * top_k)
+  weights, offsets = logits.new_empty((rows, top_k), dtype=_F32), logits.new_empty((e + 1,), dtype=torch.int32)
   desc = _lib.RouteDesc(rows, e, top_k, _CODE[logits.dtype], 0)
   lib = _lib.lib()
   ws, size = _workspace(logits, desc, lib.fwn_route_workspace_size)

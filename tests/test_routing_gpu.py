@@ -153,13 +153,12 @@ def test_nan_rows_stay_apart(cuda):
 
 
 def test_positions_outside_are_reported(cuda):
-  import dataclasses
   from faster_weathernext import _lib, experts
   rand = _randn(9)
   r = experts.route(rand(20, 4), 2)
   bad = r.position.clone()
   bad[3, 1], bad[4, 0] = 40, -1
-  wrong = dataclasses.replace(r, position=bad)
+  wrong = r._replace(position=bad)
   x = rand(20, 64)
   out = experts.combine(rand(40, 64), wrong)
   assert out.shape == (20, 64) and _lib.device_error() == _lib.FWN_ERR_INVALID_ARGUMENT
@@ -190,7 +189,6 @@ def test_graph_and_repeats(cuda):
 
 
 def test_refusals(cuda):
-  import dataclasses
   from faster_weathernext import experts
   rand = _randn(11)
   logits, x = rand(10, 4), rand(10, 8)
@@ -198,12 +196,12 @@ def test_refusals(cuda):
   for bad in (lambda: experts.route(logits, 0), lambda: experts.route(logits, 5), lambda: experts.route(logits, 2.0),
               lambda: experts.route(logits[0], 1), lambda: experts.route(logits[:, :0], 1), lambda: experts.dispatch(x[:9], r),
               lambda: experts.combine(x, r), lambda: experts.dispatch(x[:, :0], r), lambda: experts.dispatch(x[0], r),
-              lambda: experts.combine(rand(20, 8), dataclasses.replace(r, weights=r.weights[:5])),
-              lambda: experts.dispatch(x, dataclasses.replace(r, position=r.position.cpu()))):
+              lambda: experts.combine(rand(20, 8), r._replace(weights=r.weights[:5])),
+              lambda: experts.dispatch(x, r._replace(position=r.position.cpu()))):
     with pytest.raises(ValueError):
       bad()
   for bad in (lambda: experts.route(logits.double(), 2), lambda: experts.dispatch(x.half(), r),
-              lambda: experts.dispatch(x, dataclasses.replace(r, position=r.position.long()))):
+              lambda: experts.dispatch(x, r._replace(position=r.position.long()))):
     with pytest.raises(TypeError):
       bad()
   for bad in (lambda: experts.route(rand(4, 1024), 2), lambda: experts.route(rand(4, 40), 17)):
