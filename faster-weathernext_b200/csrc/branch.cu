@@ -14,29 +14,43 @@ namespace fwn {
 
 namespace {
 
-// Threads of a row and groups of eight values a thread: sixteen values, so that a thread has some 100 bytes on their way.
+// Threads of a row, groups of eight values a thread, and the block's most threads: up to 768 values a warp or less (16 or 24
+// values a thread, some 100 bytes on their way), above them a block of as many warps as the row needs (20,481 x 4,096 at eight
+// values a thread, one block of 16 warps an SM: 202 us, at sixteen 159).
 template <class F>
 cudaError_t branch_width(int room, F f) {
   using std::integral_constant;
-#define FWN_ROW(TPR, NV) \
-  if (room <= TPR * NV * 8) return f(integral_constant<int, TPR>(), integral_constant<int, NV>())
-  FWN_ROW(8, 1);
-  FWN_ROW(8, 2);
-  FWN_ROW(16, 2);
-  FWN_ROW(32, 2);
-  FWN_ROW(64, 2);
-  FWN_ROW(128, 2);
-  FWN_ROW(256, 2);
-  FWN_ROW(512, 2);
+#define FWN_ROW(TPR, NV, MAXT) \
+  if (room <= (TPR > 0 ? TPR : MAXT) * NV * 8) return f(integral_constant<int, TPR>(), integral_constant<int, NV>(), integral_constant<int, MAXT>())
+  FWN_ROW(8, 1, 256);
+  FWN_ROW(8, 2, 256);
+  FWN_ROW(8, 3, 256);
+  FWN_ROW(16, 2, 256);
+  FWN_ROW(16, 3, 256);
+  FWN_ROW(32, 2, 256);
+  FWN_ROW(32, 3, 256);
+  FWN_ROW(0, 1, 128);
+  FWN_ROW(0, 1, 256);
+  FWN_ROW(0, 2, 256);
+  FWN_ROW(0, 2, 512);
 #undef FWN_ROW
   return cudaErrorInvalidValue;
 }
-constexpr int branch_resident(int tpr) { return 512 / block_of(tpr); }
+// Threads of an SM: 255 registers a thread at 24 values, 80 at 8 values of a block's rows, 128 elsewhere.
+constexpr int branch_resident(int tpr, int nv) { return nv == 3 ? 256 : tpr == 0 && nv == 1 ? 768 : 512; }
 
-template <class X, class Y, int TPR, int MODE, int NV>
-__global__ void __launch_bounds__(block_of(TPR), branch_resident(TPR)) branch_norm_kernel(const BranchParams p) {
-  __shared__ float red[3][1][32];
-  Rows<TPR> at;
+template <class X, class Y, int TPR, int MODE, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT, (branch_resident(TPR, NV) / MAXT)) branch_norm_kernel(const BranchParams p) {
+  __shared__ __align__(16) float red[3][32];
+  clear_red<TPR>(red);
+  // Groups of one warp have adjacent rows and leave together (`base`, the row of the warp's first group, decides).
+  struct {
+    int64_t row, base, step;
+  } at;
+  const int group = TPR > 0 ? threadIdx.x / (TPR > 0 ? TPR : 1) : 0;
+  at.row = static_cast<int64_t>(blockIdx.x) * groups_of<TPR>() + group;
+  at.base = at.row - group % per_warp<TPR>();
+  at.step = static_cast<int64_t>(gridDim.x) * groups_of<TPR>();
   const int off = MODE == kShift ? static_cast<int>(at.row * p.d & 7) : 0;  // of all this group's rows
   const int d = p.d;
   const float over = 1.f / static_cast<float>(d);
@@ -52,7 +66,7 @@ __global__ void __launch_bounds__(block_of(TPR), branch_resident(TPR)) branch_no
     const bool more = (p.rows - 1 - row) * d >= 7;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, 8>(i, off);
+      const int j = column_of<TPR>(i, off);
       load_group<MODE>(static_cast<const Y*>(p.y) + row * p.y_stride, j, n, more, yr[i]);
       load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, more, xr[i]);
     }
@@ -62,14 +76,14 @@ __global__ void __launch_bounds__(block_of(TPR), branch_resident(TPR)) branch_no
   auto columns_of = [&](int64_t gate) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, 8>(i, off);
+      const int j = column_of<TPR>(i, off);
       g[i] = mul(columns<MODE>(p.post_weight, p.post_bf16, j, d), factor);
       if (p.gate != nullptr && !own_gate) g[i] = mul(g[i], columns<MODE>(gate_row(p.gate, p.gate_bf16, gate, d), p.gate_bf16, j, d));
     }
   };
   int gate = -1;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) w[i] = columns<MODE>(p.weight, p.weight_bf16, group_at<TPR, 8>(i, off), d);
+  for (int i = 0; i < NV; ++i) w[i] = columns<MODE>(p.weight, p.weight_bf16, column_of<TPR>(i, off), d);
   if (one_gate || own_gate) columns_of(0);
   const uint64_t seed = drops ? drop_seed(p.drop) : 0;
   for (; at.base < p.rows; at.base += at.step, at.row += at.step) {
@@ -83,19 +97,17 @@ __global__ void __launch_bounds__(block_of(TPR), branch_resident(TPR)) branch_no
     float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, 8>(i, off);
+      const int j = column_of<TPR>(i, off);
       s[i] = values<MODE>(yr[i], j, n);
       x[i] = mul(values<MODE>(xr[i], j, n), p.alpha);
       dot(acc, s[i], s[i]);
     }
     if (at.base + at.step < p.rows) fetch(row + at.step);
-    float sum[1] = {acc.x + acc.y};
-    row_reduce<TPR, false>(sum, red[0]);
-    const float r1 = rsqrtf(sum[0] * over + p.eps);
+    const float r1 = rsqrtf(over_row<TPR, false>(acc.x + acc.y, red[0]) * over + p.eps);
     acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, 8>(i, off);
+      const int j = column_of<TPR>(i, off);
       s[i] = mul(mul(s[i], r1), g[i]);
       if (own_gate) s[i] = mul(s[i], gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, (p.rows - 1 - row) * d >= 7));
       if (drops) s[i] = kept(s[i], drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3), least);
@@ -104,43 +116,44 @@ __global__ void __launch_bounds__(block_of(TPR), branch_resident(TPR)) branch_no
       put<MODE>(static_cast<X*>(p.s) + row * d, j, n, s[i]);
       dot(acc, s[i], s[i]);
     }
-    sum[0] = acc.x + acc.y;
-    row_reduce<TPR, false>(sum, red[1]);
-    const float r2 = rsqrtf(sum[0] * over + p.eps);
-    if (p.rstd != nullptr && (threadIdx.x & (TPR - 1)) == 0 && n > 0)
+    const float r2 = rsqrtf(over_row<TPR, false>(acc.x + acc.y, red[1]) * over + p.eps);
+    if (p.rstd != nullptr && row_first<TPR>() && n > 0)
       reinterpret_cast<float2*>(p.rstd)[row] = make_float2(r1, r2);
 #pragma unroll
     for (int i = 0; i < NV; ++i) s[i] = mul(mul(s[i], r2), w[i]);
     if (p.out_type == kRmsE4m3) {
-      float most[1] = {0.f};
+      float most = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most[0] = max_nan(most[0], fabsf(at8(s[i], e)));
-      row_reduce<TPR, true>(most, red[2]);
-      const bool tiny = most[0] < kTinyRow;  // false for NaN, which the scale and the values keep
-      const float inv = tiny ? 0.f : kE4m3Max / most[0];
-      if ((threadIdx.x & (TPR - 1)) == 0 && n > 0) p.scale[row] = tiny ? 0.f : most[0] / kE4m3Max;
+        for (int e = 0; e < 8; ++e) most = max_nan(most, fabsf(at8(s[i], e)));
+      most = over_row<TPR, true>(most, red[2]);
+      const bool tiny = most < kTinyRow;  // false for NaN, which the scale and the values keep
+      const float inv = tiny ? 0.f : kE4m3Max / most;
+      if (row_first<TPR>() && n > 0) p.scale[row] = tiny ? 0.f : most / kE4m3Max;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<e4m3_t*>(p.h) + row * d, group_at<TPR, 8>(i, off), n, mul(s[i], inv));
+      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<e4m3_t*>(p.h) + row * d, column_of<TPR>(i, off), n, mul(s[i], inv));
     } else if (p.out_type == kRmsBf16) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<bf16*>(p.h) + row * d, group_at<TPR, 8>(i, off), n, s[i]);
+      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<bf16*>(p.h) + row * d, column_of<TPR>(i, off), n, s[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<float*>(p.h) + row * d, group_at<TPR, 8>(i, off), n, s[i]);
+      for (int i = 0; i < NV; ++i) put<MODE>(static_cast<float*>(p.h) + row * d, column_of<TPR>(i, off), n, s[i]);
     }
   }
 }
 
 template <class X, class Y, int MODE>
 cudaError_t go(const BranchParams& p, cudaStream_t st) {
-  return branch_width(room_of(MODE, p.d), [&](auto tpr, auto nv) {
-    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, GROUPS = block_of(TPR) / TPR;
+  const int room = room_of(MODE, p.d);
+  return branch_width(room, [&](auto tpr, auto nv, auto maxt) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, MAXT = decltype(maxt)::value, GROUPS = groups_of<TPR>();
+    const int threads = TPR > 0 ? MAXT : (room + 256 * NV - 1) / (256 * NV) * 32;
     // Resident blocks walk the rows (kShift: a multiple of eight rows at a step).
-    int64_t blocks = std::min<int64_t>((p.rows + GROUPS - 1) / GROUPS, static_cast<int64_t>(p.sms) * branch_resident(TPR));
+    const int64_t resident = static_cast<int64_t>(p.sms) * (branch_resident(TPR, NV) / threads);
+    int64_t blocks = std::min<int64_t>((p.rows + GROUPS - 1) / GROUPS, resident);
     if (MODE == kShift && GROUPS < 8) blocks = (blocks + 7) / 8 * 8;
-    branch_norm_kernel<X, Y, TPR, MODE, NV><<<static_cast<unsigned>(blocks), block_of(TPR), 0, st>>>(p);
+    branch_norm_kernel<X, Y, TPR, MODE, NV, MAXT><<<static_cast<unsigned>(blocks), threads, 0, st>>>(p);
     return cudaGetLastError();
   });
 }

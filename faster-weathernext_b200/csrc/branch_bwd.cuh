@@ -18,51 +18,48 @@ namespace fwn {
 
 namespace {
 
-// Threads of a row and groups of eight values a thread.
+// Threads of a row, eight values each: up to 256 values a warp or less, above them a block of as many warps as the row needs
+// (of MAXT threads at most). Sixteen values a thread took as long at 512 (236 us) and longer with dropout (262 against 244):
+// eight warps a SM left the exchanges between.
 template <class F>
 cudaError_t branch_bwd_width(int room, F f) {
   using std::integral_constant;
-#define FWN_ROW(TPR, NV) \
-  if (room <= TPR * NV * 8) return f(integral_constant<int, TPR>(), integral_constant<int, NV>())
-  FWN_ROW(8, 1);
-  FWN_ROW(16, 1);
-  FWN_ROW(32, 1);
-  FWN_ROW(64, 1);
-  FWN_ROW(128, 1);
-  FWN_ROW(256, 1);
-  FWN_ROW(512, 1);
-  FWN_ROW(1024, 1);
+#define FWN_ROW(TPR, MAXT) \
+  if (room <= (TPR > 0 ? TPR : MAXT) * 8) return f(integral_constant<int, TPR>(), integral_constant<int, MAXT>())
+  FWN_ROW(8, 256);
+  FWN_ROW(16, 256);
+  FWN_ROW(32, 256);
+  FWN_ROW(0, 128);
+  FWN_ROW(0, 256);
+  FWN_ROW(0, 512);
+  FWN_ROW(0, 1024);
 #undef FWN_ROW
   return cudaErrorInvalidValue;
 }
-constexpr int branch_bwd_resident(int tpr, int nv) { return tpr > 512 ? 1 : (nv > 1 ? 256 : 512) / block_of(tpr); }
+constexpr int branch_bwd_resident(int maxt) { return maxt > 512 ? maxt : 512; }  // threads of an SM
+__host__ __device__ constexpr int branch_bwd_threads(int tpr, int maxt, int room) { return tpr > 0 ? maxt : (room + 255) / 256 * 32; }
 
-template <class X, class Y, class G, int TPR, int NV, int MODE>
-__global__ void __launch_bounds__(block_of(TPR), (branch_bwd_resident(TPR, NV))) branch_bwd_kernel(const BranchBwdParams p) {
-  constexpr int GROUPS = block_of(TPR) / TPR, PER_WARP = TPR < 32 ? 32 / TPR : 1;
+template <class X, class Y, class G, int TPR, int MAXT, int MODE>
+__global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch_bwd_kernel(const BranchBwdParams p) {
+  constexpr int GROUPS = groups_of<TPR>(), PER_WARP = per_warp<TPR>();
   extern __shared__ float part_smem[];  // more than one group: a row of d each
-  __shared__ float red[2][1][32];
-  const int d = p.d, group = threadIdx.x / TPR;
+  __shared__ __align__(16) float red[2][32];
+  clear_red<TPR>(red);
+  const int d = p.d, group = TPR > 0 ? threadIdx.x / (TPR > 0 ? TPR : 1) : 0;
   const float over = 1.f / static_cast<float>(d);
   const bool drops = p.drop.threshold > 0, own_gate = p.gate_values;
   const uint32_t least = drop_least(p.drop);
   const float factor = drops ? p.drop.factor : 1.f;
   const uint64_t seed = drops ? drop_seed(p.drop) : 0;
   const int64_t span = p.gates > 1 ? p.gate_span : p.rows, step = static_cast<int64_t>(p.slices) * GROUPS;
-  V8 dw[NV], w[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) dw[i] = all8(0.f);
-  int off = 0;
+  V8 dw = all8(0.f);
+  int j = column_of<TPR>(0, 0);
   // A block's row of partials: its groups' sums, added in order.
-  auto leave = [&](const V8 (&v)[NV], float scale, float* to) {
+  auto leave = [&](const V8& v, float scale, float* to) {
     float* mine = GROUPS > 1 ? part_smem + group * d : to;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, 8>(i, off);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (j + e >= 0 && j + e < d) mine[j + e] = at8(v[i], e) * scale;
-    }
+    for (int e = 0; e < 8; ++e)
+      if (j + e >= 0 && j + e < d) mine[j + e] = at8(v, e) * scale;
     if constexpr (GROUPS > 1) {
       __syncthreads();
       for (int c = threadIdx.x; c < d; c += blockDim.x) {
@@ -78,94 +75,66 @@ __global__ void __launch_bounds__(block_of(TPR), (branch_bwd_resident(TPR, NV)))
     const int gate = item / p.slices, slice = item % p.slices;
     const int64_t end = (gate + 1) * span;
     int64_t row = gate * span + static_cast<int64_t>(slice) * GROUPS + group;
-    if (MODE == kShift) off = static_cast<int>(row * d & 7);  // of all the item's rows; a block takes one item
-    V8 a[NV], u[NV];  // post_weight gate factor, sums of db yhat (without the factor)
-    Raw<X, 8> nx[NV], nds[NV];
-    Raw<Y, 8> ny[NV];
-    Raw<G, 8> ng[NV];
+    if (MODE == kShift) j = column_of<TPR>(0, static_cast<int>(row * d & 7));  // of all the item's rows; a block takes one item
+    Raw<X, 8> nx, nds;
+    Raw<Y, 8> ny;
+    Raw<G, 8> ng;
     float2 nr;
     auto fetch = [&](int64_t r) {
       const int n = r < end ? d : 0;
       const bool more = (p.rows - 1 - r) * d >= 7;
       nr = n > 0 ? __ldg(reinterpret_cast<const float2*>(p.rstd) + r) : make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = group_at<TPR, 8>(i, off);
-        load_group<MODE>(static_cast<const X*>(p.x) + r * p.x_stride, j, n, more, nx[i]);
-        load_group<MODE>(static_cast<const Y*>(p.y) + r * p.y_stride, j, n, more, ny[i]);
-        load_group<MODE>(static_cast<const G*>(p.dh) + r * d, j, p.dh != nullptr ? n : 0, more && p.dh != nullptr, ng[i]);
-        load_group<MODE>(static_cast<const X*>(p.ds) + r * d, j, p.ds != nullptr ? n : 0, more && p.ds != nullptr, nds[i]);
-      }
+      load_group<MODE>(static_cast<const X*>(p.x) + r * p.x_stride, j, n, more, nx);
+      load_group<MODE>(static_cast<const Y*>(p.y) + r * p.y_stride, j, n, more, ny);
+      load_group<MODE>(static_cast<const G*>(p.dh) + r * d, j, p.dh != nullptr ? n : 0, more && p.dh != nullptr, ng);
+      load_group<MODE>(static_cast<const X*>(p.ds) + r * d, j, p.ds != nullptr ? n : 0, more && p.ds != nullptr, nds);
     };
     fetch(row);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = group_at<TPR, 8>(i, off);
-      w[i] = columns<MODE>(p.weight, p.weight_bf16, j, d);
-      a[i] = mul(columns<MODE>(p.post_weight, p.post_bf16, j, d), factor);
-      if (p.gate != nullptr && !own_gate) a[i] = mul(a[i], columns<MODE>(gate_row(p.gate, p.gate_bf16, gate, d), p.gate_bf16, j, d));
-      u[i] = all8(0.f);
-    }
+    const V8 w = columns<MODE>(p.weight, p.weight_bf16, j, d);
+    V8 a = mul(columns<MODE>(p.post_weight, p.post_bf16, j, d), factor);  // post_weight gate factor
+    if (p.gate != nullptr && !own_gate) a = mul(a, columns<MODE>(gate_row(p.gate, p.gate_bf16, gate, d), p.gate_bf16, j, d));
+    V8 u = all8(0.f);  // sums of db yhat, without the factor
     for (; row - group % PER_WARP < end; row += step) {
       const int n = row < end ? d : 0;
       const bool more = (p.rows - 1 - row) * d >= 7;
       const float r1 = nr.x, r2 = nr.y;
-      V8 yh[NV], sh[NV], g[NV], dt[NV];
-      uint4 words[NV];
-      float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = group_at<TPR, 8>(i, off);
-        yh[i] = mul(values<MODE>(ny[i], j, n), r1);
-        V8 b = mul(yh[i], a[i]);
-        if (own_gate) b = mul(b, gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, more));
-        if (drops) {
-          words[i] = drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3);
-          b = kept(b, words[i], least);
-        }
-        sh[i] = mul(fma(values<MODE>(nx[i], j, n), p.alpha, b), r2);
-        g[i] = values<MODE>(ng[i], j, n);
-        dw[i] = fma(g[i], sh[i], dw[i]);
-        g[i] = mul(g[i], w[i]);
-        dot(acc, g[i], sh[i]);
-        dt[i] = values<MODE>(nds[i], j, n);
+      const V8 yh = mul(values<MODE>(ny, j, n), r1);
+      V8 b = mul(yh, a);
+      if (own_gate) b = mul(b, gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, more));
+      uint4 words;
+      if (drops) {
+        words = drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3);
+        b = kept(b, words, least);
       }
+      const V8 sh = mul(fma(values<MODE>(nx, j, n), p.alpha, b), r2);
+      V8 g = values<MODE>(ng, j, n), dt = values<MODE>(nds, j, n);
       if (row + step - group % PER_WARP < end) fetch(row + step);
-      float sum[1] = {acc.x + acc.y};
-      row_reduce<TPR, false>(sum, red[0]);
-      const float c1 = -sum[0] * over;
-      acc = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = group_at<TPR, 8>(i, off);
-        dt[i] = fma(fma(sh[i], c1, g[i]), r2, dt[i]);
-        if (p.dx != nullptr) put<MODE>(static_cast<X*>(p.dx) + row * d, j, n, mul(dt[i], p.alpha));
-        if (drops) dt[i] = kept(dt[i], words[i], least);
-        g[i] = mul(dt[i], a[i]);
-        if (own_gate) {
-          // The gate's own gradient (a is post_weight here), and the gate goes into the other two.
-          const V8 gv = gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, more);
-          const V8 dg = mul(g[i], yh[i]);
-          if (p.d_gate != nullptr) {
-            if (p.gate_bf16)
-              put<MODE>(static_cast<bf16*>(p.d_gate) + row * d, j, n, dg);
-            else
-              put<MODE>(static_cast<float*>(p.d_gate) + row * d, j, n, dg);
-          }
-          g[i] = mul(g[i], gv);
-          dt[i] = mul(dt[i], gv);
+      dw = fma(g, sh, dw);
+      g = mul(g, w);
+      float2 acc = make_float2(0.f, 0.f);
+      dot(acc, g, sh);
+      const float c1 = -over_row<TPR, false>(acc.x + acc.y, red[0]) * over;
+      dt = fma(fma(sh, c1, g), r2, dt);
+      if (p.dx != nullptr) put<MODE>(static_cast<X*>(p.dx) + row * d, j, n, mul(dt, p.alpha));
+      if (drops) dt = kept(dt, words, least);
+      g = mul(dt, a);
+      if (own_gate) {
+        // The gate's own gradient (a is post_weight here), and the gate goes into the other two.
+        const V8 gv = gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, more), dg = mul(g, yh);
+        if (p.d_gate != nullptr) {
+          if (p.gate_bf16)
+            put<MODE>(static_cast<bf16*>(p.d_gate) + row * d, j, n, dg);
+          else
+            put<MODE>(static_cast<float*>(p.d_gate) + row * d, j, n, dg);
         }
-        u[i] = fma(dt[i], yh[i], u[i]);
-        dot(acc, g[i], yh[i]);
+        g = mul(g, gv);
+        dt = mul(dt, gv);
       }
-      sum[0] = acc.x + acc.y;
-      row_reduce<TPR, false>(sum, red[1]);
-      const float c2 = -sum[0] * over;
-      if (p.dy != nullptr) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          put<MODE>(static_cast<Y*>(p.dy) + row * d, group_at<TPR, 8>(i, off), n, mul(fma(yh[i], c2, g[i]), r1));
-      }
+      u = fma(dt, yh, u);
+      acc = make_float2(0.f, 0.f);
+      dot(acc, g, yh);
+      const float c2 = -over_row<TPR, false>(acc.x + acc.y, red[1]) * over;
+      if (p.dy != nullptr) put<MODE>(static_cast<Y*>(p.dy) + row * d, j, n, mul(fma(yh, c2, g), r1));
     }
     if (p.part_u != nullptr) leave(u, factor, p.part_u + static_cast<int64_t>(item) * d);
   }
@@ -174,10 +143,11 @@ __global__ void __launch_bounds__(block_of(TPR), (branch_bwd_resident(TPR, NV)))
 
 template <class X, class Y, class G, int MODE>
 cudaError_t go_branch_bwd(const BranchBwdParams& p, cudaStream_t st) {
-  return branch_bwd_width(room_of(MODE, p.d), [&](auto tpr, auto nv) {
-    constexpr int TPR = decltype(tpr)::value;
-    const size_t smem = block_of(TPR) > TPR ? block_of(TPR) / TPR * sizeof(float) * static_cast<size_t>(p.d) : 0;
-    branch_bwd_kernel<X, Y, G, TPR, decltype(nv)::value, MODE><<<p.blocks, block_of(TPR), smem, st>>>(p);
+  const int room = room_of(MODE, p.d);
+  return branch_bwd_width(room, [&](auto tpr, auto maxt) {
+    constexpr int TPR = decltype(tpr)::value, MAXT = decltype(maxt)::value, GROUPS = groups_of<TPR>();
+    const size_t smem = GROUPS > 1 ? GROUPS * sizeof(float) * static_cast<size_t>(p.d) : 0;
+    branch_bwd_kernel<X, Y, G, TPR, MAXT, MODE><<<p.blocks, branch_bwd_threads(TPR, MAXT, room), smem, st>>>(p);
     return cudaGetLastError();
   });
 }

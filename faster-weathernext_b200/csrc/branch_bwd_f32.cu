@@ -70,9 +70,10 @@ __global__ void __launch_bounds__(1024) branch_bwd_finish_kernel(const BranchBwd
 
 void branch_bwd_shape(int64_t rows, int d, int gates, int sms, bool wide, int* slices, int* blocks) {
   const int mode = wide ? kWide : kShift;
-  branch_bwd_width(room_of(mode, d), [&](auto tpr, auto nv) {
-    constexpr int TPR = decltype(tpr)::value, GROUPS = block_of(TPR) / TPR;
-    const int resident = sms * branch_bwd_resident(TPR, decltype(nv)::value);
+  const int room = room_of(mode, d);
+  branch_bwd_width(room, [&](auto tpr, auto maxt) {
+    constexpr int TPR = decltype(tpr)::value, MAXT = decltype(maxt)::value, GROUPS = groups_of<TPR>();
+    const int resident = sms * (branch_bwd_resident(MAXT) / branch_bwd_threads(TPR, MAXT, room));
     const int64_t most = (rows / gates + GROUPS - 1) / GROUPS;  // slices of a gate with a row each
     int64_t s = std::max<int64_t>(1, std::min<int64_t>(most, (resident + gates - 1) / gates));
     // kShift: the rows of a group start off alike, eight (or a multiple) apart, unless it has one row.

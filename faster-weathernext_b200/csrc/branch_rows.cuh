@@ -9,6 +9,49 @@ namespace fwn {
 
 namespace {
 
+// How a row lies over threads. TPR > 0: a power of two of a warp's threads, several rows a block of 256. TPR = 0: the whole
+// block, of as many warps as the row needs (MAXT at most), so that few threads idle at any width.
+template <int TPR>
+__device__ __forceinline__ int column_of(int i, int off) {
+  return (TPR > 0 ? i * TPR + static_cast<int>(threadIdx.x & (TPR - 1)) : i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8 - off;
+}
+template <int TPR>
+constexpr int groups_of() { return TPR > 0 ? 256 / TPR : 1; }
+template <int TPR>
+constexpr int per_warp() { return TPR > 0 && TPR < 32 ? 32 / TPR : 1; }
+template <int TPR>
+__device__ __forceinline__ bool row_first() { return TPR > 0 ? (threadIdx.x & (TPR - 1)) == 0 : threadIdx.x == 0; }
+
+// The sum (or NaN-keeping maximum, of values that are not negative) over a row's threads, the same in each. `red`: 32 zeros
+// at first, one value per warp, read back whole; a reduction's red is free again after the next one's barrier.
+template <int TPR, bool MAX>
+__device__ __forceinline__ float over_row(float v, float* red) {
+#pragma unroll
+  for (int o = (TPR > 0 ? TPR : 32) / 2; o > 0; o >>= 1) {
+    const float u = __shfl_xor_sync(0xffffffffu, v, o);
+    v = MAX ? max_nan(v, u) : v + u;
+  }
+  if constexpr (TPR == 0) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float4 t = reinterpret_cast<const float4*>(red)[0];
+    for (int w = 4; w < static_cast<int>(blockDim.x >> 5); w += 4) {
+      const float4 u = reinterpret_cast<const float4*>(red)[w >> 2];
+      t = MAX ? make_float4(max_nan(t.x, u.x), max_nan(t.y, u.y), max_nan(t.z, u.z), max_nan(t.w, u.w))
+              : make_float4(t.x + u.x, t.y + u.y, t.z + u.z, t.w + u.w);
+    }
+    v = MAX ? max_nan(max_nan(t.x, t.y), max_nan(t.z, t.w)) : (t.x + t.y) + (t.z + t.w);
+  }
+  return v;
+}
+template <int TPR, int N>
+__device__ __forceinline__ void clear_red(float (&red)[N][32]) {
+  if constexpr (TPR == 0) {
+    for (int i = threadIdx.x; i < N * 32; i += blockDim.x) red[i / 32][i % 32] = 0.f;
+    __syncthreads();
+  }
+}
+
 struct V8 {
   float2 p[4];
 };
@@ -45,14 +88,18 @@ __device__ __forceinline__ void dot(float2& acc, const V8& a, const V8& b) {
   for (int i = 0; i < 4; ++i) acc = ffma2(a.p[i], b.p[i], acc);
 }
 
-// The values of a group as loaded; columns outside [0, d) are 0.
+// The values of a group as loaded; columns outside [0, d), which a group at the row's ends brings, are 0.
 template <int MODE, class T>
 __device__ __forceinline__ V8 values(const Raw<T, 8>& r, int j, int d) {
   V8 v;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float x = raw_at(r, e);
-    set8(v, e, MODE != kShift || (j + e >= 0 && j + e < d) ? x : 0.f);
+  for (int e = 0; e < 8; ++e) set8(v, e, raw_at(r, e));
+  if constexpr (MODE == kShift) {
+    if (j < 0 || j + 8 > d) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j + e < 0 || j + e >= d) set8(v, e, 0.f);
+    }
   }
   return v;
 }

@@ -48,36 +48,39 @@ constexpr int kClearBlocks = 64;
 __global__ void __launch_bounds__(1024) group_setup_kernel(const GroupSetup s, const __grid_constant__ GroupMaps maps, int map_blocks) {
   const int t = threadIdx.x, warp = t >> 5;
   if (blockIdx.x == 0) {
-    __shared__ int buf[2][1024];
-    // Largest offset so far, then numbers of tiles before: scans over the 1,024 threads.
-    auto scan = [&](int v, bool most) {
-      int at = 0;
-      buf[0][t] = v;
-      __syncthreads();
-      for (int o = 1; o < 1024; o <<= 1, at ^= 1) {
-        const int u = t >= o ? buf[at][t - o] : 0;
-        const int w = buf[at][t];
-        buf[at ^ 1][t] = most ? max(w, u) : w + u;
-        __syncthreads();
+    __shared__ int warps[2][32], ends[1024];
+    const int lane = t & 31;
+    // Largest offset so far, then numbers of tiles before: scans over the 1,024 threads (`flip`: two scans' own warps[]).
+    auto scan = [&](int v, bool most, int flip) {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v = most ? max(v, u) : v + u;
       }
-      v = buf[at][t];
+      if (lane == 31) warps[flip][warp] = v;
       __syncthreads();
-      return v;
+      int before = lane < warp ? warps[flip][lane] : 0;  // offsets and numbers are not negative
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const int u = __shfl_xor_sync(0xffffffffu, before, o);
+        before = most ? max(before, u) : before + u;
+      }
+      return most ? max(v, before) : v + before;
     };
     const int given = t <= s.groups ? __ldg(s.given + t) : 0;
-    const int mine = scan(clamped(given, s.m), true);
+    const int mine = scan(clamped(given, s.m), true, 0);
     if (t <= s.groups) {
       s.offsets[t] = mine;
       if (mine != given) atomicOr(&g_device_error, 0x400u);  // out of order or of the tensor
     }
-    buf[0][t] = mine;
+    ends[t] = mine;
     __syncthreads();
-    const int rows = t < s.groups ? buf[0][t + 1] - mine : 0;
-    __syncthreads();
+    const int rows = t < s.groups ? ends[t + 1] - mine : 0;
+#pragma unroll
     for (int q = 0; q < kGroupFirsts; ++q) {
       if (s.first[q] == nullptr) continue;
       const int tiles = t < s.groups ? (s.unit[q] > 0 ? (rows + s.unit[q] - 1) / s.unit[q] : 1) : 0;
-      const int upto = scan(tiles, false);
+      const int upto = scan(tiles, false, (q + 1) & 1);
       if (t < s.groups) s.first[q][t] = upto - tiles;
       if (t == s.groups) s.first[q][t] = upto;  // tiles is 0 here
     }

@@ -33,7 +33,9 @@ template <class T, int LPR, int NV>
 __device__ void choose(const RouteParams& p, int64_t first, int* hist) {
   const int lane = threadIdx.x & (LPR - 1), per = blockDim.x / LPR;
   const T* logits = static_cast<const T*>(p.logits);
-  for (int r = threadIdx.x / LPR; r < kRouteRows; r += per) {
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kRouteRows), p.rows - first));
+  // Whole warps go on while the first of their rows is there.
+  for (int r = threadIdx.x / LPR; r - static_cast<int>(threadIdx.x & 31) / LPR < rows; r += per) {
     const int64_t row = first + r;
     const bool in = row < p.rows;
     unsigned long long keys[NV];

@@ -70,7 +70,9 @@ class _Dropout(torch.autograd.Function):
   def backward(ctx, dy):
     seed = ctx.saved_tensors[0] if ctx.seed is None else ctx.seed
     _no_tangent("dropout's gradient", dy)
-    return _Dropout.apply(dy, ctx.threshold, seed, ctx.site), None, None, None
+    if torch.is_grad_enabled():  # a graph of the gradient is kept
+      return _Dropout.apply(dy, ctx.threshold, seed, ctx.site), None, None, None
+    return _on_device(dy, _dropout_launch, dy.contiguous(), ctx.threshold, seed, ctx.site), None, None, None
 
 
 def dropout(x, p, seed, *, site=0):
@@ -173,8 +175,8 @@ class _BranchNorm(torch.autograd.Function):
   rounded stream) and the two reciprocal roots of each row, and makes the mask again."""
 
   @staticmethod
-  def forward(ctx, x, y, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site):
-    ctx.args = span, out_dtype, eps, scale, threshold, site
+  def forward(ctx, x, y, pw, w, gate, seed, args):
+    span, out_dtype, eps, scale, threshold, site = ctx.args = args
     ctx.seed = None if isinstance(seed, torch.Tensor) else seed
     h, _, s, rstd = _branch_forward(x, y, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site, True)
     ctx.set_materialize_grads(False)
@@ -186,10 +188,10 @@ class _BranchNorm(torch.autograd.Function):
     x, y, pw, w, gate, rstd, seed = ctx.saved_tensors
     _no_tangent("branch_norm's gradient", x, y, pw, w, gate, dh, ds)
     if dh is None and ds is None:
-      return (None,) * 12
+      return (None,) * 7
     _first_order("branch_norm")
     grads = _on_device(x, _BranchNorm._launch, ctx, x, y, pw, w, gate, rstd, ctx.seed if seed is None else seed, dh, ds)
-    return (*grads, None, None, None, None, None, None, None)
+    return (*grads, None, None)
 
   @staticmethod
   def _launch(stream, ctx, x, y, pw, w, gate, rstd, seed, dh, ds):
@@ -198,9 +200,9 @@ class _BranchNorm(torch.autograd.Function):
     d = x.shape[-1]
     x2, xs, y2, ys = _wide_or_plain(d, x, y)
     pw2, w2, gate2, dh, ds = _plain(pw), _plain(w), _plain(gate), _plain(dh), _plain(ds)
-    new = lambda t, wanted: torch.empty_like(t, memory_format=torch.contiguous_format) if wanted else None  # noqa: E731
-    dx, dy, dpw, dw = new(x, need[0]), new(y, need[1]), new(pw, need[2]), new(w, need[3])
-    dgate = new(gate, need[4])
+    dx, dy, dpw, dw, dgate = [t.new_empty(t.shape) if wanted else None for t, wanted in zip((x, y, pw, w, gate), need)]
+    if need[4] and x.numel() == 0:
+      dgate.zero_()
     desc = _branch_desc(x2, xs, y2, ys, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site)
     lib = _lib.lib()
     ws, size = _workspace(x, _branch_desc(x2, xs, y2, ys, pw, w, gate, span, out_dtype, 0.0, 0.0, 0, None, 0),
@@ -259,7 +261,7 @@ def branch_norm(x, y, post_weight=None, weight=None, *, gate=None, residual_scal
     seed = None
   _no_tangent("branch_norm", x, y, post_weight, weight, gate)
   if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, post_weight, weight, gate)):
-    return _BranchNorm.apply(x, y, post_weight, weight, gate, span, out_dtype, eps, residual_scale, threshold, seed, site)
+    return _BranchNorm.apply(x, y, post_weight, weight, gate, seed, (span, out_dtype, eps, residual_scale, threshold, site))
   h, _, s, _ = _branch_forward(x, y, post_weight, weight, gate, span, out_dtype, eps, residual_scale, threshold, seed, site)
   return h, s
 

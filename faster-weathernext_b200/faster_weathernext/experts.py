@@ -251,9 +251,18 @@ def route(logits, top_k):
   return Routing(*_on_device(logits, _route_launch, _rows(logits), top_k))
 
 
+_MOVES = {}  # descriptors of the rows' ways
+
+
 def _move_desc(t, position):
-  rows, top_k = position.shape
-  return _lib.RouteDesc(rows, top_k, top_k, _CODE[t.dtype], 0)  # the number of experts does not matter here
+  key = (position.shape, t.dtype)
+  desc = _MOVES.get(key)
+  if desc is None:
+    if len(_MOVES) >= 4096:
+      _MOVES.clear()
+    rows, top_k = position.shape
+    desc = _MOVES[key] = _lib.RouteDesc(rows, top_k, top_k, _CODE[t.dtype], 0)  # the number of experts does not matter here
+  return desc
 
 
 def _spread_launch(stream, x, position, weights, y, wanted):

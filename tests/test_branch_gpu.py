@@ -173,6 +173,13 @@ CASES = [
     ((5, 4099), F32, BF16, "value", BF16, BF16, 1.0, 0.4),
     ((4, 8192), BF16, BF16, "channel", F32, BF16, 1.0, 0.1),
     ((11, 8185), F32, F32, None, F32, F32, 0.0, 0.1),
+    ((333, 192), F32, BF16, "channel", F32, BF16, 1.0, 0.1),
+    ((90, 333), BF16, F32, "channel", F32, BF16, 1.0, 0.0),
+    ((2, 70, 760), F32, BF16, "sample", BF16, F32, 1.0, 0.1),
+    ((33, 771), F32, BF16, "value", F32, BF16, 1.0, 0.1),
+    ((40, 1152), BF16, BF16, "channel", F32, BF16, 1.0, 0.2),
+    ((3, 9, 1700), F32, F32, "sample", F32, BF16, 1.0, 0.0),
+    ((21, 5000), F32, BF16, "channel", F32, BF16, 1.0, 0.1),
     ((1000, 1, 64), F32, BF16, "sample", F32, BF16, 1.0, 0.1),
     ((301, 2, 24), F32, BF16, "sample", F32, BF16, 1.0, 0.1),
     ((40, 3, 13), F32, BF16, "sample", F32, BF16, 1.0, 0.1),
@@ -352,6 +359,16 @@ def test_empty_and_partial_gradients(cuda):
   assert h.shape == (0, 64)
   gx, gw = torch.autograd.grad((h, s), (e[0], e[2]), (torch.zeros_like(h), torch.zeros_like(s)))
   assert gx.shape == (0, 64) and (gw == 0).all()
+
+
+@pytest.mark.parametrize("shape,gate", [((0, 64), (64,)), ((3, 0, 64), (3, 64)), ((0, 5, 64), (0, 64)), ((0, 64), (0, 64))])
+def test_gates_of_no_rows(cuda, shape, gate):
+  from faster_weathernext import branch
+  x, g = torch.zeros(shape, device="cuda", requires_grad=True), torch.ones(gate, device="cuda", requires_grad=True)
+  torch.full((1 << 20,), 7.0, device="cuda")  # memory that is not zero
+  h, _ = branch.branch_norm(x, torch.zeros(shape, device="cuda"), gate=g)
+  d_gate, = torch.autograd.grad(h, g, torch.zeros_like(h))
+  assert d_gate.shape == gate and (d_gate == 0).all()
 
 
 def test_gradient_against_differences(cuda):
