@@ -212,12 +212,15 @@ class _Route(torch.autograd.Function):
   def forward(ctx, logits, top_k):
     chosen, weights, position, order, offsets = _on_device(logits, _route_launch, _rows(logits), top_k)
     ctx.mark_non_differentiable(chosen, position, order, offsets)
+    ctx.set_materialize_grads(False)  # zeros for each of them, otherwise
     ctx.shape, ctx.dtype = logits.shape, logits.dtype
     ctx.save_for_backward(chosen, weights)
     return chosen, weights, position, order, offsets
 
   @staticmethod
   def backward(ctx, _chosen, d_weights, *_rest):
+    if d_weights is None:
+      return None, None
     chosen, weights = ctx.saved_tensors
     _no_tangent("route's gradient", weights, d_weights)
     _first_order("route")
