@@ -229,7 +229,7 @@ cudaError_t launch_branch(const BranchParams& p, cudaStream_t st) {
   return p.y_bf16 ? by_mode<float, bf16>(p, st) : by_mode<float, float>(p, st);
 }
 
-cudaError_t launch_dropout(const void* x, void* out, int64_t n, bool bf16_values, bool wide, int sms, const DropParams& drop,
+cudaError_t launch_dropout(const void* x, void* out, int64_t n, bool bf16_values, bool wide, const DropParams& drop,
                            cudaStream_t st) {
   if (n == 0) return cudaSuccess;
   return bf16_values ? dropout_by<bf16>(x, out, n, wide, drop, st) : dropout_by<float>(x, out, n, wide, drop, st);

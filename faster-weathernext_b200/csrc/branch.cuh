@@ -61,7 +61,7 @@ cudaError_t launch_branch_bwd_bf16(const BranchBwdParams& p, cudaStream_t stream
 cudaError_t launch_branch_bwd_finish(const BranchBwdParams& p, cudaStream_t stream);
 
 // out[i] = x[i] under the mask, i < n; x, out bf16 or float32, `wide`: both start where 8 values are one access.
-cudaError_t launch_dropout(const void* x, void* out, int64_t n, bool bf16_values, bool wide, int sms, const DropParams& drop,
+cudaError_t launch_dropout(const void* x, void* out, int64_t n, bool bf16_values, bool wide, const DropParams& drop,
                            cudaStream_t stream);
 
 }  // namespace fwn

@@ -79,7 +79,7 @@ fwn_status fwn_dropout(const fwn_dropout_desc* drop, const void* x, void* out, i
   if (n == 0) return abi_ok();
   if (!x || !out) return abi_fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
   if (fwn_status s = abi_elements({{x, abi_size(dtype)}, {out, abi_size(dtype)}}); s != FWN_OK) return s;
-  cudaError_t e = launch_dropout(x, out, n, dtype == FWN_DTYPE_BF16, starts_wide(x, dtype) && starts_wide(out, dtype), abi_sms(),
+  cudaError_t e = launch_dropout(x, out, n, dtype == FWN_DTYPE_BF16, starts_wide(x, dtype) && starts_wide(out, dtype),
                                  drop_of(*drop), static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return abi_cuda_fail(e, "dropout");
   return abi_ok();

@@ -261,14 +261,14 @@ def _pack_launch(stream, src, ld, out, rows, cols):
   return _lib.lib().fwn_linear_pack(src.data_ptr(), ld, out.data_ptr(), out.shape[1], rows, cols, _lib.DTYPE_BF16, stream)
 
 
-# Workspace bytes by a call's device (its number of SMs counts), shape, types, strides and the alignment of its operands
-# (asked once for each).
+# Workspace bytes by a call's entry point, device (its number of SMs counts), shape, types, strides and the alignment of its
+# operands (asked once for each).
 _WORKSPACE = {}
 
 
 def _workspace(like, desc, size_of, *ptrs):
   """(tensor or None, bytes) that `size_of` wants for a call with these operands."""
-  key = (like.get_device(), bytes(desc), *[p & 15 for p in ptrs])
+  key = (size_of.__name__, like.get_device(), bytes(desc), *[p & 15 for p in ptrs])
   size = _WORKSPACE.get(key)
   if size is None:
     need = ctypes.c_size_t(0)

@@ -389,7 +389,7 @@ typedef struct fwn_dropout_desc {
 } fwn_dropout_desc;
 
 /* out[i] = x[i] under the mask, n values of dtype (bf16 or float32; dropout's gradient is the same call on the output's
- * gradient). out may be x. */
+ * gradient). out does not overlap x. */
 FWN_API fwn_status fwn_dropout(const fwn_dropout_desc* drop, const void* x, void* out, int64_t n, int32_t dtype, void* stream);
 
 /* With rstd(v) = 1 / sqrt(mean(v^2) + eps) over rows of d values:
