@@ -61,17 +61,22 @@ __global__ void __launch_bounds__(MAXT, (branch_resident(TPR, NV) / MAXT)) branc
   // The next row is on its way while one is worked on; the columns' factors stay in registers.
   Raw<X, 8> xr[NV];
   Raw<Y, 8> yr[NV];
+  const int64_t whole = whole_rows(p.rows, d);
   auto fetch = [&](int64_t row) {
     const int n = row < p.rows ? d : 0;
-    const bool more = (p.rows - 1 - row) * d >= 7;
+    const X* x = static_cast<const X*>(p.x) + row * p.x_stride;
+    const Y* y = static_cast<const Y*>(p.y) + row * p.y_stride;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = column_of<TPR>(i, off);
-      load_group<MODE>(static_cast<const Y*>(p.y) + row * p.y_stride, j, n, more, yr[i]);
-      load_group<MODE>(static_cast<const X*>(p.x) + row * p.x_stride, j, n, more, xr[i]);
+      grab<MODE>(y, j, n, row < whole, yr[i]);
+      grab<MODE>(x, j, n, row < whole, xr[i]);
     }
   };
   fetch(at.row);
+  Cut<MODE> cut[NV] = {};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) cut[i] = Cut<MODE>(column_of<TPR>(i, off), d);
   V8 g[NV], w[NV];  // post_weight gate factor, weight
   auto columns_of = [&](int64_t gate) {
 #pragma unroll
@@ -97,9 +102,8 @@ __global__ void __launch_bounds__(MAXT, (branch_resident(TPR, NV) / MAXT)) branc
     float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = column_of<TPR>(i, off);
-      s[i] = values<MODE>(yr[i], j, n);
-      x[i] = mul(values<MODE>(xr[i], j, n), p.alpha);
+      s[i] = values(yr[i], cut[i]);
+      x[i] = mul(values(xr[i], cut[i]), p.alpha);
       dot(acc, s[i], s[i]);
     }
     if (at.base + at.step < p.rows) fetch(row + at.step);
@@ -109,7 +113,7 @@ __global__ void __launch_bounds__(MAXT, (branch_resident(TPR, NV) / MAXT)) branc
     for (int i = 0; i < NV; ++i) {
       const int j = column_of<TPR>(i, off);
       s[i] = mul(mul(s[i], r1), g[i]);
-      if (own_gate) s[i] = mul(s[i], gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, (p.rows - 1 - row) * d >= 7));
+      if (own_gate) s[i] = mul(s[i], gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, row < whole, cut[i]));
       if (drops) s[i] = kept(s[i], drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3), least);
 #pragma unroll
       for (int q = 0; q < 4; ++q) s[i].p[q] = fadd2(s[i].p[q], x[i].p[q]);
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(MAXT, (branch_resident(TPR, NV) / MAXT)) branc
 
 template <class X, class Y, int MODE>
 cudaError_t go(const BranchParams& p, cudaStream_t st) {
-  const int room = room_of(MODE, p.d);
+  const int room = branch_room(MODE, p.d);
   return branch_width(room, [&](auto tpr, auto nv, auto maxt) {
     constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, MAXT = decltype(maxt)::value, GROUPS = groups_of<TPR>();
     const int threads = TPR > 0 ? MAXT : (room + 256 * NV - 1) / (256 * NV) * 32;

@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
   const float factor = drops ? p.drop.factor : 1.f;
   const uint64_t seed = drops ? drop_seed(p.drop) : 0;
   const int64_t span = p.gates > 1 ? p.gate_span : p.rows, step = static_cast<int64_t>(p.slices) * GROUPS;
+  const int64_t whole = whole_rows(p.rows, d);
   V8 dw = all8(0.f);
   int j = column_of<TPR>(0, 0);
   // A block's row of partials: its groups' sums, added in order.
@@ -76,18 +77,19 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
     const int64_t end = (gate + 1) * span;
     int64_t row = gate * span + static_cast<int64_t>(slice) * GROUPS + group;
     if (MODE == kShift) j = column_of<TPR>(0, static_cast<int>(row * d & 7));  // of all the item's rows; a block takes one item
+    const Cut<MODE> cut(j, d);
     Raw<X, 8> nx, nds;
     Raw<Y, 8> ny;
     Raw<G, 8> ng;
     float2 nr;
     auto fetch = [&](int64_t r) {
-      const int n = r < end ? d : 0;
-      const bool more = (p.rows - 1 - r) * d >= 7;
+      const int n = r < end ? d : 0;  // a row that is not there adds nothing
+      const bool all = r < whole;
       nr = n > 0 ? __ldg(reinterpret_cast<const float2*>(p.rstd) + r) : make_float2(0.f, 0.f);
-      load_group<MODE>(static_cast<const X*>(p.x) + r * p.x_stride, j, n, more, nx);
-      load_group<MODE>(static_cast<const Y*>(p.y) + r * p.y_stride, j, n, more, ny);
-      load_group<MODE>(static_cast<const G*>(p.dh) + r * d, j, p.dh != nullptr ? n : 0, more && p.dh != nullptr, ng);
-      load_group<MODE>(static_cast<const X*>(p.ds) + r * d, j, p.ds != nullptr ? n : 0, more && p.ds != nullptr, nds);
+      grab<MODE>(static_cast<const X*>(p.x) + r * p.x_stride, j, n, all, nx);
+      grab<MODE>(static_cast<const Y*>(p.y) + r * p.y_stride, j, n, all, ny);
+      grab<MODE>(static_cast<const G*>(p.dh) + r * d, j, p.dh != nullptr ? n : 0, all, ng);
+      grab<MODE>(static_cast<const X*>(p.ds) + r * d, j, p.ds != nullptr ? n : 0, all, nds);
     };
     fetch(row);
     const V8 w = columns<MODE>(p.weight, p.weight_bf16, j, d);
@@ -96,18 +98,17 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
     V8 u = all8(0.f);  // sums of db yhat, without the factor
     for (; row - group % PER_WARP < end; row += step) {
       const int n = row < end ? d : 0;
-      const bool more = (p.rows - 1 - row) * d >= 7;
       const float r1 = nr.x, r2 = nr.y;
-      const V8 yh = mul(values<MODE>(ny, j, n), r1);
+      const V8 yh = mul(values(ny, cut), r1);
       V8 b = mul(yh, a);
-      if (own_gate) b = mul(b, gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, more));
+      if (own_gate) b = mul(b, gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, row < whole, cut));
       uint4 words;
       if (drops) {
         words = drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3);
         b = kept(b, words, least);
       }
-      const V8 sh = mul(fma(values<MODE>(nx, j, n), p.alpha, b), r2);
-      V8 g = values<MODE>(ng, j, n), dt = values<MODE>(nds, j, n);
+      const V8 sh = mul(fma(values(nx, cut), p.alpha, b), r2);
+      V8 g = values(ng, cut), dt = values(nds, cut);
       if (row + step - group % PER_WARP < end) fetch(row + step);
       dw = fma(g, sh, dw);
       g = mul(g, w);
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
       g = mul(dt, a);
       if (own_gate) {
         // The gate's own gradient (a is post_weight here), and the gate goes into the other two.
-        const V8 gv = gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, more), dg = mul(g, yh);
+        const V8 gv = gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, row < whole, cut), dg = mul(g, yh);
         if (p.d_gate != nullptr) {
           if (p.gate_bf16)
             put<MODE>(static_cast<bf16*>(p.d_gate) + row * d, j, n, dg);
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
 
 template <class X, class Y, class G, int MODE>
 cudaError_t go_branch_bwd(const BranchBwdParams& p, cudaStream_t st) {
-  const int room = room_of(MODE, p.d);
+  const int room = branch_room(MODE, p.d);
   return branch_bwd_width(room, [&](auto tpr, auto maxt) {
     constexpr int TPR = decltype(tpr)::value, MAXT = decltype(maxt)::value, GROUPS = groups_of<TPR>();
     const size_t smem = GROUPS > 1 ? GROUPS * sizeof(float) * static_cast<size_t>(p.d) : 0;

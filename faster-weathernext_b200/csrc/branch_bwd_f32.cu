@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(1024) branch_bwd_finish_kernel(const BranchBwd
 
 void branch_bwd_shape(int64_t rows, int d, int gates, int sms, bool wide, int* slices, int* blocks) {
   const int mode = wide ? kWide : kShift;
-  const int room = room_of(mode, d);
+  const int room = branch_room(mode, d);
   branch_bwd_width(room, [&](auto tpr, auto maxt) {
     constexpr int TPR = decltype(tpr)::value, MAXT = decltype(maxt)::value, GROUPS = groups_of<TPR>();
     const int resident = sms * (branch_bwd_resident(MAXT) / branch_bwd_threads(TPR, MAXT, room));

@@ -88,25 +88,132 @@ __device__ __forceinline__ void dot(float2& acc, const V8& a, const V8& b) {
   for (int i = 0; i < 4; ++i) acc = ffma2(a.p[i], b.p[i], acc);
 }
 
-// The values of a group as loaded; columns outside [0, d), which a group at the row's ends brings, are 0.
-template <int MODE, class T>
-__device__ __forceinline__ V8 values(const Raw<T, 8>& r, int j, int d) {
+// Which of a group's eight columns lie in [0, d), for kShift, where the groups at a row's ends are cut: bits, and masks of the
+// words of two bf16 values.
+template <int MODE>
+struct Cut {
+  uint32_t bits, words[MODE == kShift ? 4 : 1];
+  Cut() = default;
+  __device__ __forceinline__ Cut(int j, int d) : bits(j < d ? 0xFFu : 0u) {
+    if constexpr (MODE == kShift) {
+      if (j < 0) bits = 0xFFu << -j & 0xFFu;
+      if (j < d && j + 8 > d) bits &= (1u << (d - j)) - 1u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) words[i] = (bits >> (2 * i) & 1u ? 0xFFFFu : 0u) | (bits >> (2 * i + 1) & 1u ? 0xFFFF0000u : 0u);
+    }
+  }
+};
+// The values of a group as loaded; columns that are cut off, which may hold anything, are 0.
+template <int MODE>
+__device__ __forceinline__ V8 values(const Raw<bf16, 8>& r, const Cut<MODE>& cut) {
+  Raw<bf16, 8> m = r;
+  if constexpr (MODE == kShift) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m.u[i] &= cut.words[i];
+  }
+  V8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) set8(v, e, raw_at(m, e));
+  return v;
+}
+template <int MODE>
+__device__ __forceinline__ V8 values(const Raw<float, 8>& r, const Cut<MODE>& cut) {
   V8 v;
 #pragma unroll
   for (int e = 0; e < 8; ++e) set8(v, e, raw_at(r, e));
   if constexpr (MODE == kShift) {
-    if (j < 0 || j + 8 > d) {
+    if (cut.bits != 0xFFu) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (j + e < 0 || j + e >= d) set8(v, e, 0.f);
+      for (int e = 0; e < 8; ++e) set8(v, e, cut.bits >> e & 1u ? at8(v, e) : 0.f);
     }
   }
   return v;
 }
+// The group from column j of the row of n values at p (0: a row that is not there): a wide access, and single values only at
+// the tensor's end, where it would reach past it (not `whole`). What is not loaded is 0.
 template <int MODE, class T>
-__device__ __forceinline__ void put(T* p, int j, int d, const V8& v) {
+__device__ __forceinline__ void grab(const T* p, int j, int n, bool whole, Raw<T, 8>& r) {
+  if constexpr (MODE == kWide) {
+    load_group<MODE>(p, j, n, true, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(r.u) / 4); ++i) r.u[i] = 0;
+    const bool wide = whole || j + 8 <= n;
+    if (j < n && wide) load_raw(p + j, r);
+    if (j < n && !wide) load_group<MODE>(p, j, n, false, r);
+  }
+}
+// Rows before this one are followed by seven values or more.
+__device__ __forceinline__ int64_t whole_rows(int64_t rows, int d) { return rows - (d + 6) / d; }
+// Groups that kShift's rows of d values take, in values: a row starts up to 8 - gcd(d, 8) values past an aligned address.
+inline int branch_room(int mode, int d) { return mode == kShift ? d + 8 - std::min(8, d & -d) : d; }
+
+// A cut group at p + j: the columns from `lo` on (its row's first), or those before `hi` (its last), in at most three stores
+// of one, two and four values, each aligned as the whole is. Single values instead, eight of them with their conversions and
+// comparisons, took as long as the rest of a narrow row (163,848 x 250 bf16 backward 283 us).
+__device__ __forceinline__ uint32_t pick(const uint32_t (&w)[4], int i) { return i & 2 ? (i & 1 ? w[3] : w[2]) : (i & 1 ? w[1] : w[0]); }
+__device__ __forceinline__ void put_cut(float* p, const V8& v, int lo, int hi) {
+  if (lo > 0) {
+    if (lo & 1) p[lo] = lo & 4 ? (lo & 2 ? v.p[3].y : v.p[2].y) : (lo & 2 ? v.p[1].y : v.p[0].y);
+    const int q = (lo + 1) & ~1;
+    if (q & 2) *reinterpret_cast<float2*>(p + q) = q & 4 ? v.p[3] : v.p[1];
+    if (lo <= 4) *reinterpret_cast<float4*>(p + 4) = make_float4(v.p[2].x, v.p[2].y, v.p[3].x, v.p[3].y);
+  } else {
+    if (hi & 4) *reinterpret_cast<float4*>(p) = make_float4(v.p[0].x, v.p[0].y, v.p[1].x, v.p[1].y);
+    if (hi & 2) *reinterpret_cast<float2*>(p + (hi & 4)) = hi & 4 ? v.p[2] : v.p[0];
+    if (hi & 1) p[hi - 1] = hi & 4 ? (hi & 2 ? v.p[3].x : v.p[2].x) : (hi & 2 ? v.p[1].x : v.p[0].x);
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float2 v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void put_cut(bf16* out, const V8& v, int lo, int hi) {
+  const uint32_t w[4] = {pack2(v.p[0]), pack2(v.p[1]), pack2(v.p[2]), pack2(v.p[3])};
+  uint16_t* p = reinterpret_cast<uint16_t*>(out);
+  if (lo > 0) {
+    if (lo & 1) p[lo] = static_cast<uint16_t>(pick(w, lo >> 1) >> 16);
+    const int q = (lo + 1) & ~1;
+    if (q & 2) *reinterpret_cast<uint32_t*>(p + q) = q & 4 ? w[3] : w[1];
+    if (lo <= 4) *reinterpret_cast<uint2*>(p + 4) = make_uint2(w[2], w[3]);
+  } else {
+    if (hi & 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    if (hi & 2) *reinterpret_cast<uint32_t*>(p + (hi & 4)) = hi & 4 ? w[2] : w[0];
+    if (hi & 1) p[hi - 1] = static_cast<uint16_t>(pick(w, hi >> 1));
+  }
+}
+__device__ __forceinline__ void put_cut(e4m3_t* out, const V8& v, int lo, int hi) {
+  const uint32_t w[4] = {pack_e4m3x2(v.p[0].x, v.p[0].y), pack_e4m3x2(v.p[1].x, v.p[1].y), pack_e4m3x2(v.p[2].x, v.p[2].y),
+                         pack_e4m3x2(v.p[3].x, v.p[3].y)};
+  uint8_t* p = reinterpret_cast<uint8_t*>(out);
+  if (lo > 0) {
+    if (lo & 1) p[lo] = static_cast<uint8_t>(pick(w, lo >> 1) >> 8);
+    const int q = (lo + 1) & ~1;
+    if (q & 2) *reinterpret_cast<uint16_t*>(p + q) = static_cast<uint16_t>(q & 4 ? w[3] : w[1]);
+    if (lo <= 4) *reinterpret_cast<uint32_t*>(p + 4) = w[2] | w[3] << 16;
+  } else {
+    if (hi & 4) *reinterpret_cast<uint32_t*>(p) = w[0] | w[1] << 16;
+    if (hi & 2) *reinterpret_cast<uint16_t*>(p + (hi & 4)) = static_cast<uint16_t>(hi & 4 ? w[2] : w[0]);
+    if (hi & 1) p[hi - 1] = static_cast<uint8_t>(pick(w, hi >> 1));
+  }
+}
+// Eight values to column j of a row of n columns (0: nothing).
+template <int MODE, class T>
+__device__ __forceinline__ void put(T* p, int j, int n, const V8& v) {
   const float t[8] = {v.p[0].x, v.p[0].y, v.p[1].x, v.p[1].y, v.p[2].x, v.p[2].y, v.p[3].x, v.p[3].y};
-  store_group<MODE>(p, j, d, t);
+  if constexpr (MODE == kShift) {
+    if (j >= 0 && j + 8 <= n) {
+      store_vals(p + j, t);
+    } else if (j < n) {
+      if (j >= 0 || j + 8 <= n) {
+        put_cut(p + j, v, j < 0 ? -j : 0, n - j);
+      } else {  // a row within one group
+        store_group<MODE>(p, j, n, t);
+      }
+    }
+  } else {
+    store_group<MODE>(p, j, n, t);
+  }
 }
 // Eight of a row of columns (weights, a gate's row); ones where there is none, 0 outside [0, d).
 template <int MODE>
@@ -121,15 +228,16 @@ __device__ __forceinline__ const void* gate_row(const void* gate, bool gate_bf16
 }
 // Eight of a row of a gate that has one for every row: aligned as the row itself is.
 template <int MODE>
-__device__ __forceinline__ V8 gate_values(const void* gate, bool gate_bf16, int64_t row, int j, int d, int width, bool more) {
+__device__ __forceinline__ V8 gate_values(const void* gate, bool gate_bf16, int64_t row, int j, int d, int width, bool whole,
+                                          const Cut<MODE>& cut) {
   if (gate_bf16) {
     Raw<bf16, 8> r;
-    load_group<MODE>(static_cast<const bf16*>(gate) + row * width, j, d, more, r);
-    return values<MODE>(r, j, d);
+    grab<MODE>(static_cast<const bf16*>(gate) + row * width, j, d, whole, r);
+    return values(r, cut);
   }
   Raw<float, 8> r;
-  load_group<MODE>(static_cast<const float*>(gate) + row * width, j, d, more, r);
-  return values<MODE>(r, j, d);
+  grab<MODE>(static_cast<const float*>(gate) + row * width, j, d, whole, r);
+  return values(r, cut);
 }
 // Values that dropout takes become 0, whatever they were.
 __device__ __forceinline__ V8 kept(const V8& v, const uint4& words, uint32_t least) {

@@ -3,8 +3,10 @@ masks where they can go wrong; captured graphs, streams, refusals.
 
 Tolerances. A result rounded to type t is off by finfo(t).eps / 2 of itself. Before that the kernels compute in float32: a
 norm's root is good to (d / 64 + 16) 2^-24 (sums of d squares, over at least 8 threads in exchanges), a value is the product
-of at most six factors and a sum of two or three terms, each of the size of the row's largest: (d / 64 + 40) 2^-24 of the
-row's largest bounds them. Column sums add a term for each row in at most rows / 64 + 80 steps.
+of at most six factors and a sum of two or three terms: (d / 64 + 40) 2^-24 of the terms bounds it. The terms of s are
+residual_scale x and the branch, which may cancel: with T the row's largest sum of their absolute values, s is off by
+(d / 64 + 40) 2^-24 T at most, and what is divided by s's root mean square R by T / R times as much of itself (a row of one
+column, or of a few, can have T far above R). Column sums add a term for each row in at most rows / 64 + 80 steps.
 """
 import numpy as np
 import pytest
@@ -174,6 +176,11 @@ CASES = [
     ((4, 8192), BF16, BF16, "channel", F32, BF16, 1.0, 0.1),
     ((11, 8185), F32, F32, None, F32, F32, 0.0, 0.1),
     ((333, 192), F32, BF16, "channel", F32, BF16, 1.0, 0.1),
+    ((700, 250), BF16, BF16, "channel", F32, BF16, 1.0, 0.1),
+    ((300, 252), F32, F32, "value", F32, F32, 1.0, 0.0),
+    ((1000, 1), F32, BF16, "channel", F32, F32, 1.0, 0.3),
+    ((500, 3), BF16, BF16, "channel", F32, BF16, 1.0, 0.0),
+    ((211, 9), F32, BF16, "value", F32, BF16, 1.0, 0.1),
     ((90, 333), BF16, F32, "channel", F32, BF16, 1.0, 0.0),
     ((2, 70, 760), F32, BF16, "sample", BF16, F32, 1.0, 0.1),
     ((33, 771), F32, BF16, "value", F32, BF16, 1.0, 0.1),
@@ -204,8 +211,10 @@ def test_branch_norm_and_gradients(cuda, case):
   mask = _mask(shape, p, 42, 2) if p else None
   v, h64, s64 = _formula(x, y, pw, w, g, alpha, 1e-6, mask)
   d = shape[-1]
-  _close(s.detach(), s64.detach(), _rows_room(s64.detach(), d), "s")
-  _close(h.detach(), h64.detach(), _rows_room(h64.detach(), d), "h")
+  terms = _terms(x, s64, alpha)
+  amp = 1 + 2 * terms / torch.sqrt((s64.detach() ** 2).sum(-1, keepdim=True) / d + 1e-6)
+  _close(s.detach(), s64.detach(), (d / 64 + 40) * U * terms, "s")
+  _close(h.detach(), h64.detach(), amp * _rows_room(h64.detach(), d), "h")
   leaves = [t for t in v if t is not None]
   want = torch.autograd.grad((h64, s64), leaves, (dh.double(), ds.double()))
   names = [n for n, t in zip(("x", "y", "post_weight", "weight", "gate"), ins) if t is not None]
@@ -214,29 +223,35 @@ def test_branch_norm_and_gradients(cuda, case):
     for name, a, b in zip(names, got, want):
       if name in ("x", "y") or (name == "gate" and a.shape == x.shape):
         # Gradients of a row: differences of terms of the size of the row's largest gradient times the factors' largest.
-        room = (d / 64 + 60) * U * 8 * b.abs().amax(-1, keepdim=True).clamp(min=_size_of_terms(x, y, dh, ds, w, name, leaves, names, alpha))
+        room = (d / 64 + 60) * U * 8 * torch.maximum(b.abs().amax(-1, keepdim=True), _size_of_terms(y, s64, dh, ds, name, leaves, names)) * amp
         _close(a, b, room, "d_" + name)
       else:
-        terms = _column_terms(name, x, y, dh, ds, v, alpha, mask)
-        _close(a, b, (rows / 64 + 200 + d / 8) * U * terms.view(b.shape), "d_" + name)
+        columns = _column_terms(name, x, y, dh, ds, v, alpha, mask, amp)
+        _close(a, b, (rows / 64 + 200 + d / 8) * U * columns.view(b.shape), "d_" + name)
 
 
-def _size_of_terms(x, y, dh, ds, w, name, leaves, names, alpha):
+def _terms(x, s64, alpha):
+  """The row's largest |residual_scale x| + |branch|."""
+  ax = alpha * x.detach().double()
+  return (ax.abs() + (s64.detach() - ax).abs()).amax(-1, keepdim=True)
+
+
+def _size_of_terms(y, s64, dh, ds, name, leaves, names):
   """A bound of the terms that a row's gradient is made of, from the row's values (float64 [..., 1])."""
-  d = x.shape[-1]
-  r1 = 1 / torch.sqrt((y.double() ** 2).sum(-1, keepdim=True) / d + 1e-6)
+  d = y.shape[-1]
+  r1 = 1 / torch.sqrt((y.detach().double() ** 2).sum(-1, keepdim=True) / d + 1e-6)
+  r2 = 1 / torch.sqrt((s64.detach() ** 2).sum(-1, keepdim=True) / d + 1e-6)
   v = dict(zip(names, leaves))
-  s_rms = torch.sqrt(((alpha * x.double()) ** 2).sum(-1, keepdim=True) / d + 1e-6)
   g = dh.abs().double().amax(-1, keepdim=True) * (v["weight"].abs().max() if "weight" in v else 1.0)
-  dt = 2 * g * d ** 0.5 / torch.minimum(s_rms, torch.ones_like(s_rms)).clamp(min=0.05) + ds.abs().double().amax(-1, keepdim=True)
+  dt = 2 * g * d ** 0.5 * r2 + ds.abs().double().amax(-1, keepdim=True)
   if name == "x":
     return dt
   f = (v["post_weight"].abs().max() if "post_weight" in v else 1.0) * (v["gate"].abs().max() if "gate" in v else 1.0)
   return dt * f * 4 * (r1 if name == "y" else d ** 0.5)
 
 
-def _column_terms(name, x, y, dh, ds, v, alpha, mask):
-  """Sum over rows of the absolute terms of a column's sum, with autograd's own derivative of the absolute values' bound."""
+def _column_terms(name, x, y, dh, ds, v, alpha, mask, amp):
+  """Sum over rows of the absolute terms of a column's sum, each with its row's `amp`."""
   d = x.shape[-1]
   xs, ys = x.double(), y.double()
   yhat = ys / torch.sqrt((ys ** 2).sum(-1, keepdim=True) / d + 1e-6)
@@ -251,9 +266,9 @@ def _column_terms(name, x, y, dh, ds, v, alpha, mask):
   shat = s * r2
   gs = dh.double() * w
   dt = r2 * (gs.abs() + shat.abs() * (gs * shat).abs().mean(-1, keepdim=True)) + ds.double().abs()
-  db = dt * (mask if mask is not None else 1.0)
+  db = dt * amp * (mask if mask is not None else 1.0)
   if name == "weight":
-    return (dh.double().abs() * shat.abs()).reshape(-1, d).sum(0)
+    return (dh.double().abs() * shat.abs() * amp).reshape(-1, d).sum(0)
   if name == "post_weight":
     return (db * (yhat * g).abs()).reshape(-1, d).sum(0)
   t = db * (yhat * pw).abs()
@@ -340,6 +355,23 @@ def test_strides_offsets_and_layouts(cuda):
   twin = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for t in leaves]
   want = torch.autograd.grad(branch.branch_norm(*twin)[0], twin, dh.contiguous())
   assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_columns_off_their_alignment(cuda):
+  """Weights and gates that start anywhere, of widths that are multiples of 8: the form for rows of any width."""
+  from faster_weathernext import _lib, branch
+  rand = _randn(21)
+  x, y = rand(50, 64), rand(50, 64).to(BF16)
+  pool = 1 + 0.1 * rand(200)
+  odd = [pool[i:i + 64] for i in (1, 66, 131)]
+  want = branch.branch_norm(x, y, odd[0].clone(), odd[1].clone(), gate=odd[2].clone())
+  s, h = torch.empty_like(x), torch.empty(50, 64, device="cuda", dtype=BF16)
+  desc = _lib.BranchDesc(50, 64, 64, 50, 64, _lib.DTYPE_F32, _lib.DTYPE_BF16, 1, 1, 1, _lib.DTYPE_BF16, 1e-6, 1.0, 0)
+  _lib.check(_lib.lib().fwn_branch_norm(desc, x.data_ptr(), y.data_ptr(), *[t.data_ptr() for t in odd], s.data_ptr(), h.data_ptr(),
+                                        None, None, torch.cuda.current_stream().cuda_stream))
+  _close(h, want[0].double(), 2.0 ** -7 * want[0].double().abs())
+  _close(s, want[1].double(), 8 * U * want[1].double().abs().amax())
+  assert all(torch.equal(a, b) for a, b in zip(branch.branch_norm(x, y, odd[0], odd[1], gate=odd[2]), want))
 
 
 def test_empty_and_partial_gradients(cuda):
