@@ -15,20 +15,21 @@ __device__ __forceinline__ void put_at(void* p, bool is_bf16, int64_t i, float v
     static_cast<float*>(p)[i] = v;
 }
 
-// A block takes 8 columns, a warp four rows of partials at a time. blockIdx.y 0: the slices' partials of u, gate by gate (as
-// many gates at once as leave each a power of two of the 32 warps), to d_gate and, over the gates, to d_post_weight; 1: the
-// blocks' partials of d_weight.
-__global__ void __launch_bounds__(1024) branch_bwd_finish_kernel(const BranchBwdParams p) {
-  __shared__ float red[32][8];
+// A block of W warps takes 8 columns, a warp four rows of partials at a time. blockIdx.y 0: the slices' partials of u, gate by
+// gate (as many gates at once as leave each a power of two of the warps), to d_gate and, over the gates, to d_post_weight; 1:
+// the blocks' partials of d_weight.
+template <int W>
+__global__ void __launch_bounds__(32 * W) branch_bwd_finish_kernel(const BranchBwdParams p) {
+  __shared__ float red[W][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int j = blockIdx.x * 8 + (lane & 7), d = p.d;
   const bool in = j < d;
   const bool for_u = blockIdx.y == 0 && p.part_u != nullptr;
   const float* part = for_u ? p.part_u : p.part_w;
   const int gates = for_u ? p.gates : 1, rows = for_u ? p.slices : p.blocks;
-  int per = 32;  // warps of a gate
-  while (per > 1 && 32 / per < gates) per >>= 1;
-  const int at_once = 32 / per, sub = warp % per;
+  int per = W;  // warps of a gate
+  while (per > 1 && W / per < gates) per >>= 1;
+  const int at_once = W / per, sub = warp % per;
   const bool gated = for_u && p.gate != nullptr && !p.gate_values;
   const float pw = for_u && p.post_weight != nullptr && in ? value_at(p.post_weight, p.post_bf16, j) : 1.f;
   float total = 0.f;
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(1024) branch_bwd_finish_kernel(const BranchBwd
   if (lane < 8) red[warp][lane] = total;  // 0 where sub > 0
   __syncthreads();
   if (warp == 0 && lane < 8 && in) {
-    for (int q = 1; q < 32; ++q) total += red[q][lane];
+    for (int q = 1; q < W; ++q) total += red[q][lane];
     if (for_u) {
       if (p.d_post != nullptr) put_at(p.d_post, p.post_bf16, j, total);
     } else {
@@ -93,7 +94,11 @@ cudaError_t launch_branch_bwd_finish(const BranchBwdParams& p, cudaStream_t st) 
   const int sums = (p.part_u != nullptr ? 1 : 0) + (p.part_w != nullptr ? 1 : 0);
   if (sums == 0) return cudaSuccess;
   const dim3 grid(static_cast<unsigned>((p.d + 7) / 8), static_cast<unsigned>(sums));
-  branch_bwd_finish_kernel<<<grid, 1024, 0, st>>>(p);
+  // Narrow rows have few blocks of many partials each, wide ones many of few.
+  if (p.d <= 1024)
+    branch_bwd_finish_kernel<32><<<grid, 1024, 0, st>>>(p);
+  else
+    branch_bwd_finish_kernel<8><<<grid, 256, 0, st>>>(p);
   return cudaGetLastError();
 }
 
