@@ -29,7 +29,7 @@ cudaError_t launch_route(const RouteParams& p, cudaStream_t stream);
 cudaError_t launch_route_bwd(const float* weights, const int32_t* chosen, const float* d_weights, int64_t rows, int experts,
                              int top, void* d_logits, bool bf16_logits, cudaStream_t stream);
 
-// Rows of `d` values, float32 or bf16. `wide`: every row of each tensor starts where 8 values are one access.
+// Rows of `d` values, float32 or bf16. `wide`, `pairs`: every row of each tensor starts where 8 (2) values are one access.
 struct RowMoveParams {
   const void* x;         // [rows, d], row stride x_stride
   const void* y;         // [rows top, d] contiguous: spread's other operand of the dots, gather's rows; or null
@@ -39,7 +39,7 @@ struct RowMoveParams {
   float* dots;           // [rows, top] or null: x[r] . y[position[r, j]]
   int64_t rows, x_stride;
   int d, top;
-  bool bf16_rows, wide;
+  bool bf16_rows, wide, pairs;
 };
 // to[position[r, j]] = weights[r, j] x[r], and the dots.
 cudaError_t launch_spread(const RowMoveParams& p, cudaStream_t stream);

@@ -37,10 +37,11 @@ RowMoveParams move_of(const fwn_route_desc& d, int32_t width, const int32_t* pos
   p.bf16_rows = d.dtype == FWN_DTYPE_BF16;
   return p;
 }
-// Whether tensors start where 8 values are one access.
-bool starts_wide(int32_t dtype, std::initializer_list<const void*> tensors) {
+// Whether rows of `width` values, `stride` apart, of these tensors start where n values are one access.
+bool rows_start(int n, int32_t dtype, int32_t width, int64_t stride, std::initializer_list<const void*> tensors) {
+  if (width % n != 0 || stride % n != 0) return false;
   for (const void* t : tensors)
-    if (!abi_aligned(t, 8 * abi_size(dtype))) return false;
+    if (!abi_aligned(t, n * abi_size(dtype))) return false;
   return true;
 }
 
@@ -101,7 +102,6 @@ fwn_status fwn_route_bwd(const fwn_route_desc* desc, const float* weights, const
   if (d.rows == 0) return abi_ok();
   if (!weights || !experts || !d_weights || !d_logits) return abi_fail(FWN_ERR_INVALID_ARGUMENT, "null pointer");
   if (fwn_status s = abi_elements({{weights, 4}, {experts, 4}, {d_weights, 4}, {d_logits, abi_size(d.dtype)}}); s != FWN_OK) return s;
-  if (d.rows * d.experts > 255ll * INT32_MAX) return abi_fail(FWN_ERR_UNSUPPORTED, "rows=%lld too large", static_cast<long long>(d.rows));
   cudaError_t e = launch_route_bwd(weights, experts, d_weights, d.rows, d.experts, d.top, d_logits, d.dtype == FWN_DTYPE_BF16,
                                    static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return abi_cuda_fail(e, "route_bwd");
@@ -123,7 +123,9 @@ fwn_status fwn_route_spread(const fwn_route_desc* desc, int32_t width, const voi
   p.y = y;
   p.to = out;
   p.dots = dots;
-  p.wide = width % 8 == 0 && (d.rows == 1 || x_stride % 8 == 0) && starts_wide(d.dtype, {x, y, out});
+  const int64_t stride = d.rows == 1 ? width : x_stride;
+  p.wide = rows_start(8, d.dtype, width, stride, {x, y, out});
+  p.pairs = rows_start(2, d.dtype, width, stride, {x, y, out});
   cudaError_t e = launch_spread(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return abi_cuda_fail(e, "route_spread");
   return abi_ok();
@@ -140,7 +142,8 @@ fwn_status fwn_route_gather(const fwn_route_desc* desc, int32_t width, const voi
   RowMoveParams p = move_of(d, width, position, weights);
   p.y = y;
   p.to = out;
-  p.wide = width % 8 == 0 && starts_wide(d.dtype, {y, out});
+  p.wide = rows_start(8, d.dtype, width, width, {y, out});
+  p.pairs = rows_start(2, d.dtype, width, width, {y, out});
   cudaError_t e = launch_gather(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return abi_cuda_fail(e, "route_gather");
   return abi_ok();

@@ -49,7 +49,7 @@ def _check_plan(r, idx, e):
 
 @pytest.mark.parametrize("rows,e,k", [(1, 1, 1), (1, 64, 4), (3, 8, 8), (127, 5, 3), (128, 8, 2), (129, 8, 2), (1000, 9, 1),
                                       (1000, 16, 16), (513, 17, 3), (2000, 33, 8), (700, 64, 2), (700, 128, 5), (400, 200, 12),
-                                      (400, 300, 2), (260, 1023, 16), (100, 1023, 7), (40000, 8, 2)])
+                                      (400, 300, 2), (260, 1023, 16), (100, 1023, 7), (40000, 8, 2), (300, 65, 4), (129, 10, 10), (1000, 31, 6), (128, 300, 3)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_route(cuda, rows, e, k, dtype):
   from faster_weathernext import experts
@@ -69,23 +69,26 @@ def test_route(cuda, rows, e, k, dtype):
   _close(got, want, 80 * U * size, "d_logits")
 
 
-def test_ties_and_special_logits(cuda):
+@pytest.mark.parametrize("times", [1, 40])
+def test_ties_and_special_logits(cuda, times):
+  """Few rows (one block, several lanes a row) and many (a thread a row)."""
   from faster_weathernext import experts
   inf, nan = float("inf"), float("nan")
   logits = torch.tensor([[0.0, -0.0, 0.0, 0.0], [1, 1, 1, 1], [-inf, 3, -inf, -inf], [-inf] * 4, [2, nan, 5, nan],
-                         [-3.4e38, -inf, -3.4e38, -inf], [3.4e38, 3.4e38, 0, -3.4e38]], device="cuda").requires_grad_()
+                         [-3.4e38, -inf, -3.4e38, -inf], [3.4e38, 3.4e38, 0, -3.4e38]], device="cuda").repeat(times, 1).requires_grad_()
   r = experts.route(logits, 2)
-  _check_plan(r, np.array([[0, 1], [0, 1], [1, 0], [0, 1], [1, 3], [0, 2], [0, 1]]), 4)
+  _check_plan(r, np.tile(np.array([[0, 1], [0, 1], [1, 0], [0, 1], [1, 3], [0, 2], [0, 1]]), (times, 1)), 4)
   w = r.weights.detach()
   half = torch.tensor([0.5, 0.5], device="cuda")
   assert torch.equal(w[0], half) and torch.equal(w[1], half) and torch.equal(w[5], half) and torch.equal(w[6], half)
   assert torch.equal(w[2], torch.tensor([1.0, 0.0], device="cuda")) and (w[3] == 0).all() and torch.isnan(w[4]).all()
-  g, = torch.autograd.grad(r.weights, logits, torch.tensor([[1.0, 2.0]], device="cuda").repeat(7, 1))
+  g, = torch.autograd.grad(r.weights, logits, torch.tensor([[1.0, 2.0]], device="cuda").repeat(7 * times, 1))
   assert (g[2] == 0).all() and (g[3] == 0).all() and torch.isfinite(g[[0, 1, 5, 6]]).all() and torch.equal(g[0], torch.tensor([-0.25, 0.25, 0, 0], device="cuda"))
 
 
 @pytest.mark.parametrize("rows,e,k,d", [(1, 4, 2, 2048), (7, 4, 1, 8), (130, 8, 2, 512), (333, 6, 3, 65), (257, 16, 4, 1000), (90, 32, 8, 129),
-                                        (50, 20, 16, 264), (12, 4, 2, 1), (2000, 8, 2, 515)])
+                                        (50, 20, 16, 264), (12, 4, 2, 1), (2000, 8, 2, 515), (301, 8, 2, 514), (77, 8, 8, 128), (77, 8, 3, 120),
+                                        (1001, 12, 12, 64), (33, 20, 9, 56), (9, 4, 1, 250)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_there_and_back(cuda, rows, e, k, d, dtype):
   from faster_weathernext import experts
