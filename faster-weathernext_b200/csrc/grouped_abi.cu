@@ -87,11 +87,11 @@ int plan_rows(int64_t m, int64_t n, int64_t k, int groups, int32_t act, bool pre
   return best_tile;
 }
 
-// The weights' gradient: out [rows, cols] of each expert, its rows summed over whole (run 0) or in runs of equal length,
-// which balance experts of different sizes and fill the SMs where experts and tiles are few, at the cost of a float32 part
-// for each run, written and added through L2.
+// The weights' gradient: out [rows, cols] of each expert, its rows summed over whole (run 0) or in equal runs of at most
+// `run` stages, which balance experts of different sizes and fill the SMs where experts and tiles are few, at the cost of a
+// float32 part for each run, written and added through L2.
 struct WeightPlan {
-  int tile, run;     // run: stages of 64 rows; 0: an expert's rows at once
+  int tile, run;     // run: stages of 64 rows at most; 0: an expert's rows at once
   int64_t most;      // runs (or experts)
 };
 constexpr int64_t kMaxStages = 1 << 20;  // of a run: a tile's epilogue waits for it, within the limit of its waits
@@ -430,7 +430,6 @@ fwn_status fwn_linear_grouped_bwd(const fwn_grouped_desc* desc, const void* a, c
     gp.first = g.first[2];
     gp.map_a = map_of(pl.turned ? 6 : 5);
     gp.map_b = map_of(pl.turned ? 5 : 6);
-    gp.run = runs ? pl.w.run : static_cast<int>(kMaxStages);
     gp.by_run = runs;
     if ((e = launch_grouped_weights(pl.w.tile, to, p, gp, items, sms, st)) != cudaSuccess) return abi_cuda_fail(e, "grouped d_b");
     if (runs && (e = launch_grouped_run_sum(reinterpret_cast<float*>(ws + pl.part_w), gp.first, d.groups, pl.w_rows,

@@ -53,7 +53,6 @@ struct GroupParams {
   const CUtensorMap* map_x;
   const CUtensorMap* map_o;
   int groups;
-  int run;                    // kGroupK: stages of k in a run
   bool by_run;                // kGroupK: out has a matrix for every run (else for every expert)
 };
 

@@ -357,7 +357,7 @@ struct TileWalk {
 
 // The tiles of a product grouped by expert, n fastest. kGroupRows: an expert's rows are cut into tiles of TM rows from its
 // first; the walk counts them over all experts (gp.first). kGroupK: every expert's product has m_tiles x n_tiles tiles, and
-// the sum over its rows is cut into runs of gp.run stages, counted likewise.
+// the sum over its rows is cut into equal runs, counted likewise.
 template <int GROUP, int TM>
 struct GroupWalk {
   int t, nt, mt, g, at, items;  // at: the tile of rows, or the run, over all experts
@@ -417,9 +417,12 @@ struct GroupWalk {
       row0 = row + mine * TM;
       end = past;
     } else {
+      // The expert's stages in equal parts, as many as it has runs.
       k_row = row;
-      kb_first = mine * gp.run;
-      kb_last = min(kb_first + gp.run, (past - row + 63) >> 6);
+      const int stages = (past - row + 63) >> 6, runs = __ldg(gp.first + g + 1) - __ldg(gp.first + g);
+      const int each = stages / runs, more = stages - each * runs;
+      kb_first = mine * each + min(mine, more);
+      kb_last = kb_first + each + (mine < more ? 1 : 0);
     }
   }
   __device__ __forceinline__ bool in(const LinearParams&) const { return t < items; }
