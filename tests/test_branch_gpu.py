@@ -393,6 +393,60 @@ def test_empty_and_partial_gradients(cuda):
   assert gx.shape == (0, 64) and (gw == 0).all()
 
 
+@pytest.mark.parametrize("d", [64, 333, 1001])
+@pytest.mark.parametrize("have", ["post_weight", "weight", "gate", "post_weight gate", "weight gate"])
+def test_some_of_the_columns(cuda, d, have):
+  """Either weight or the gate alone: what is not given counts as ones, and only what is given gets a gradient."""
+  from faster_weathernext import branch
+  x, y, pw, w, g = _inputs((3, 17, d), F32, BF16, "sample", F32)
+  kw = {"post_weight": pw, "weight": w, "gate": g}
+  given = {k: v.requires_grad_() for k, v in kw.items() if k in have.split()}
+  ones = {k: v if k in given else torch.ones_like(v) for k, v in kw.items()}
+  x.requires_grad_()
+  dh, ds = _randn(1)(3, 17, d).to(BF16), _randn(2)(3, 17, d)
+  leaves = [x, *given.values()]
+  a, b = branch.branch_norm(x, y, p=0.1, seed=1, **given), branch.branch_norm(x, y, p=0.1, seed=1, **ones)
+  assert all(torch.equal(u, v) for u, v in zip(a, b))
+  got, want = (torch.autograd.grad(o, leaves, (dh, ds)) for o in (a, b))
+  assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+@pytest.mark.parametrize("d", [65, 250, 1001, 2047])
+def test_one_gradient_of_odd_rows(cuda, d):
+  """Rows that start anywhere, with the gradient of one output alone: the other one's is not there to read."""
+  from faster_weathernext import branch
+  for xd, yd in ((F32, BF16), (BF16, F32)):
+    ins = _inputs((2, 21, d), xd, yd, "sample", F32)
+    for t in ins:
+      t.requires_grad_()
+    h, s = branch.branch_norm(*ins[:4], gate=ins[4], p=0.2, seed=3)
+    dh, ds = _randn(1)(2, 21, d).to(BF16), _randn(2)(2, 21, d).to(xd)
+    only_h = torch.autograd.grad(h, ins, dh, retain_graph=True)
+    both = torch.autograd.grad((h, s), ins, (dh, torch.zeros_like(ds)), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(only_h, both))
+    only_s = torch.autograd.grad(s, ins, ds, allow_unused=True, retain_graph=True)
+    both = torch.autograd.grad((h, s), ins, (torch.zeros_like(dh), ds))
+    assert all(torch.equal(a, b) for a, b in zip(only_s, both))
+
+
+@pytest.mark.parametrize("d", [64, 65, 100, 250, 1001])
+@pytest.mark.parametrize("gate", ["sample", "value"])
+def test_nan_stays_with_its_gate(cuda, d, gate):
+  """A sample's NaN reaches no other sample's rows nor its gate's gradient."""
+  from faster_weathernext import branch
+  ins = _inputs((4, 9, d), F32, BF16, gate, F32)
+  dh, ds = _randn(1)(4, 9, d).to(BF16), _randn(2)(4, 9, d)
+  for t in ins:
+    t.requires_grad_()
+  want = torch.autograd.grad(branch.branch_norm(*ins[:4], gate=ins[4]), (ins[0], ins[1], ins[4]), (dh, ds))
+  with torch.no_grad():
+    for t in ins[:2]:
+      t[2] = float("nan")
+    dh[2], ds[2] = float("nan"), float("nan")
+  got = torch.autograd.grad(branch.branch_norm(*ins[:4], gate=ins[4]), (ins[0], ins[1], ins[4]), (dh, ds))
+  assert all(torch.equal(a[[0, 1, 3]], b[[0, 1, 3]]) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("shape,gate", [((0, 64), (64,)), ((3, 0, 64), (3, 64)), ((0, 5, 64), (0, 64)), ((0, 64), (0, 64))])
 def test_gates_of_no_rows(cuda, shape, gate):
   from faster_weathernext import branch
