@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(MAXT, (branch_resident(TPR, NV) / MAXT)) branc
     for (int i = 0; i < NV; ++i) {
       const int j = column_of<TPR>(i, off);
       s[i] = mul(mul(s[i], r1), g[i]);
-      if (own_gate) s[i] = mul(s[i], gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, row < whole, cut[i]));
+      if (own_gate) s[i] = mul(s[i], gate_values<MODE>(p.gate, p.gate_bf16, row, j, d, n > 0, row < whole, cut[i]));
       if (drops) s[i] = kept(s[i], drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3), least);
 #pragma unroll
       for (int q = 0; q < 4; ++q) s[i].p[q] = fadd2(s[i].p[q], x[i].p[q]);

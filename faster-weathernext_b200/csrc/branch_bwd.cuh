@@ -11,7 +11,7 @@
 // row's loads ahead; its columns' sums stay in registers and leave as one row of partials per block and gate slice, added
 // in order by branch_bwd_finish: no atomics, the same bits every time. Measured at 163,848 x 512, float32 stream, bf16 branch
 // (of the measured copy rate): 230 us (1.00), with dropout 245 (0.94; bf16 stream 206, 0.75), and 7 for the sums; 40,962 x
-// 2,048 233 (0.99); 163,848 x 333 286 (0.52).
+// 2,048 233 (0.99); 163,848 x 333 247 (0.61).
 #pragma once
 
 #include "branch_rows.cuh"
@@ -86,12 +86,22 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
     float2 nr;
     auto fetch = [&](int64_t r) {
       const int n = r < end ? d : 0;  // a row that is not there adds nothing
-      const bool all = r < whole;
       nr = n > 0 ? __ldg(reinterpret_cast<const float2*>(p.rstd) + r) : make_float2(0.f, 0.f);
-      grab<MODE>(static_cast<const X*>(p.x) + r * p.x_stride, j, n, all, nx);
-      grab<MODE>(static_cast<const Y*>(p.y) + r * p.y_stride, j, n, all, ny);
-      grab<MODE>(static_cast<const G*>(p.dh) + r * d, j, p.dh != nullptr ? n : 0, all, ng);
-      grab<MODE>(static_cast<const X*>(p.ds) + r * d, j, p.ds != nullptr ? n : 0, all, nds);
+      const X *x = static_cast<const X*>(p.x) + r * p.x_stride, *ds = static_cast<const X*>(p.ds) + r * d;
+      const Y* y = static_cast<const Y*>(p.y) + r * p.y_stride;
+      const G* dh = static_cast<const G*>(p.dh) + r * d;
+      if constexpr (MODE == kWide) {
+        grab<MODE>(x, j, n, true, nx);
+        grab<MODE>(y, j, n, true, ny);
+        grab<MODE>(dh, j, p.dh != nullptr ? n : 0, true, ng);
+        grab<MODE>(ds, j, p.ds != nullptr ? n : 0, true, nds);
+      } else {
+        const bool there = n > 0, all = r < whole;
+        grab_shifted(x, j, d, there, all, nx);
+        grab_shifted(y, j, d, there, all, ny);
+        grab_shifted(dh, j, d, there && p.dh != nullptr, all, ng);
+        grab_shifted(ds, j, d, there && p.ds != nullptr, all, nds);
+      }
     };
     fetch(row);
     const V8 w = columns<MODE>(p.weight, p.weight_bf16, j, d);
@@ -103,7 +113,7 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
       const float r1 = nr.x, r2 = nr.y;
       const V8 yh = mul(values(ny, cut), r1);
       V8 b = mul(yh, a);
-      if (own_gate) b = mul(b, gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, row < whole, cut));
+      if (own_gate) b = mul(b, gate_values<MODE>(p.gate, p.gate_bf16, row, j, d, n > 0, row < whole, cut));
       uint4 words;
       if (drops) {
         words = drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3);
@@ -123,7 +133,7 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
       g = mul(dt, a);
       if (own_gate) {
         // The gate's own gradient (a is post_weight here), and the gate goes into the other two.
-        const V8 gv = gate_values<MODE>(p.gate, p.gate_bf16, row, j, n, d, row < whole, cut), dg = mul(g, yh);
+        const V8 gv = gate_values<MODE>(p.gate, p.gate_bf16, row, j, d, n > 0, row < whole, cut), dg = mul(g, yh);
         if (p.d_gate != nullptr) {
           if (p.gate_bf16)
             put<MODE>(static_cast<bf16*>(p.d_gate) + row * d, j, n, dg);

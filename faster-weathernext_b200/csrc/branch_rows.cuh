@@ -132,7 +132,7 @@ __device__ __forceinline__ V8 values(const Raw<float, 8>& r, const Cut<MODE>& cu
 // The group from column j of the row of n values at p (0: a row that is not there): a wide access, and single values only at
 // the tensor's end, where it would reach past it (not `whole`). What is not loaded is 0. (With the groups past a row's end in
 // the single values' loop too, and every column masked by comparisons, 163,848 x 250 bf16 took 132 us forward and 270
-// backward, so 75 and 127.)
+// backward.)
 template <int MODE, class T>
 __device__ __forceinline__ void grab(const T* p, int j, int n, bool whole, Raw<T, 8>& r) {
   if constexpr (MODE == kWide) {
@@ -144,6 +144,17 @@ __device__ __forceinline__ void grab(const T* p, int j, int n, bool whole, Raw<T
     if (in && wide) load_raw(p + j, r);
     if (in && !wide) load_group<MODE>(p, j, n, false, r);
   }
+}
+// The same of kShift, of a row of d values that is `there` or not: one condition for all of a row's tensors. The gradient,
+// which reads four, takes this one (40,962 x 1,001 bf16 123 us, with grab 147; 163,848 x 333 244 and 288), the forward the
+// other (73, and 78 with this one).
+template <class T>
+__device__ __forceinline__ void grab_shifted(const T* p, int j, int d, bool there, bool whole, Raw<T, 8>& r) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(r.u) / 4); ++i) r.u[i] = 0;
+  const bool quick = there && whole;
+  if (quick && j < d) load_raw(p + j, r);
+  if (there && !quick && j < d) load_group<kShift>(p, j, d, false, r);
 }
 // Rows before this one are followed by seven values or more.
 __device__ __forceinline__ int64_t whole_rows(int64_t rows, int d) { return rows - (d + 6) / d; }
@@ -230,15 +241,15 @@ __device__ __forceinline__ const void* gate_row(const void* gate, bool gate_bf16
 }
 // Eight of a row of a gate that has one for every row: aligned as the row itself is.
 template <int MODE>
-__device__ __forceinline__ V8 gate_values(const void* gate, bool gate_bf16, int64_t row, int j, int d, int width, bool whole,
+__device__ __forceinline__ V8 gate_values(const void* gate, bool gate_bf16, int64_t row, int j, int d, bool there, bool whole,
                                           const Cut<MODE>& cut) {
   if (gate_bf16) {
     Raw<bf16, 8> r;
-    grab<MODE>(static_cast<const bf16*>(gate) + row * width, j, d, whole, r);
+    grab<MODE>(static_cast<const bf16*>(gate) + row * d, j, there ? d : 0, whole, r);
     return values(r, cut);
   }
   Raw<float, 8> r;
-  grab<MODE>(static_cast<const float*>(gate) + row * width, j, d, whole, r);
+  grab<MODE>(static_cast<const float*>(gate) + row * d, j, there ? d : 0, whole, r);
   return values(r, cut);
 }
 // Values that dropout takes become 0, whatever they were.
