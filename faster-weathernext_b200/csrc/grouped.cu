@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(128) grouped_run_sum_kernel(const float* __res
     }
     bf16* to = out + (g * rows + row) * n + j;
     const float u[4] = {t.x, t.y, t.z, t.w};
-    if (n % 4 == 0) {
+    if (n % 4 == 0 && reinterpret_cast<uintptr_t>(to) % 8 == 0) {
       *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(u[0], u[1]), pack_bf16(u[2], u[3]));
     } else {
 #pragma unroll

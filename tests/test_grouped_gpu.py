@@ -286,6 +286,36 @@ def test_graph_takes_new_offsets(cuda):
     assert all(torch.equal(x, y) for x, y in zip(out, step()))
 
 
+@pytest.mark.parametrize("m,e,n,k", [(20000, 2, 64, 96), (3000, 40, 72, 64)])
+def test_c_entry_with_results_that_start_anywhere(cuda, m, e, n, k):
+  """Results at addresses of whole elements alone (the first shape sums its weights' gradient in runs, the second at once)."""
+  from faster_weathernext import _lib, experts
+  lib = _lib.lib()
+  a, w, b = _inputs(m, e, k, n, F32, "nk")
+  offsets = _offsets([m // e] * e)
+  dy = _randn(1)(m, n).to(BF16)
+  ins = [t.requires_grad_() for t in (a, w, b)]
+  y = experts.linear_grouped(a, w, offsets, b, activation="gelu")
+  want = [y.detach(), *torch.autograd.grad(y, ins, dy)]
+  pool = [torch.zeros(t.numel() + 8, device="cuda", dtype=t.dtype) for t in want]
+  got = [p[1:1 + t.numel()].view(t.shape) for p, t in zip(pool, want)]
+  desc = _lib.GroupedDesc(m, e, n, k, 0, 1, 0, _lib.ACT_GELU_TANH, 0, k, k, n * k, n)
+  stream = torch.cuda.current_stream().cuda_stream
+  import ctypes
+  size = ctypes.c_size_t(0)
+  _lib.check(lib.fwn_linear_grouped_workspace_size(desc, size))
+  ws = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+  _lib.check(lib.fwn_linear_grouped(desc, a.data_ptr(), w.data_ptr(), b.data_ptr(), offsets.data_ptr(), got[0].data_ptr(),
+                                    ws.data_ptr(), size.value, stream))
+  _lib.check(lib.fwn_linear_grouped_bwd_workspace_size(desc, dy.data_ptr(), size))
+  ws = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+  _lib.check(lib.fwn_linear_grouped_bwd(desc, a.data_ptr(), w.data_ptr(), b.data_ptr(), offsets.data_ptr(), dy.data_ptr(),
+                                        got[1].data_ptr(), got[2].data_ptr(), got[3].data_ptr(), ws.data_ptr(), size.value, stream))
+  for g, t, p in zip(got, want, pool):
+    assert (g.float() - t.float()).abs().max() <= 2.0 ** -7 * t.float().abs().max()   # other tiles: a step of the type
+    assert p[0] == 0 and (p[1 + t.numel():] == 0).all()
+
+
 def test_streams_and_repeats(cuda):
   from faster_weathernext import experts
   a, w, b = _inputs(3000, 8, 512, 512, F32, "nk")
