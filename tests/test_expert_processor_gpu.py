@@ -8,6 +8,13 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def _generators_as_they_were():
+  """What these tests draw from torch's default generators does not move the values of the tests after them."""
+  with torch.random.fork_rng():
+    yield
+
+
 def _cfg(**kw):
   from faster_weathernext.processor import ProcessorConfig
   return ProcessorConfig(**{**dict(layers=2, d_model=128, heads=2, head_dim=64, mlp_hidden=256, cond_dim=8), **kw})
