@@ -44,8 +44,8 @@ cudaError_t launch_grouped_rows(const void* a, int64_t lda, const void* b, int64
 constexpr int kCastRows = 256;
 cudaError_t launch_grouped_cast(const void* x, bool x_f32, int64_t ldx, int n, void* cast, int64_t ldc, float* part,
                                 const GroupParams& g, int64_t most, bool wide, cudaStream_t stream);
-// out[e, j] = sum of part's rows first[e] per to first[e + 1] per.
-cudaError_t launch_grouped_column_sum(const float* part, const int32_t* first, int groups, int per, int n, void* out,
+// out[e, j] = sum of part's rows first[e] per to first[e + 1] per (at most `most` tiles of `per` rows in all).
+cudaError_t launch_grouped_column_sum(const float* part, const int32_t* first, int groups, int64_t most, int per, int n, void* out,
                                       bool out_bf16, cudaStream_t stream);
 // out[e] (bf16, [rows, n] contiguous) = sum over the expert's runs of part [runs, rows, ldp].
 cudaError_t launch_grouped_run_sum(const float* part, const int32_t* first, int groups, int64_t rows, int n, int64_t ldp,

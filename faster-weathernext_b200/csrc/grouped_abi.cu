@@ -376,8 +376,8 @@ fwn_status fwn_linear_grouped_bwd(const fwn_grouped_desc* desc, const void* a, c
                                  tiles_most(d.m, d.groups, kCastRows), wide, st)) != cudaSuccess)
       return abi_cuda_fail(e, "grouped cast");
   }
-  if (d_bias && (e = launch_grouped_column_sum(part_sum, gp.first, d.groups, act ? g.unit[0] / 32 : 1, d.n, d_bias,
-                                               d.bias_dtype == FWN_DTYPE_BF16, st)) != cudaSuccess)
+  if (d_bias && (e = launch_grouped_column_sum(part_sum, gp.first, d.groups, tiles_most(d.m, d.groups, g.unit[0]),
+                                               act ? g.unit[0] / 32 : 1, d.n, d_bias, d.bias_dtype == FWN_DTYPE_BF16, st)) != cudaSuccess)
     return abi_cuda_fail(e, "grouped column sums");
 
   if (d_a) {
