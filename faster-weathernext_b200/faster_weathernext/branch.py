@@ -13,11 +13,13 @@ fwn_branch_norm*). Every call runs on the current stream of its tensors' device 
 allocator.
 """
 
+import ctypes
+
 import torch
 
 from faster_weathernext import _lib
 from faster_weathernext.projection import (_BF16, _CODE, _E4M3, _F32, _check, _constant, _first_order, _no_tangent,
-                                           _on_device, _rows, _workspace)
+                                           _on_device, _rows)
 
 
 # ---- dropout --------------------------------------------------------------------------------------------------------
@@ -152,7 +154,7 @@ def _ptr(t):
 
 
 def _branch_launch(stream, x, xs, y, ys, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site, keep_rstd, shape):
-  """(h, its scales or None, s, both roots of each row or None), h and s of x's shape."""
+  """(h, its scales or None, s, both roots of each row or None, the call's descriptor), h and s of x's shape."""
   s = x.new_empty(shape)
   h = x.new_empty(shape, dtype=out_dtype)
   h_scale = x.new_empty(shape[:-1], dtype=_F32) if out_dtype is _E4M3 else None
@@ -162,12 +164,27 @@ def _branch_launch(stream, x, xs, y, ys, pw, w, gate, span, out_dtype, eps, scal
                                       h.data_ptr(), _ptr(h_scale), _ptr(rstd), stream)
   if status:
     _lib.check(status)
-  return h, h_scale, s, rstd
+  return h, h_scale, s, rstd, desc
 
 
 def _branch_forward(x, y, pw, w, gate, span, out_dtype, eps, scale, threshold=0, seed=None, site=0, keep_rstd=False):
   return _on_device(x, _branch_launch, *_wide_or_plain(x.shape[-1], x, y), _plain(pw), _plain(w), _plain(gate), span, out_dtype,
                     eps, scale, threshold, seed, site, keep_rstd, x.shape)
+
+
+_BWD_BYTES = {}  # workspaces' sizes, which go by the shape alone
+
+
+def _bwd_bytes(x, desc):
+  key = (x.get_device(), desc.rows, desc.d, desc.gate_span)
+  size = _BWD_BYTES.get(key)
+  if size is None:
+    need = ctypes.c_size_t(0)
+    _lib.check(_lib.lib().fwn_branch_norm_bwd_workspace_size(desc, need))
+    if len(_BWD_BYTES) >= 4096:
+      _BWD_BYTES.clear()
+    size = _BWD_BYTES[key] = need.value
+  return size
 
 
 class _BranchNorm(torch.autograd.Function):
@@ -178,7 +195,7 @@ class _BranchNorm(torch.autograd.Function):
   def forward(ctx, x, y, pw, w, gate, seed, args):
     span, out_dtype, eps, scale, threshold, site = ctx.args = args
     ctx.seed = None if isinstance(seed, torch.Tensor) else seed
-    h, _, s, rstd = _branch_forward(x, y, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site, True)
+    h, _, s, rstd, ctx.desc = _branch_forward(x, y, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site, True)
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(x, y, pw, w, gate, rstd, seed if isinstance(seed, torch.Tensor) else None)
     return h, s
@@ -203,10 +220,12 @@ class _BranchNorm(torch.autograd.Function):
     dx, dy, dpw, dw, dgate = [t.new_empty(t.shape) if wanted else None for t, wanted in zip((x, y, pw, w, gate), need)]
     if need[4] and x.numel() == 0:
       dgate.zero_()
-    desc = _branch_desc(x2, xs, y2, ys, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site)
+    desc = ctx.desc  # the forward's, but where saved tensors came back in other places (hooks may move them)
+    if isinstance(seed, torch.Tensor) or (desc.x_stride, desc.y_stride) != (xs, ys):
+      desc = _branch_desc(x2, xs, y2, ys, pw, w, gate, span, out_dtype, eps, scale, threshold, seed, site)
     lib = _lib.lib()
-    ws, size = _workspace(x, _branch_desc(x2, xs, y2, ys, pw, w, gate, span, out_dtype, 0.0, 0.0, 0, None, 0),
-                          lib.fwn_branch_norm_bwd_workspace_size)  # it goes by the shape alone
+    size = _bwd_bytes(x, desc)
+    ws = x.new_empty((size,), dtype=torch.uint8) if size else None
     status = lib.fwn_branch_norm_bwd(desc, x2.data_ptr(), y2.data_ptr(), _ptr(pw2), _ptr(w2), _ptr(gate2), rstd.data_ptr(),
                                      _ptr(dh), _ptr(ds), _ptr(dx), _ptr(dy), _ptr(dpw), _ptr(dw), _ptr(dgate), _ptr(ws), size,
                                      stream)
@@ -262,7 +281,7 @@ def branch_norm(x, y, post_weight=None, weight=None, *, gate=None, residual_scal
   _no_tangent("branch_norm", x, y, post_weight, weight, gate)
   if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, y, post_weight, weight, gate)):
     return _BranchNorm.apply(x, y, post_weight, weight, gate, seed, (span, out_dtype, eps, residual_scale, threshold, site))
-  h, _, s, _ = _branch_forward(x, y, post_weight, weight, gate, span, out_dtype, eps, residual_scale, threshold, seed, site)
+  h, _, s, _, _ = _branch_forward(x, y, post_weight, weight, gate, span, out_dtype, eps, residual_scale, threshold, seed, site)
   return h, s
 
 

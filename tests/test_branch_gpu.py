@@ -583,3 +583,24 @@ def test_refusals(cuda):
     for call in (lambda: branch.dropout(dual, 0.1, 1), lambda: branch.branch_norm(dual, y)):
       with pytest.raises(NotImplementedError):
         call()
+
+
+def test_gradients_of_saved_tensors_that_come_back_elsewhere(cuda):
+  """Saved tensors may be moved between forward and backward (torch.autograd.graph's hooks): rows with a stride come back
+  without one, the seed at another address. The same bits as without."""
+  from faster_weathernext import branch
+  r = _randn(61)
+  wide, y, pw, w, gate = r(33, 160), r(33, 72).to(BF16), r(72), r(72).to(BF16), r(33, 72)
+  dh, ds = r(33, 72).to(BF16), r(33, 72)
+  seed = torch.tensor([77], dtype=torch.int64, device="cuda")
+
+  def grads(seed):
+    leaves = [t.clone().requires_grad_() for t in (wide, y, pw, w, gate)]
+    h, s = branch.branch_norm(leaves[0][:, 8:80], *leaves[1:4], gate=leaves[4], p=0.25, seed=seed)
+    return torch.autograd.grad((h, s), leaves, (dh, ds))
+
+  for used in (seed, 77):
+    want = grads(used)
+    with torch.autograd.graph.save_on_cpu():
+      got = grads(used)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
