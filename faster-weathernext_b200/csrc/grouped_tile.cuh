@@ -1,8 +1,8 @@
 // The tensor-core kernel over products grouped by expert (linear_tile.cuh's body, walked by GroupWalk), and its launch.
 //
 // Bound and tiles as the plain product's (linear_tile.cuh). Measured at 81,924 x 512 x 2,048 over 1 / 8 / 64 experts (plain):
-// GELU 151 / 154 / 169 us (146), act'() with column sums 236 / 239 / 247 (238), d_a 120 / 123 / 133 (119), the weights' gradient
-// 125 / 137 / 135 (125), of uneven experts 132 over 8 and 163 over 64, and its parts' sum 5 / 17 / 0.
+// GELU 152 / 154 / 169 us (146), act'() with column sums 228 / 232 / 240 (224), d_a 120 / 123 / 134 (120), the weights' gradient
+// 124 / 136 / 137 (124), of uneven experts 132 over 8 and 163 over 64, and its parts' sum 4 / 17 / 0.
 #pragma once
 
 #include "grouped.cuh"

@@ -287,7 +287,7 @@ __device__ __forceinline__ void activate4(float* v) {
 // 254-262 us = 1.31-1.35 PFLOP/s (cuBLAS 253-275 on the same boxes), the MMAs; 512 x 2,048 plain 294 (cuBLAS 316-355);
 // GELU 293-308 and e4m3 GELU 226, the latency of an epilogue chunk's steps (TMEM, arithmetic, shared memory, store), with no
 // unit full (tensor pipe 57 and 35 %, issue slots 50 and 64 %); residual in float32 285-303, the MMAs and 8 bytes a value of
-// HBM traffic; act'() with column sums at 81,924 rows 242, shared memory (x in, sums, result) and arithmetic. One product
+// HBM traffic; act'() with column sums at 81,924 rows 224, shared memory (x in, sums, result) and arithmetic. One product
 // recomputed in the backward instead of keeping the pre-activation: 102 us of MMAs under that epilogue, against 8 bytes a
 // value (0.2 ms) in float32. d_pre leaves in bf16, the operand of the two products that read it: 2.3e-3 of their results
 // against 1.7e-3 for their own rounding alone; two bf16 parts of it would double both (81,924 rows: 2 x 120 us).
@@ -649,7 +649,7 @@ __device__ __forceinline__ void linear_tile_body(const CUtensorMap& tm_a, const 
       tile_load<1>(slot, tm, w.nt * C::BN + part * C::HC + ch * CC, static_cast<int>(row_of(w)), x_bar(ew));
     };
     // dy of a tile in one chunk: its load follows the previous tile's store out of the same slot, and its way from HBM shows.
-    // So it goes to L2 a tile ahead: act'() 241 -> 234 us (81,924 x 512 x 2,048), 130 -> 124 (163,848 x 512 x 512). Of more
+    // So it goes to L2 a tile ahead: act'() 236 -> 224 us (81,924 x 512 x 2,048), 43 -> 41 (10,242), 20 -> 19 (2,562). Of more
     // chunks a tile the later ones' loads wait anyway: 295 -> 301 (40,000 x 2,048 x 2,048), a float32 residual 282 -> 312.
     constexpr bool kAhead = PRE && C::NCH == 1;
     auto prefetch_x = [&](const Walk& w) {
