@@ -101,7 +101,8 @@ def _grouped_launch(stream, a, weight, offsets, bias, act, out_dtype):
 
 
 class _LinearGrouped(torch.autograd.Function):
-  """linear_grouped with gradients, as projection._Linear's for each expert (fwn_linear_grouped_bwd)."""
+  """linear_grouped with gradients, as projection._Linear's for each expert (fwn_linear_grouped_bwd). Saved tensors may come
+  back in other places (hooks may move them): the operands are laid out again where they did."""
 
   @staticmethod
   def forward(ctx, a, weight, offsets, bias, act, out_dtype):
@@ -116,7 +117,9 @@ class _LinearGrouped(torch.autograd.Function):
     _no_tangent("linear_grouped's gradient", a, weight, bias, dy)
     need_a, need_w, _, need_b = ctx.needs_input_grad[:4]
     _first_order("linear_grouped")
-    d_a, d_w, d_b = _on_device(a, _LinearGrouped._launch, a, weight, offsets, bias, ctx.act, _rows(dy), need_a, need_w, need_b)
+    a, weight = _laid_rows(_rows(a)), _laid_out(weight)
+    d_a, d_w, d_b = _on_device(a, _LinearGrouped._launch, a, weight, offsets.contiguous(),
+                               None if bias is None else bias.contiguous(), ctx.act, _rows(dy), need_a, need_w, need_b)
     return d_a, d_w, None, d_b, None, None
 
   @staticmethod

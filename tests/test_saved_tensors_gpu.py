@@ -1,0 +1,55 @@
+"""GPU: gradients where saved tensors come back in other places between forward and backward (torch.autograd.graph's hooks
+move them): rows with a stride come back without one, or every value with one. What the kernels take is laid out again."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _randn(seed):
+  g = torch.Generator(device="cuda").manual_seed(seed)
+  return lambda *s: torch.randn(*s, device="cuda", generator=g)
+
+
+def _spread():
+  """Every saved tensor comes back as a view whose neighbouring values are two apart, the ones between being others."""
+  return torch.autograd.graph.saved_tensors_hooks(lambda t: torch.stack((t, t.flip(0)), -1), lambda t: t[..., 0])
+
+
+HOOKS = {"cpu": torch.autograd.graph.save_on_cpu, "spread": _spread}
+
+
+def _same(step, hooks, room=0.0):
+  want = step()
+  with HOOKS[hooks]():
+    got = step()
+  assert len(got) == len(want)
+  for a, b in zip(got, want):
+    assert a.shape == b.shape and a.dtype is b.dtype
+    if room:
+      assert (a.double() - b.double()).abs().max() <= room * b.double().abs().max()
+    else:
+      assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+@pytest.mark.parametrize("k,n,layout,act", [(65, 33, "nk", "gelu"), (1001, 515, "nk", None), (128, 64, "nk", "swish"),
+                                            (65, 40, "kn", "gelu"), (64, 35, "kn", None)])
+def test_grouped(cuda, hooks, k, n, layout, act):
+  """Padded copies of odd widths, wide rows and transposed weights. The transposed come back the other way round, whose
+  gradient may take other tiles: another order of the float32 sums, a step of bf16."""
+  from faster_weathernext import experts
+  r = _randn(k)
+  wide, w, b = r(210, k + 9).to(BF16), (r(3, n, k) * k ** -0.5).to(BF16), r(3, n)
+  if layout == "kn":
+    w = w.transpose(1, 2).contiguous().transpose(1, 2)
+  offsets = torch.tensor([2, 102, 102, 200], dtype=torch.int32, device="cuda")
+  dy = r(210, n).to(BF16)
+
+  def step():
+    leaves = [t.detach().requires_grad_() for t in (wide, w, b)]
+    y = experts.linear_grouped(leaves[0][:, 3:3 + k], leaves[1], offsets, leaves[2], activation=act)
+    return torch.autograd.grad(y, leaves, dy)
+
+  _same(step, hooks, 2.0 ** -7 if layout == "kn" else 0.0)
