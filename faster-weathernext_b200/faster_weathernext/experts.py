@@ -227,7 +227,7 @@ class _Route(torch.autograd.Function):
     chosen, weights = ctx.saved_tensors
     _no_tangent("route's gradient", weights, d_weights)
     _first_order("route")
-    return _on_device(weights, _Route._launch, ctx, chosen, weights, d_weights.contiguous()), None
+    return _on_device(weights, _Route._launch, ctx, chosen.contiguous(), weights.contiguous(), d_weights.contiguous()), None
 
   @staticmethod
   def _launch(stream, ctx, chosen, weights, d_weights):
@@ -305,7 +305,7 @@ class _Dispatch(torch.autograd.Function):
     position, = ctx.saved_tensors
     _no_tangent("dispatch's gradient", d_rows)
     _first_order("dispatch")
-    return _on_device(d_rows, _gather_launch, d_rows.contiguous(), position, None), None
+    return _on_device(d_rows, _gather_launch, d_rows.contiguous(), position.contiguous(), None), None
 
 
 class _Combine(torch.autograd.Function):
@@ -321,8 +321,8 @@ class _Combine(torch.autograd.Function):
     y, weights, position = ctx.saved_tensors
     _no_tangent("combine's gradient", y, weights, d_out)
     _first_order("combine")
-    d_y, d_weights = _on_device(d_out, _spread_launch, _rows(d_out), position, weights, y if ctx.needs_input_grad[1] else None,
-                                ctx.needs_input_grad[0])
+    d_y, d_weights = _on_device(d_out, _spread_launch, _rows(d_out), position.contiguous(), weights.contiguous(),
+                                y.contiguous() if ctx.needs_input_grad[1] else None, ctx.needs_input_grad[0])
     return d_y, d_weights, None
 
 

@@ -53,3 +53,18 @@ def test_grouped(cuda, hooks, k, n, layout, act):
     return torch.autograd.grad(y, leaves, dy)
 
   _same(step, hooks, 2.0 ** -7 if layout == "kn" else 0.0)
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+@pytest.mark.parametrize("rows,d", [(37, 64), (300, 65)])
+def test_routing(cuda, hooks, rows, d):
+  from faster_weathernext import experts
+  r = _randn(rows)
+  x, y, logits, d_rows, d_out = r(rows, d), r(rows * 3, d), r(rows, 7), r(rows * 3, d), r(rows, d)
+
+  def step():
+    leaves = [t.detach().requires_grad_() for t in (x, y, logits)]
+    routing = experts.route(leaves[2], 3)
+    return torch.autograd.grad((experts.dispatch(leaves[0], routing), experts.combine(leaves[1], routing)), leaves, (d_rows, d_out))
+
+  _same(step, hooks)
