@@ -216,7 +216,7 @@ class _BranchNorm(torch.autograd.Function):
     need = ctx.needs_input_grad
     d = x.shape[-1]
     x2, xs, y2, ys = _wide_or_plain(d, x, y)
-    pw2, w2, gate2, dh, ds = _plain(pw), _plain(w), _plain(gate), _plain(dh), _plain(ds)
+    pw2, w2, gate2, rstd, dh, ds = _plain(pw), _plain(w), _plain(gate), _plain(rstd), _plain(dh), _plain(ds)
     dx, dy, dpw, dw, dgate = [t.new_empty(t.shape) if wanted else None for t, wanted in zip((x, y, pw, w, gate), need)]
     if need[4] and x.numel() == 0:
       dgate.zero_()

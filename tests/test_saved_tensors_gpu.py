@@ -68,3 +68,21 @@ def test_routing(cuda, hooks, rows, d):
     return torch.autograd.grad((experts.dispatch(leaves[0], routing), experts.combine(leaves[1], routing)), leaves, (d_rows, d_out))
 
   _same(step, hooks)
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+@pytest.mark.parametrize("d", [72, 333])
+def test_branch(cuda, hooks, d):
+  from faster_weathernext import branch
+  r = _randn(d)
+  wide, y, pw, w, gate = r(33, d + 88), r(33, d).to(BF16), r(d), r(d).to(BF16), r(33, d)
+  dh, ds = r(33, d).to(BF16), r(33, d)
+  seed = torch.tensor([77], dtype=torch.int64, device="cuda")
+
+  def step():
+    leaves = [t.detach().requires_grad_() for t in (wide, y, pw, w, gate)]
+    h, s = branch.branch_norm(leaves[0][:, 8:8 + d], *leaves[1:4], gate=leaves[4], p=0.25, seed=seed)
+    dropped = branch.dropout(leaves[1], 0.5, seed, site=1)
+    return torch.autograd.grad((h, s, dropped), leaves, (dh, ds, dh))
+
+  _same(step, hooks)
