@@ -335,7 +335,7 @@ class _Linear(torch.autograd.Function):
       d_b = torch.zeros_like(bias) if need_b else None
     elif need_a or need_w or need_b:
       _first_order("linear")
-      d_a, d_w, d_b = _on_device(a, _Linear._launch, a, weight, bias, ctx.act,
+      d_a, d_w, d_b = _on_device(a, _Linear._launch, a, weight, None if bias is None else bias.contiguous(), ctx.act,
                                  _rows(dy if dy.dim() == 2 else dy.reshape(a.shape[0], -1)), need_a, need_w, need_b)
       if need_a and len(ctx.shape) != 2:
         d_a = d_a.view(ctx.shape)

@@ -86,3 +86,20 @@ def test_branch(cuda, hooks, d):
     return torch.autograd.grad((h, s, dropped), leaves, (dh, ds, dh))
 
   _same(step, hooks)
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+@pytest.mark.parametrize("k,n", [(64, 48), (65, 33)])
+def test_projection(cuda, hooks, k, n):
+  from faster_weathernext import projection
+  r = _randn(n)
+  x, w, b, nw, a = r(90, k), (r(n, k) * k ** -0.5).to(BF16), r(n), r(k), r(90, k)
+  dy, ds = r(90, n).to(BF16), r(90, k)
+
+  def step():
+    leaves = [t.detach().requires_grad_() for t in (x, w, b, nw, a)]
+    h, s = projection.rms_norm(leaves[0], leaves[3], residual=leaves[4])
+    y = projection.linear(h, leaves[1], leaves[2], activation="gelu")
+    return torch.autograd.grad((y, s), leaves, (dy, ds))
+
+  _same(step, hooks)
