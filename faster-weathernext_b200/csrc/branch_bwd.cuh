@@ -12,6 +12,10 @@
 // in order by branch_bwd_finish: no atomics, the same bits every time. Measured at 163,848 x 512, float32 stream, bf16 branch
 // (of the measured copy rate): 230 us (1.00), with dropout 245 (0.94; bf16 stream 206, 0.75), and 7 for the sums; 40,962 x
 // 2,048 233 (0.99); 163,848 x 333 247 (0.61).
+//
+// The gradient of s alone (no dh, G = none_t) does not depend on s: dt = ds, and x and rstd(s), which may hold anything then,
+// take no part. A kernel of its own: a condition in the loop cost the other up to 29 % (163,848 x 512 230 -> 240 us, bf16
+// stream with dropout 206 -> 245, 20,481 x 4,096 264 -> 339).
 #pragma once
 
 #include "branch_rows.cuh"
@@ -41,9 +45,11 @@ cudaError_t branch_bwd_width(int room, F f) {
 constexpr int branch_bwd_resident(int maxt) { return maxt > 512 ? maxt : 512; }  // threads of an SM
 __host__ __device__ constexpr int branch_bwd_threads(int tpr, int maxt, int room) { return tpr > 0 ? maxt : (room + 255) / 256 * 32; }
 
+// G: dh's type, none_t without one.
 template <class X, class Y, class G, int TPR, int MAXT, int MODE>
 __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch_bwd_kernel(const BranchBwdParams p) {
   constexpr int GROUPS = groups_of<TPR>(), PER_WARP = per_warp<TPR>();
+  constexpr bool NORMED = !is_none<G>;
   extern __shared__ float part_smem[];  // more than one group: a row of d each
   __shared__ __align__(16) float red[2][32];
   clear_red<TPR>(red);
@@ -82,24 +88,23 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
     const Cut<MODE> cut(j, d);
     Raw<X, 8> nx, nds;
     Raw<Y, 8> ny;
-    Raw<G, 8> ng;
+    Raw<std::conditional_t<NORMED, G, bf16>, 8> ng;
     float2 nr;
     auto fetch = [&](int64_t r) {
       const int n = r < end ? d : 0;  // a row that is not there adds nothing
       nr = n > 0 ? __ldg(reinterpret_cast<const float2*>(p.rstd) + r) : make_float2(0.f, 0.f);
       const X *x = static_cast<const X*>(p.x) + r * p.x_stride, *ds = static_cast<const X*>(p.ds) + r * d;
       const Y* y = static_cast<const Y*>(p.y) + r * p.y_stride;
-      const G* dh = static_cast<const G*>(p.dh) + r * d;
       if constexpr (MODE == kWide) {
-        grab<MODE>(x, j, n, true, nx);
+        if constexpr (NORMED) grab<MODE>(x, j, n, true, nx);
         grab<MODE>(y, j, n, true, ny);
-        grab<MODE>(dh, j, p.dh != nullptr ? n : 0, true, ng);
+        if constexpr (NORMED) grab<MODE>(static_cast<const G*>(p.dh) + r * d, j, n, true, ng);
         grab<MODE>(ds, j, p.ds != nullptr ? n : 0, true, nds);
       } else {
         const bool there = n > 0, all = r < whole;
-        grab_shifted(x, j, d, there, all, nx);
+        if constexpr (NORMED) grab_shifted(x, j, d, there, all, nx);
         grab_shifted(y, j, d, there, all, ny);
-        grab_shifted(dh, j, d, there && p.dh != nullptr, all, ng);
+        if constexpr (NORMED) grab_shifted(static_cast<const G*>(p.dh) + r * d, j, d, there, all, ng);
         grab_shifted(ds, j, d, there && p.ds != nullptr, all, nds);
       }
     };
@@ -119,15 +124,22 @@ __global__ void __launch_bounds__(MAXT, branch_bwd_resident(MAXT) / MAXT) branch
         words = drop_words(p.drop, seed, static_cast<uint64_t>(row * d + j) >> 3);
         b = kept(b, words, least);
       }
-      const V8 sh = mul(fma(values(nx, cut), p.alpha, b), r2);
-      V8 g = values(ng, cut), dt = values(nds, cut);
+      V8 g, sh, dt = values(nds, cut);
+      if constexpr (NORMED) {
+        sh = mul(fma(values(nx, cut), p.alpha, b), r2);
+        g = values(ng, cut);
+      }
       if (row + step - group % PER_WARP < end) fetch(row + step);
-      dw = fma(g, sh, dw);
-      g = mul(g, w);
       float2 acc = make_float2(0.f, 0.f);
-      dot(acc, g, sh);
-      const float c1 = -over_row<TPR, false>(acc.x + acc.y, red[0]) * over;
-      dt = fma(fma(sh, c1, g), r2, dt);
+      if constexpr (NORMED) {
+        dw = fma(g, sh, dw);
+        g = mul(g, w);
+        dot(acc, g, sh);
+        const float c1 = -over_row<TPR, false>(acc.x + acc.y, red[0]) * over;
+        dt = fma(fma(sh, c1, g), r2, dt);
+      } else if constexpr (TPR == 0) {
+        __syncthreads();  // red[1] was read, which the other reduction's barrier orders otherwise
+      }
       if (p.dx != nullptr) put<MODE>(static_cast<X*>(p.dx) + row * d, j, n, mul(dt, p.alpha));
       if (drops) dt = kept(dt, words, least);
       g = mul(dt, a);
@@ -166,6 +178,7 @@ cudaError_t go_branch_bwd(const BranchBwdParams& p, cudaStream_t st) {
 }
 template <class X, class Y>
 cudaError_t branch_bwd_by(const BranchBwdParams& p, cudaStream_t st) {
+  if (p.dh == nullptr) return p.wide ? go_branch_bwd<X, Y, none_t, kWide>(p, st) : go_branch_bwd<X, Y, none_t, kShift>(p, st);
   if (p.dh_bf16) return p.wide ? go_branch_bwd<X, Y, bf16, kWide>(p, st) : go_branch_bwd<X, Y, bf16, kShift>(p, st);
   return p.wide ? go_branch_bwd<X, Y, float, kWide>(p, st) : go_branch_bwd<X, Y, float, kShift>(p, st);
 }

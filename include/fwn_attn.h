@@ -425,8 +425,9 @@ FWN_API fwn_status fwn_branch_norm(const fwn_branch_desc* desc, const void* x, c
                                    void* stream);
 
 /* Backward: the forward's inputs and rstd, dh [rows, d] (out_dtype) and ds [rows, d] (x_dtype), the gradients of h and s,
- * either NULL (none). dx, dy, d_post_weight, d_weight, d_gate as the tensors they belong to, each NULL (not computed).
- * Deterministic. workspace: fwn_branch_norm_bwd_workspace_size bytes, 16-byte aligned (0 bytes: may be NULL). */
+ * either NULL (none; without dh the gradients do not depend on x and rstd(s), whatever these hold, and d_weight is 0). dx, dy,
+ * d_post_weight, d_weight, d_gate as the tensors they belong to, each NULL (not computed). Deterministic. workspace:
+ * fwn_branch_norm_bwd_workspace_size bytes, 16-byte aligned (0 bytes: may be NULL). */
 FWN_API fwn_status fwn_branch_norm_bwd_workspace_size(const fwn_branch_desc* desc, size_t* bytes);
 FWN_API fwn_status fwn_branch_norm_bwd(const fwn_branch_desc* desc, const void* x, const void* y, const void* post_weight,
                                        const void* weight, const void* gate, const float* rstd, const void* dh,
