@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(1024) group_setup_kernel(const GroupSetup s, c
 #pragma unroll
     for (int q = 0; q < kGroupFirsts; ++q) {
       if (s.first[q] == nullptr) continue;
-      const int tiles = t < s.groups ? (s.unit[q] > 0 ? (rows + s.unit[q] - 1) / s.unit[q] : 1) : 0;
+      const int tiles = t < s.groups ? group_tiles(rows, s.unit[q]) : 0;
       const int upto = scan(tiles, false, (q + 1) & 1);
       if (t < s.groups) s.first[q][t] = upto - tiles;
       if (t == s.groups) s.first[q][t] = upto;  // tiles is 0 here

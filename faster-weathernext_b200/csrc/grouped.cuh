@@ -8,6 +8,10 @@ namespace fwn {
 constexpr int kGroupsMax = 1023;
 constexpr int kGroupMaps = 7, kGroupFirsts = 3;
 
+// Tiles (or runs) of `unit` rows that an expert's rows take; unit 0: one run, whatever they are. Without rows + unit, which may
+// pass 2^31: a run of the weights' gradient takes millions of rows where few columns make few tiles.
+constexpr int group_tiles(int rows, int unit) { return unit > 0 ? rows / unit + (rows % unit != 0 ? 1 : 0) : 1; }
+
 // What a call's kernels read of the offsets, made on the device by one launch before them: the offsets in order and within
 // the tensor, the tiles (or runs) before each expert, the experts' tensor maps, and zeros in the rows of no expert.
 struct GroupSetup {
