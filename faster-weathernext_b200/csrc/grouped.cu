@@ -99,15 +99,12 @@ __global__ void __launch_bounds__(1024) group_setup_kernel(const GroupSetup s, c
     asm volatile("tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned [%0], [%1], 128;"
                  ::"l"(reinterpret_cast<uint64_t>(s.maps + i)), "r"(at)
                  : "memory");
-  } else {
+  } else {  // launched where there is a tensor to clear
     const int first = end_before(s.given, 0, s.m), last = end_before(s.given, s.groups, s.m);
     const int block = blockIdx.x - 1 - map_blocks;
-    for (int q = 0; q < 2; ++q) {
-      if (s.clear[q] == nullptr) continue;
-      uint8_t* p = static_cast<uint8_t*>(s.clear[q]);
-      clear_bytes(p, 0, first * s.clear_row[q], block, kClearBlocks);
-      clear_bytes(p, last * s.clear_row[q], s.m * s.clear_row[q], block, kClearBlocks);
-    }
+    uint8_t* p = static_cast<uint8_t*>(s.clear);
+    clear_bytes(p, 0, first * s.clear_row, block, kClearBlocks);
+    clear_bytes(p, last * s.clear_row, s.m * s.clear_row, block, kClearBlocks);
   }
 }
 
@@ -366,8 +363,7 @@ __global__ void __launch_bounds__(128) grouped_run_sum_kernel(const float* __res
 
 cudaError_t launch_group_setup(const GroupSetup& s, const GroupMaps& maps, cudaStream_t st) {
   const int map_blocks = (s.n_maps * s.groups + 31) / 32;
-  const bool clears = s.clear[0] != nullptr || s.clear[1] != nullptr;
-  group_setup_kernel<<<1 + map_blocks + (clears ? kClearBlocks : 0), 1024, 0, st>>>(s, maps, map_blocks);
+  group_setup_kernel<<<1 + map_blocks + (s.clear != nullptr ? kClearBlocks : 0), 1024, 0, st>>>(s, maps, map_blocks);
   return cudaGetLastError();
 }
 

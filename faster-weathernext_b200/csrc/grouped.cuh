@@ -1,4 +1,4 @@
-// Launch interface of the products grouped by expert (grouped_fwd.cu, grouped_bwd.cu, grouped.cu), called by experts_abi.cu.
+// Launch interface of the products grouped by expert (grouped_fwd.cu, grouped_bwd.cu, grouped.cu), called by grouped_abi.cu.
 #pragma once
 
 #include "linear.cuh"
@@ -23,8 +23,8 @@ struct GroupSetup {
   int unit[kGroupFirsts];    // rows of a tile (or run); 0: one run an expert, whatever its rows
   CUtensorMap* maps;         // [n_maps, groups]
   int n_maps;
-  void* clear[2];            // tensors of m contiguous rows of clear_row bytes whose rows of no expert become 0; or null
-  int64_t clear_row[2];
+  void* clear;               // m contiguous rows of clear_row bytes whose rows of no expert become 0; or null
+  int64_t clear_row;
 };
 struct GroupMaps {
   CUtensorMap map[kGroupMaps];    // over all rows: the experts' copies end at their last

@@ -259,8 +259,8 @@ fwn_status fwn_linear_grouped(const fwn_grouped_desc* desc, const void* a, const
   g.unit[0] = tm;
   g.maps = reinterpret_cast<CUtensorMap*>(ws + pl.maps);
   g.n_maps = p.out_direct ? 1 : 2;
-  g.clear[0] = out;
-  g.clear_row[0] = d.n * es;
+  g.clear = out;
+  g.clear_row = d.n * es;
   if ((e = launch_group_setup(g, maps, st)) != cudaSuccess) return abi_cuda_fail(e, "experts' maps");
   GroupParams gp{};
   gp.offsets = g.offsets;
@@ -336,8 +336,8 @@ fwn_status fwn_linear_grouped_bwd(const fwn_grouped_desc* desc, const void* a, c
   g.unit[2] = pl.w.run * 64;
   g.maps = reinterpret_cast<CUtensorMap*>(ws + pl.maps);
   g.n_maps = kGroupMaps;
-  g.clear[0] = d_a;
-  g.clear_row[0] = 2ll * d.k;
+  g.clear = d_a;
+  g.clear_row = 2ll * d.k;
   if ((e = launch_group_setup(g, maps, st)) != cudaSuccess) return abi_cuda_fail(e, "experts' maps");
   auto map_of = [&](int i) { return g.maps + static_cast<int64_t>(i) * d.groups; };
   GroupParams gp{};
