@@ -501,6 +501,7 @@ def attention_backward(q, k, v, o, lse, do, tiles: AttentionTiles, scale: float,
   lib = _lib.lib()
   q, k, v = _canon(q, k, v)
   o, do = _canon(o.contiguous(), do.contiguous())
+  lse = lse.contiguous()
   if dqkv is not None:
     dq, dk, dv = dqkv[:, :, :, 0], dqkv[:, :, :, 1], dqkv[:, :, :, 2]
     desc = _desc(q, o, scale, mode, grad=dq)

@@ -103,3 +103,46 @@ def test_projection(cuda, hooks, k, n):
     return torch.autograd.grad((y, s), leaves, (dy, ds))
 
   _same(step, hooks)
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+@pytest.mark.parametrize("fused", [False, True])
+def test_attention(cuda, hooks, fused):
+  from faster_weathernext import mesh, tiled_attn
+  mask, _, _ = mesh.config_mask(1)
+  tiles = tiled_attn.AttentionTiles.from_mask(mask, device=cuda)
+  r = _randn(4)
+  qkv, dy = r(1, mask.shape[0], 2, 3, 64).to(BF16), r(1, mask.shape[0], 2, 64).to(BF16)
+
+  def step():
+    leaf = qkv.detach().requires_grad_()
+    if fused:
+      y = tiled_attn.attention_qkv(leaf, tiles, scale=0.125)
+    else:
+      y = tiled_attn.attention(*leaf.unbind(3), tiles, scale=0.125)
+    return torch.autograd.grad(y, leaf, dy)
+
+  _same(step, hooks)
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+def test_expert_processor(cuda, hooks):
+  """A training step of the operators together, at an odd width of the experts' MLPs. Transposed weights come back the other way
+  round, so that products may be summed in another order: each run is within the processor's bound for gradients of bf16
+  products, 5e-2 of their norm, and so are the two of each other."""
+  from faster_weathernext import mesh, tiled_attn
+  from faster_weathernext.expert_processor import ExpertProcessor
+  from faster_weathernext.processor import ProcessorConfig
+  cfg = ProcessorConfig(layers=2, d_model=128, heads=2, head_dim=64, mlp_hidden=251, cond_dim=8)
+  mask, _, _ = mesh.config_mask(1)
+  r = _randn(1)
+  model = ExpertProcessor(cfg, seed=3, device=cuda, dropout=0.1)
+  x, cond, dy = r(1, mask.shape[0], 128), r(1, 8), r(1, mask.shape[0], 128)
+  tiles = tiled_attn.AttentionTiles.from_mask(mask, device=cuda)
+  leaves = [x.requires_grad_(), *model.parameters()]
+  step = lambda: torch.autograd.grad(model(x, tiles, cond, seed=5), leaves, dy)  # noqa: E731
+  want = step()
+  with HOOKS[hooks]():
+    got = step()
+  for a, b in zip(got, want):
+    assert (a.double() - b.double()).norm() <= 5e-2 * b.double().norm()
