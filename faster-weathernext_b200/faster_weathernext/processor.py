@@ -86,7 +86,7 @@ class _CondNorm(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, *grads):
-    xn, so = ctx.saved_tensors
+    xn, so = (t.contiguous() for t in ctx.saved_tensors)  # hooks may bring them back with strides
     g_xn, g_h = (grads[0], grads[1]) if ctx.has_a else (None, grads[0])
     m, d = xn.shape
     if g_h is None:
@@ -141,7 +141,7 @@ class _GeluMLP(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, d_out):
-    h, pre, act, w1t, w2h = ctx.saved_tensors
+    h, pre, act, w1t, w2h = (t.contiguous() for t in ctx.saved_tensors)
     lib = _lib.lib()
     m, hidden = pre.shape
     d = h.shape[1]

@@ -146,3 +146,21 @@ def test_expert_processor(cuda, hooks):
     got = step()
   for a, b in zip(got, want):
     assert (a.double() - b.double()).norm() <= 5e-2 * b.double().norm()
+
+
+@pytest.mark.parametrize("hooks", HOOKS)
+def test_processor(cuda, hooks):
+  """The processor's own functions (torch's products around them take moved operands in another order of their sums)."""
+  from faster_weathernext import processor
+  r = _randn(2)
+  x, a, so, dx, dh = r(84, 128), r(84, 128).to(BF16), r(2, 256), r(84, 128), r(84, 128).to(BF16)
+  w1, b1, w2, b2 = r(128, 256) * 0.1, r(256), r(256, 128) * 0.1, r(128)
+
+  def step():
+    leaves = [t.detach().requires_grad_() for t in (x, a, so, w1, b1, w2, b2)]
+    added, h = processor._CondNorm.apply(*leaves[:3], 42, BF16)
+    first = processor._CondNorm.apply(leaves[0], None, leaves[2], 42, F32)
+    y = processor._GeluMLP.apply(h, *leaves[3:])
+    return torch.autograd.grad((added, y, first), leaves, (dx, dh, dx))
+
+  _same(step, hooks)
