@@ -32,7 +32,8 @@ _BF16, _F32 = torch.bfloat16, torch.float32
 @dataclasses.dataclass
 class ExpertPlan:
   """The weights of a forecast, laid out once: bf16 tensors with rows along the summed dimension, q / k / v optionally as
-  (e4m3 values, scales); norms, biases and gates float32. Holds copies: build it again after the weights change."""
+  (e4m3 values, scales); norms, biases and gates float32. Holds copies: build it again after the weights change. Rows are as
+  long as their dimension: those off multiples of 8 (an odd mlp_hidden) are laid out again by every product."""
   eight_bit: bool
   blocks: list
   norm_first: torch.Tensor
